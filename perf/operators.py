@@ -181,7 +181,7 @@ def _prepare_attention(case, seed):
     q = torch.randn(tokens, q_dim, generator=g, device="cuda") * 1.5
     key = torch.randn(n_pages, P, kv_dim, generator=g, device="cuda").to(_cache_type(case))
     value = torch.randn(n_pages, P, kv_dim, generator=g, device="cuda").to(_cache_type(case))
-    # (host copies of the lengths' maxima: what a server that made the lengths knows; the plain form pads to them)
+    # (host copies of the lengths' maxima: what a server that made the lengths knows)
     return dict(q=q, key_cache=key, value_cache=value, table=table.cuda(), row_start=row_start.cuda(), kv_len=kv.to(torch.int32).cuda(), out=torch.zeros(tokens, q_dim, device="cuda"),
                 longest_new=int(new.max()), longest_kv=int(kv.max()))
 
@@ -231,7 +231,7 @@ def _own_append(s):
 def _own_attention(s):
     from inferi_b200.ops import PagedAttention, PagedAttentionConfig
     c = s["case"]
-    PagedAttention(backend()).launch(PagedAttentionConfig(c["heads"], c["mul"], c["hs"], c["window"], c["sinks"]), s["q"], s["key_cache"], s["value_cache"], s["table"], s["row_start"], s["kv_len"], s["out"])
+    PagedAttention(backend()).launch(PagedAttentionConfig(c["heads"], c["mul"], c["hs"], c["window"], c["sinks"], s["longest_new"]), s["q"], s["key_cache"], s["value_cache"], s["table"], s["row_start"], s["kv_len"], s["out"])
     return s["out"]
 
 
