@@ -41,29 +41,29 @@ def listed():
     att = dict(kind="attention", page=16, window=0, sinks=0, pad=0, kv="f16")
     return [
         # a decode step of a small server: sixteen requests, one token each
-        dict(name="plan, 16 decoding", kind="plan", requests=16, page=16, longest=2000, chunk=0, ended=0.1, short=False),
+        dict(name="plan 16 decoding", kind="plan", requests=16, page=16, longest=2000, chunk=0, ended=0.1, short=False),
         # a step of a large one: prompts' chunks between decoding requests, some of which have ended, and fewer free pages than are asked for
-        dict(name="plan, 2000 mixed", kind="plan", requests=2000, page=32, longest=8000, chunk=256, ended=0.05, short=True),
+        dict(name="plan 2000 mixed", kind="plan", requests=2000, page=32, longest=8000, chunk=256, ended=0.05, short=True),
         # a decode step's keys and values, 1B heads
-        dict(name="append, 64 tokens", kind="append", tokens=64, heads=32, mul=4, hs=64, page=16, variant=ORIGINAL, far=4000, pad=0, kv="f16"),
+        dict(name="append 64 tokens", kind="append", tokens=64, heads=32, mul=4, hs=64, page=16, variant=ORIGINAL, far=4000, pad=0, kv="f16"),
         # chunks of prompts at far positions, 8B heads
-        dict(name="append, 8001 tokens", kind="append", tokens=8001, heads=32, mul=4, hs=128, page=64, variant=NEOX, far=120000, pad=191, kv="f16"),
+        dict(name="append 8001 tokens", kind="append", tokens=8001, heads=32, mul=4, hs=128, page=64, variant=NEOX, far=120000, pad=191, kv="f16"),
         # one request decoding, 1B heads: latency
-        dict(att, name="decode, 1 of 500", requests=1, new=1, same=True, cached=500, heads=32, mul=4, hs=64),
+        dict(att, name="decode 1 of 500", requests=1, new=1, same=True, cached=500, heads=32, mul=4, hs=64),
         # a ragged decode batch, 8B heads: the cache's bytes count
-        dict(att, name="decode, 64 up to 8000", requests=64, new=1, same=True, cached=8000, heads=32, mul=4, hs=128, pad=3),
+        dict(att, name="decode 64 up to 8000", requests=64, new=1, same=True, cached=8000, heads=32, mul=4, hs=128, pad=3),
         # a chunk of a long prompt behind what is cached already, 8B heads
-        dict(att, name="chunk, 1000 after 15000", requests=1, new=1000, same=True, cached=15000, heads=32, mul=4, hs=128, page=64),
+        dict(att, name="chunk 1000 after 15000", requests=1, new=1000, same=True, cached=15000, heads=32, mul=4, hs=128, page=64),
         # several prompts of a batch together, with the window that a model with a sliding window has, 1B heads
-        dict(att, name="chunks, window and sinks", requests=7, new=700, same=False, cached=5000, heads=32, mul=4, hs=64, page=32, window=1024, sinks=4, pad=55),
+        dict(att, name="chunks window and sinks", requests=7, new=700, same=False, cached=5000, heads=32, mul=4, hs=64, page=32, window=1024, sinks=4, pad=55),
         # a few proposed tokens per request to be verified, 32-bit cache
-        dict(att, name="verify, 32-bit cache", requests=24, new=5, same=False, cached=3000, heads=32, mul=8, hs=128, kv="f32"),
+        dict(att, name="verify 32-bit cache", requests=24, new=5, same=False, cached=3000, heads=32, mul=8, hs=128, kv="f32"),
         # one row of an 8B vocabulary: latency
-        dict(name="sample, 1 row", kind="sample", rows=1, vocab=128256, sharp=3.0, filters="top-p"),
+        dict(name="sample 1 row", kind="sample", rows=1, vocab=128256, sharp=3.0, filters="top-p"),
         # a batch with settings of every request's own
-        dict(name="sample, 250 rows", kind="sample", rows=250, vocab=128256, sharp=3.0, filters="mixed"),
+        dict(name="sample 250 rows", kind="sample", rows=250, vocab=128256, sharp=3.0, filters="mixed"),
         # a smaller vocabulary, hot: long tails are kept
-        dict(name="sample, 33 rows hot", kind="sample", rows=33, vocab=32003, sharp=0.7, filters="mixed"),
+        dict(name="sample 33 rows hot", kind="sample", rows=33, vocab=32003, sharp=0.7, filters="mixed"),
     ]
 
 
