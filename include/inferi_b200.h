@@ -167,6 +167,82 @@ IB_API int32_t ib_argmax(ib_ctx *ctx, void *stream, const float *logits_dev, uin
 IB_API int32_t ib_sample(ib_ctx *ctx, void *stream, const float *logits_dev, uint32_t n, float temperature, float topp, float coin,
                          uint32_t *out_dev);
 
+/* ---- a batch of requests over a paged cache ----
+ * No counterpart in the reference, which holds one sequence in a contiguous cache.  The cache of a layer is n_pages pages of page_size rows of
+ * [kv_dim] for K and as many for V; a request's row of the block table names its pages in the order of its positions: position j of request r
+ * is row j % page_size of page block_table[r][j / page_size].  A slot is page * page_size + row.  One step of a server is ib_page_plan, then for every
+ * layer ib_paged_append and ib_paged_attention, then ib_sample_batch.  Lengths, tables and settings stay on the device: the host has to
+ * know only how many requests and rows there are room for, so a step can be captured once and replayed for others of that size.
+ * The scratch that some of these calls need is the context's, of a size that does not depend on the arguments; it is made by the first call of its
+ * kind, also while a stream is being captured, and never moved.  Calls whose kernels may overlap on the GPU (two streams, graphs that are replayed side by side) need a context each. */
+
+/* Sizes of a cache.  page_size: a power of two from 16 to 1024.  page_stride: elements from a page to the next one, at least page_size * kv_dim (more
+ * where K's and V's pages lie in turn); it and kv_dim times the element size are multiples of 16 bytes, and both caches start on 16-byte boundaries. */
+typedef struct ib_paged_cache {
+    void *k_dev, *v_dev;
+    uint64_t page_stride;
+    uint32_t n_pages, page_size;   /* n_pages * page_size < 2^31 */
+    uint32_t kv_dim;
+    int32_t kv_dtype;
+} ib_paged_cache;
+
+/* Block tables and slot maps of a step, from the requests' lengths.  All arrays are int32 on the device:
+ *   cached_len[n_requests]   positions of the request that are in the cache
+ *   new_len[n_requests]      tokens that this step adds; negative: the request has ended
+ *   block_table[n_requests][max_pages]   in: the pages of the cached positions; out: also those of the new ones (other entries stay)
+ *   free_pages[n_pages], n_free[1]       the free pages, a stack: entries 0 .. n_free - 1
+ *   kv_len[n_requests], n_free_out[1]    cached_len and n_free of the next step (may be the same arrays as those)
+ *   row_start[n_requests + 1]            first row of each request among the step's tokens, and their number
+ *   positions[max_tokens], slots[max_tokens]   of the step's tokens, request by request; rows behind the last one get position 0 and slot -1
+ *   status[n_requests]       IB_PLAN_*
+ * The pages of ended requests go on top of the stack, by requests and positions, and their kv_len is 0.  Then pages are taken from its top in the order of
+ * the requests.  A request that does not fit is left as it is, without tokens in this step, and its status says why: a cached_len below 0 or beyond its
+ * row of the table (INVALID; kv_len 0, and it returns no pages), a table row too short for the new tokens (TABLE_FULL), more tokens than max_tokens together with the requests before it
+ * (NO_ROOM), more pages than are free together with those before it (NO_PAGES); once one does not fit, none behind it that needs the same does.  A page
+ * belongs to one request.  A page number outside the cache is never followed: its slots are -1.
+ * n_requests <= 8192. */
+enum { IB_PLAN_OK = 0, IB_PLAN_NO_PAGES = 1, IB_PLAN_TABLE_FULL = 2, IB_PLAN_NO_ROOM = 3, IB_PLAN_INVALID = 4 };
+typedef struct ib_page_plan_args {
+    uint32_t n_requests, max_pages, max_tokens, n_pages, page_size;
+    const int32_t *cached_len, *new_len, *n_free;
+    int32_t *block_table, *free_pages;
+    int32_t *kv_len, *row_start, *positions, *slots, *n_free_out, *status;
+} ib_page_plan_args;
+IB_API int32_t ib_page_plan(ib_ctx *ctx, void *stream, const ib_page_plan_args *args);
+
+/* Rotation and cache append of n rows: q_out = rotation of q at the row's position, the rotation of k and v itself go to the row's slot of the cache, rounded
+ * to its type.  `variant`, head_size and base_freq as in ib_rope; the angle is the product of position and frequency in 64 bits, so far positions
+ * lose nothing.  Rows are *_stride floats apart; q_out may be q (with the same stride).  A row whose slot is outside the cache (-1: padding) is left out: neither
+ * q_out nor the cache is written.  The slots of a call differ from one another.  head_size even, up to 256, dividing q_dim and kv_dim. */
+typedef struct ib_paged_append_args {
+    const float *q_dev, *k_dev, *v_dev;
+    float *q_out_dev;
+    uint64_t q_stride, k_stride, v_stride, q_out_stride;
+    const int32_t *positions, *slots;
+    uint32_t n, q_dim, head_size;
+    int32_t variant;
+    float base_freq;
+} ib_paged_append_args;
+IB_API int32_t ib_paged_append(ib_ctx *ctx, void *stream, const ib_paged_append_args *args, const ib_paged_cache *cache);
+
+/* Attention of the new tokens of n_requests requests over their pages: row row_start[r] + i of q is token i of request r's row_start[r + 1] - row_start[r]
+ * new ones, at position p = kv_len[r] - (number of new ones) + i, whose keys and values are in the cache already.  It sees the positions j <= p with
+ * p - j < window or j < sinks (window 0: all of them): out = softmax(q K^T / sqrt(head_size)) V over these, and 0 where there are none.  Head h uses kv
+ * head h / kv_mul.  head_size 64 or 128; kv_mul up to 64; kv_dim of the cache = n_heads / kv_mul * head_size.  Rows of q and out are *_stride floats apart; rows
+ * behind row_start[n_requests] are neither read nor written.  Masked positions and rows of pages behind kv_len may hold anything, infinities and NaN too.
+ * A page number outside the cache is never followed; what the rows of that request get then is not specified.
+ * longest_new: the most new tokens that a request has, where the host knows it, else 0.  It chooses kernels, and any value gives right results. */
+typedef struct ib_paged_attn_args {
+    const float *q_dev;
+    float *out_dev;
+    uint64_t q_stride, out_stride;
+    const int32_t *block_table, *row_start, *kv_len;
+    uint32_t n_requests, n_tokens, max_pages;   /* n_tokens: rows of q and out */
+    uint32_t n_heads, kv_mul, head_size;
+    uint32_t window, sinks, longest_new;
+} ib_paged_attn_args;
+IB_API int32_t ib_paged_attention(ib_ctx *ctx, void *stream, const ib_paged_attn_args *args, const ib_paged_cache *cache);
+
 /* = `Llama2Config` (crates/inferi/src/models/llama2/cpu.rs:46-66). */
 typedef struct ib_llama_config {
     uint32_t hidden_size;

@@ -29,6 +29,31 @@ class AttnParams(C.Structure):
     _fields_ = [(n, C.c_uint32) for n in ("seq_len", "kv_dim", "kv_mul", "n_heads", "head_size", "pos")]
 
 
+class PagedCache(C.Structure):
+    """= ib_paged_cache"""
+    _fields_ = [("k_dev", C.c_void_p), ("v_dev", C.c_void_p), ("page_stride", C.c_uint64), ("n_pages", C.c_uint32), ("page_size", C.c_uint32), ("kv_dim", C.c_uint32),
+                ("kv_dtype", C.c_int32)]
+
+
+class PagePlanArgs(C.Structure):
+    """= ib_page_plan_args"""
+    _fields_ = [(n, C.c_uint32) for n in ("n_requests", "max_pages", "max_tokens", "n_pages", "page_size")] + [
+        (n, C.c_void_p) for n in ("cached_len", "new_len", "n_free", "block_table", "free_pages", "kv_len", "row_start", "positions", "slots", "n_free_out", "status")]
+
+
+class PagedAppendArgs(C.Structure):
+    """= ib_paged_append_args"""
+    _fields_ = [(n, C.c_void_p) for n in ("q_dev", "k_dev", "v_dev", "q_out_dev")] + [(n, C.c_uint64) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride")] + [
+        (n, C.c_void_p) for n in ("positions", "slots")] + [(n, C.c_uint32) for n in ("n", "q_dim", "head_size")] + [("variant", C.c_int32), ("base_freq", C.c_float)]
+
+
+class PagedAttnArgs(C.Structure):
+    """= ib_paged_attn_args"""
+    _fields_ = [(n, C.c_void_p) for n in ("q_dev", "out_dev")] + [(n, C.c_uint64) for n in ("q_stride", "out_stride")] + [
+        (n, C.c_void_p) for n in ("block_table", "row_start", "kv_len")] + [
+        (n, C.c_uint32) for n in ("n_requests", "n_tokens", "max_pages", "n_heads", "kv_mul", "head_size", "window", "sinks", "longest_new")]
+
+
 class LlamaConfig(C.Structure):
     """= Llama2Config (crates/inferi/src/models/llama2/cpu.rs:46-66)."""
     _fields_ = [(n, C.c_uint32) for n in ("hidden_size", "intermediate_size", "num_hidden_layers", "num_attention_heads",
@@ -82,6 +107,9 @@ SIGNATURES = {
     "ib_attention_static": (_i32, [_vp, C.POINTER(AttnParams), _vp, _vp, _vp, _i32, _vp]),
     "ib_argmax": (_i32, [_vp, _vp, _vp, _u32, _vp]),
     "ib_sample": (_i32, [_vp, _vp, _vp, _u32, _f, _f, _f, _vp]),
+    "ib_page_plan": (_i32, [_vp, _vp, C.POINTER(PagePlanArgs)]),
+    "ib_paged_append": (_i32, [_vp, _vp, C.POINTER(PagedAppendArgs), C.POINTER(PagedCache)]),
+    "ib_paged_attention": (_i32, [_vp, _vp, C.POINTER(PagedAttnArgs), C.POINTER(PagedCache)]),
     "ib_llama_set_sampler": (_i32, [_vp, _f, _f, _u64]),
     "ib_llama_generate_until": (_i32, [_vp, _vp, _vp, _u32, _u32, _u32, _u32, _vp, C.POINTER(_u32)]),
     "ib_llama_chat": (_i32, [_vp, _vp, _vp, _u32, _u32, _u32, _u32, TOKEN_EVENT_FN, _vp, C.POINTER(_u32)]),

@@ -20,19 +20,6 @@ int32_t set_error(int32_t code, const char *fmt, ...) {
     return code;
 }
 
-struct DeviceGuard {
-    int prev = -1;
-    bool ok = true;
-    explicit DeviceGuard(int dev) {
-        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-        if (prev != dev) ok = (cudaSetDevice(dev) == cudaSuccess);
-    }
-    ~DeviceGuard() {
-        int cur = -1;
-        if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
-    }
-};
-
 int32_t check_device_error(ib_ctx *ctx) {
     const uint32_t e = *(volatile uint32_t *)ctx->err_host;
     if (e == 0) return IB_OK;
@@ -65,13 +52,6 @@ void host_populate(void *p, size_t nbytes) {
     constexpr int POPULATE_WRITE = 23;   // MADV_POPULATE_WRITE
     madvise((void *)a, (uintptr_t)p + nbytes - a, POPULATE_WRITE);
 }
-// What the calling thread does between these is not held against a capture that another stream of the process is in (its capture mode would refuse it, and end the
-// capture).
-struct BesideCaptures {
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    BesideCaptures() { cudaThreadExchangeStreamCaptureMode(&mode); }
-    ~BesideCaptures() { cudaThreadExchangeStreamCaptureMode(&mode); }
-};
 static void free_staging(ib_ctx *ctx) {
     if (ctx->stage_host) cudaFreeHost(ctx->stage_host);
     ctx->stage_host = nullptr;
@@ -111,11 +91,6 @@ int32_t read_back(ib_ctx *ctx, cudaStream_t s, void *dst, const void *src, size_
 }  // namespace ib
 
 using namespace ib;
-
-#define IB_ENTER(ctx)                                                   \
-    IB_REQUIRE((ctx) != nullptr, "null context");                       \
-    ib::DeviceGuard _guard((ctx)->device);                              \
-    if (!_guard.ok) return ib::set_error(IB_ERR_CUDA, "cudaSetDevice(%d) failed", (ctx)->device)
 
 extern "C" {
 
@@ -177,6 +152,7 @@ int32_t ib_ctx_destroy(ib_ctx *ctx) {
     if (ctx->err_host) cudaFreeHost(ctx->err_host);
     if (ctx->stream_counters) cudaFree(ctx->stream_counters);
     if (ctx->tc_scratch) cudaFree(ctx->tc_scratch);
+    if (ctx->paged_scratch) cudaFree(ctx->paged_scratch);
     free_staging(ctx);
     delete ctx;
     return IB_OK;

@@ -97,6 +97,9 @@ struct ib_ctx {
     void *stage_host = nullptr;
     cudaEvent_t stage_event[ib::STAGE_PIECES - 1] = {};   // a piece has arrived
     std::mutex stage_lock;
+    // partials and arrival counters of the attention over a paged cache (paged_attention.cu), of one size whatever the calls
+    float *paged_scratch = nullptr;
+    uint32_t *paged_counters = nullptr;
     // limit of every wait inside a kernel (on a shared-memory barrier, on another rank's arrival); ib_ctx_set_wait_limit
     uint64_t wait_limit_ns = 2000000000ull;
 };
@@ -236,4 +239,31 @@ inline uint32_t attn_regime_of(const uint32_t (&limits)[3], uint64_t positions) 
     return positions <= limits[ATTN_SHORT] ? ATTN_SHORT : (positions <= limits[ATTN_MIDDLE] ? ATTN_MIDDLE : ATTN_LONG);
 }
 
+// ---- entry points ----
+struct DeviceGuard {
+    int prev = -1;
+    bool ok = true;
+    explicit DeviceGuard(int dev) {
+        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+        if (prev != dev) ok = (cudaSetDevice(dev) == cudaSuccess);
+    }
+    ~DeviceGuard() {
+        int cur = -1;
+        if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
+    }
+};
+
+// What the calling thread does between these is not held against a capture that another stream of the process is in (its capture mode would refuse it, and end the
+// capture).
+struct BesideCaptures {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    BesideCaptures() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~BesideCaptures() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 }  // namespace ib
+
+#define IB_ENTER(ctx)                                                   \
+    IB_REQUIRE((ctx) != nullptr, "null context");                       \
+    ib::DeviceGuard _guard((ctx)->device);                              \
+    if (!_guard.ok) return ib::set_error(IB_ERR_CUDA, "cudaSetDevice(%d) failed", (ctx)->device)

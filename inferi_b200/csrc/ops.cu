@@ -1,37 +1,12 @@
 // Stand-alone element-wise ops of the token loop (RMSNorm, RoPE, SwiGLU, residual add, arg-max).
 // Inside the model these are fused into GEMV prologues/epilogues; the stand-alone kernels serve the
 // op-level API that mirrors crates/inferi/src/ops/{rms_norm,rope,silu}.rs and context.rs:516-530.
-//
-// All of them are launched with programmatic dependent launch: each lets its successor start at once and waits for its
-// predecessor before it touches an operand, so that in a chain of op calls the next kernel's launch and set-up overlap the
-// previous kernel's tail (worth 1-2 us per launch where a kernel itself takes 2 us).
-#include "common.cuh"
+#include "op_launch.cuh"
 
 #include <math.h>
 #include <string.h>
 
 namespace ib {
-
-__device__ __forceinline__ void pdl_enter() {
-    asm volatile("griddepcontrol.launch_dependents;");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
-template <typename... KArgs, typename... Args>
-static int32_t launch_op(ib_ctx *ctx, cudaStream_t s, void (*kernel)(KArgs...), uint32_t grid, uint32_t block, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(block);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    IB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, (KArgs)args...));
-    ctx->launches++;
-    return IB_OK;
-}
 
 // ---- RMSNorm: crates/inferi-shaders/src/rms_norm.rs:78-121 ----
 // One CTA; latency bound (one load, a block reduction, one store).  The first RMS_KEEP values of a thread stay in registers,

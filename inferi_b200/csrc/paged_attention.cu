@@ -1,0 +1,66 @@
+// ib_paged_attention: checks, scratch, and which kernel takes which requests.
+#include "paged_attention.cuh"
+
+namespace ib {
+
+int32_t check_paged_cache(const char *who, const ib_paged_cache *c);   // paged.cu
+uint32_t log2_of(uint32_t power);
+
+// Scratch of a context, of one size whatever the arguments: made once and never moved, so a captured launch may be replayed at any time.  (Made while a stream is being
+// captured, it is cleared on a stream of its own: the capture does not get the clearing as a node.)
+static int32_t ensure_paged_scratch(ib_ctx *ctx) {
+    if (ctx->paged_scratch) return IB_OK;
+    const size_t floats = paged_decode_scratch_floats(ctx, 128), counters = paged_decode_ctas(ctx);
+    BesideCaptures beside;
+    float *scratch = nullptr;
+    cudaStream_t own = nullptr;
+    IB_CHECK_CUDA(cudaMalloc(&scratch, floats * sizeof(float) + counters * sizeof(uint32_t)));
+    cudaError_t e = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMemsetAsync(scratch + floats, 0, counters * sizeof(uint32_t), own);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(own);
+    if (own) cudaStreamDestroy(own);
+    if (e != cudaSuccess) {
+        cudaFree(scratch);
+        return set_error(IB_ERR_CUDA, "ib_paged_attention: clearing the counters failed: %s", cudaGetErrorString(e));
+    }
+    ctx->paged_scratch = scratch;
+    ctx->paged_counters = reinterpret_cast<uint32_t *>(scratch + floats);
+    return IB_OK;
+}
+
+}  // namespace ib
+
+using namespace ib;
+
+extern "C" int32_t ib_paged_attention(ib_ctx *ctx, void *stream, const ib_paged_attn_args *args, const ib_paged_cache *cache) {
+    IB_ENTER(ctx);
+    IB_REQUIRE(args, "ib_paged_attention: null argument");
+    const ib_paged_attn_args &p = *args;
+    int32_t rc = check_paged_cache("ib_paged_attention", cache);
+    if (rc) return rc;
+    if (p.n_requests == 0 || p.n_tokens == 0) return IB_OK;
+    IB_REQUIRE(p.q_dev && p.out_dev && p.block_table && p.row_start && p.kv_len, "ib_paged_attention: null pointer");
+    IB_REQUIRE(p.kv_mul >= 1 && p.kv_mul <= 64 && p.n_heads >= p.kv_mul && p.n_heads % p.kv_mul == 0, "ib_paged_attention: n_heads=%u is not a multiple of kv_mul=%u (1 to 64)", p.n_heads, p.kv_mul);
+    if (p.head_size != 64 && p.head_size != 128) return set_error(IB_ERR_UNSUPPORTED, "ib_paged_attention: head_size=%u (supported: 64, 128)", p.head_size);
+    IB_REQUIRE(p.n_heads <= (1u << 16), "ib_paged_attention: %u heads (up to 65536)", p.n_heads);
+    IB_REQUIRE(cache->kv_dim == p.n_heads / p.kv_mul * p.head_size, "ib_paged_attention: kv_dim=%u != n_kv_heads*head_size=%u", cache->kv_dim, p.n_heads / p.kv_mul * p.head_size);
+    const uint32_t dim = p.n_heads * p.head_size;
+    IB_REQUIRE(p.q_stride >= dim && p.out_stride >= dim && p.q_stride < (1ull << 40) && p.out_stride < (1ull << 40), "ib_paged_attention: rows overlap (a stride below %u), or a stride above 2^40", dim);
+    IB_REQUIRE(p.n_requests <= 65536 && p.n_tokens < (1u << 25), "ib_paged_attention: %u requests (up to 65536) with %u rows (below 2^25)", p.n_requests, p.n_tokens);
+    IB_REQUIRE(p.max_pages >= 1 && (uint64_t)p.max_pages * cache->page_size < (1ull << 31), "ib_paged_attention: rows of %u pages of %u positions (1 to 2^31 - 1 positions)", p.max_pages, cache->page_size);
+    rc = ensure_paged_scratch(ctx);
+    if (rc) return rc;
+    PagedAttn a = {};
+    a.q = p.q_dev; a.out = p.out_dev; a.q_stride = p.q_stride; a.out_stride = p.out_stride;
+    a.table = p.block_table; a.row_start = p.row_start; a.kv_len = p.kv_len;
+    a.k = cache->k_dev; a.v = cache->v_dev; a.page_stride = cache->page_stride;
+    a.n_requests = p.n_requests; a.n_tokens = p.n_tokens; a.max_pages = p.max_pages; a.n_pages = cache->n_pages; a.page_log2 = log2_of(cache->page_size);
+    a.kv_heads = p.n_heads / p.kv_mul; a.kv_mul = p.kv_mul; a.kv_dim = cache->kv_dim;
+    a.window = p.window; a.sinks = p.sinks;
+    a.vec = (uintptr_t)p.q_dev % 16 == 0 && (uintptr_t)p.out_dev % 16 == 0 && p.q_stride % 4 == 0 && p.out_stride % 4 == 0;
+    a.scratch = ctx->paged_scratch; a.counters = ctx->paged_counters;
+    a.err = ctx->err_dev; a.wait_ns = ctx->wait_limit_ns;
+    a.rows_from = 1;
+    a.rows_to = 0xFFFFFFFFu;
+    return launch_paged_decode(ctx, (cudaStream_t)stream, a, p.head_size, cache->kv_dtype);
+}

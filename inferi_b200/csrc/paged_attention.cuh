@@ -1,0 +1,309 @@
+// Attention of new tokens over a paged cache: what its kernels share - a launch's arguments, how the work is handed out, and the rows that are done again.
+//
+// Rows and tiles.  The query heads of a kv head see the same positions, so a request's tokens and those heads together are the rows of a product with K: row t * heads + g is
+// head g of token t.  A query tile is some tokens of a request with all heads of a group (TileShape); the positions it sees are cut into key tiles of KT.
+//
+// The units (request, head group, query tile, key tile), in that order, are cut into contiguous, equally long ranges, one per CTA of a grid that fills the GPU once, whatever
+// the requests' lengths: a batch of one long and many short requests needs no other treatment than one of equal ones.  A query tile whose key tiles fall to several CTAs gets a
+// partial (maximum, sum, accumulator) from each; a CTA has at most two such tiles, the one that its range begins in and the one that it ends in, so the scratch has
+// two places per CTA whatever the lengths.  The last CTA of a tile to arrive (an atomic counter; nobody waits) adds up the partials in the order of the CTAs: the result does not depend on who
+// was last.  Every CTA finds its range by itself from row_start and kv_len, by a sum over the requests: lengths never have to come to the host, and no launch ahead
+// has to prepare the work.
+#pragma once
+
+#include "common.cuh"
+
+#include <math.h>
+
+namespace ib {
+
+struct PagedAttn {
+    const float *q;
+    float *out;
+    uint64_t q_stride, out_stride;
+    const int32_t *table, *row_start, *kv_len;
+    const void *k, *v;
+    uint64_t page_stride;
+    uint32_t n_requests, n_tokens, max_pages, n_pages, page_log2;
+    uint32_t kv_heads, kv_mul, kv_dim;
+    uint32_t window, sinks;
+    uint32_t rows_from, rows_to;   // the launch takes the requests with that many rows (new tokens * kv_mul)
+    uint32_t least_units;          // units of a CTA's range, at least
+    uint32_t vec;                  // q and out are on 16-byte boundaries
+    float *scratch;                // two partials per CTA
+    uint32_t *counters;            // of arrivals, one per CTA and half of its tiles; zero between launches
+    uint32_t *err;
+    unsigned long long wait_ns;
+};
+
+struct PagedRequest {
+    uint32_t start, n;   // first row of q, new tokens
+    int32_t p0;          // position of the first one (below 0: lengths that do not fit together; such tokens see nothing)
+};
+// Lengths come from the caller's arrays: whatever they hold, rows stay inside q and positions inside the row of the table.
+__device__ __forceinline__ PagedRequest paged_request(const PagedAttn &a, uint32_t r) {
+    PagedRequest q;
+    const int32_t s = a.row_start[r], e = a.row_start[r + 1], top = (int32_t)a.n_tokens, kv = a.kv_len[r];
+    const int32_t s1 = min(max(s, 0), top), e1 = min(max(e, s1), top);
+    q.start = (uint32_t)s1;
+    q.n = (uint32_t)(e1 - s1);
+    if ((uint64_t)q.n * a.kv_mul < a.rows_from || (uint64_t)q.n * a.kv_mul > a.rows_to) q.n = 0;   // not of this launch
+    q.p0 = min(max(kv, 0), (int32_t)(a.max_pages << a.page_log2)) - (int32_t)(e1 - s1);
+    return q;
+}
+
+// How rows are grouped: `heads` query heads of a kv head at a time (`groups` times per kv head), with `tokens` tokens per query tile
+struct TileShape { uint32_t heads, groups, tokens; };
+
+// The key tiles of a query tile: the first `sink_tiles` ones, then those from `first` on; `units` together (one at least: a tile whose tokens see nothing
+// still has its rows written)
+struct KeySpan { uint32_t sink_tiles, first, units, end; };   // end: positions before it are seen by some row
+template <uint32_t KT>
+__device__ __forceinline__ KeySpan key_span(const PagedAttn &a, const PagedRequest &q, uint32_t tokens, uint32_t j) {
+    const long long lo = (long long)q.p0 + (long long)j * tokens, hi = (long long)q.p0 + min((j + 1) * tokens, q.n);   // positions of the tile's tokens: lo .. hi - 1
+    KeySpan s = {0, 0, 1, hi > 0 ? (uint32_t)hi : 0u};
+    const uint32_t tiles = (s.end + KT - 1) / KT;
+    if (a.window) {
+        const long long from = lo - (long long)a.window + 1;
+        if (from > 0) {
+            s.first = (uint32_t)from / KT;
+            s.sink_tiles = (uint32_t)((min((long long)a.sinks, from) + KT - 1) / KT);
+            if (s.sink_tiles >= s.first) s.first = s.sink_tiles = 0;
+        }
+    }
+    const uint32_t n = s.sink_tiles + tiles - s.first;
+    if (n > 1) s.units = n;
+    return s;
+}
+__device__ __forceinline__ uint32_t key_tile(const KeySpan &s, uint32_t unit) { return unit < s.sink_tiles ? unit : s.first + unit - s.sink_tiles; }
+
+// Units of a head group of every lane's own request.  Called by a whole warp: long requests are shared among the lanes.
+template <uint32_t KT>
+__device__ __forceinline__ unsigned long long request_units(const PagedAttn &a, const PagedRequest &q, uint32_t tokens) {
+    const uint32_t lane = threadIdx.x & 31, tiles = (q.n + tokens - 1) / tokens;
+    unsigned long long sum = 0;
+    if (tiles <= 4)
+        for (uint32_t j = 0; j < tiles; j++) sum += key_span<KT>(a, q, tokens, j).units;
+    for (uint32_t who = __ballot_sync(0xffffffffu, tiles > 4); who; who &= who - 1) {
+        const int l = __ffs(who) - 1;
+        PagedRequest b;
+        b.start = 0;
+        b.n = __shfl_sync(0xffffffffu, q.n, l);
+        b.p0 = __shfl_sync(0xffffffffu, q.p0, l);
+        const uint32_t t = (b.n + tokens - 1) / tokens;
+        unsigned long long part = 0;
+        for (uint32_t j = lane; j < t; j += 32) part += key_span<KT>(a, b, tokens, j).units;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+        if ((int)lane == l) sum = part;
+    }
+    return sum;
+}
+
+// ---- a CTA's range ----
+struct PagedRange {
+    unsigned long long total, offset;   // units of the launch; the range's first unit, counted inside its request
+    uint32_t ranges, request;
+    __device__ __forceinline__ unsigned long long first_unit(uint32_t c) const { return (unsigned long long)c * total / ranges; }
+    __device__ __forceinline__ uint32_t range_of(unsigned long long unit) const { return (uint32_t)(((unit + 1) * ranges - 1) / total); }
+};
+struct PagedRangeShared { unsigned long long sum[33], offset; uint32_t owner, request; };
+
+// Called by a whole CTA of THREADS threads (every thread a stretch of the requests); ends with a barrier.  total == 0: nothing to do in this launch.
+template <uint32_t KT, uint32_t THREADS>
+__device__ __forceinline__ PagedRange paged_range(const PagedAttn &a, const TileShape &shape, PagedRangeShared &sh) {
+    constexpr uint32_t WARPS = THREADS / 32;
+    static_assert(WARPS <= 32, "one sum per warp");
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per = (a.n_requests + THREADS - 1) / THREADS, head_groups = a.kv_heads * shape.groups;
+    auto units_of = [&](uint32_t r) {
+        PagedRequest q = {0, 0, 0};
+        if (r < a.n_requests) q = paged_request(a, r);
+        return request_units<KT>(a, q, shape.tokens) * head_groups;
+    };
+    unsigned long long mine = 0;
+    for (uint32_t b = 0; b < per; b++) mine += units_of(tid * per + b);
+    unsigned long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long t = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= (uint32_t)o) upto += t;
+    }
+    if (lane == 31) sh.sum[warp] = upto;
+    __syncthreads();
+    unsigned long long ahead = 0, total = 0;
+    for (uint32_t w = 0; w < WARPS; w++) {
+        if (w < warp) ahead += sh.sum[w];
+        total += sh.sum[w];
+    }
+    PagedRange g = {total, 0, 0, 0};
+    if (total == 0) return g;
+    const unsigned long long most = (total + a.least_units - 1) / a.least_units;
+    g.ranges = most < gridDim.x ? (uint32_t)most : gridDim.x;
+    const unsigned long long first = g.first_unit(blockIdx.x), before = ahead + upto - mine;
+    if (blockIdx.x < g.ranges && first >= before && first < before + mine) {
+        sh.owner = tid;
+        sh.offset = first - before;
+        sh.request = tid;
+    }
+    __syncthreads();
+    if (per > 1) {   // which of the owner's requests
+        if (warp == 0 && blockIdx.x < g.ranges) {
+            const uint32_t base = sh.owner * per;
+            unsigned long long left = sh.offset;
+            __syncwarp();   // (everyone has read what the finder overwrites)
+            for (uint32_t b = 0; b < per; b += 32) {
+                const unsigned long long u = units_of(b + lane < per ? base + b + lane : a.n_requests);
+                unsigned long long run = u;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const unsigned long long t = __shfl_up_sync(0xffffffffu, run, o);
+                    if (lane >= (uint32_t)o) run += t;
+                }
+                const bool here = left >= run - u && left < run;
+                if (here) {
+                    sh.request = base + b + lane;
+                    sh.offset = left - (run - u);
+                }
+                if (__any_sync(0xffffffffu, here)) break;
+                left -= __shfl_sync(0xffffffffu, run, 31);
+            }
+        }
+        __syncthreads();
+    }
+    g.request = sh.request;
+    g.offset = sh.offset;
+    return g;
+}
+
+// ---- a walk over the range, piece by piece; every warp that needs it walks for itself ----
+template <uint32_t KT>
+struct PagedWalk {
+    PagedRequest q;
+    KeySpan span;
+    unsigned long long unit, end, per_group;   // the current unit and the range's end, counted over the launch; units of the request's head groups
+    uint32_t request, group, tile, tiles;      // group: of all kv heads' groups
+    uint32_t at, count;                        // the piece: units at .. at + count - 1 of its query tile
+
+    __device__ __forceinline__ void load(const PagedAttn &a, const TileShape &s, uint32_t r) {
+        request = r;
+        q = paged_request(a, r);
+        tiles = (q.n + s.tokens - 1) / s.tokens;
+    }
+    __device__ __forceinline__ void cut() {
+        const unsigned long long left = end - unit;
+        count = span.units - at < left ? span.units - at : (uint32_t)left;
+    }
+    __device__ __forceinline__ void begin(const PagedAttn &a, const TileShape &s, const PagedRange &g) {
+        const uint32_t lane = threadIdx.x & 31;
+        unit = g.first_unit(blockIdx.x);
+        end = g.first_unit(blockIdx.x + 1);
+        load(a, s, g.request);
+        PagedRequest one = q;
+        if (lane) one.n = 0;   // (the others help)
+        per_group = __shfl_sync(0xffffffffu, request_units<KT>(a, one, s.tokens), 0);
+        group = (uint32_t)(g.offset / per_group);
+        unsigned long long left = g.offset - group * per_group;
+        for (uint32_t j = 0;; j += 32) {   // the query tile
+            const uint32_t u = j + lane < tiles ? key_span<KT>(a, q, s.tokens, j + lane).units : 0u;
+            unsigned long long run = u;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned long long t = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= (uint32_t)o) run += t;
+            }
+            const uint32_t hit = __ballot_sync(0xffffffffu, left < run);
+            if (hit || j + 32 >= tiles) {
+                const int l = hit ? __ffs(hit) - 1 : 0;
+                tile = j + l;
+                at = (uint32_t)(left - __shfl_sync(0xffffffffu, run - u, l));
+                break;
+            }
+            left -= __shfl_sync(0xffffffffu, run, 31);
+        }
+        span = key_span<KT>(a, q, s.tokens, tile);
+        cut();
+    }
+    // the next piece; false: the range is done
+    __device__ __forceinline__ bool next(const PagedAttn &a, const TileShape &s) {
+        unit += count;
+        if (unit >= end) return false;
+        at = 0;
+        if (++tile == tiles) {
+            tile = 0;
+            if (++group == a.kv_heads * s.groups) {
+                group = 0;
+                const uint32_t lane = threadIdx.x & 31;
+                for (uint32_t r = request + 1;; r += 32) {   // the next request of this launch (there is one: the range goes on)
+                    const bool some = r + lane < a.n_requests && paged_request(a, r + lane).n > 0;
+                    const uint32_t who = __ballot_sync(0xffffffffu, some);
+                    if (who || r + 32 >= a.n_requests) {
+                        load(a, s, who ? r + __ffs(who) - 1 : a.n_requests - 1);
+                        break;
+                    }
+                }
+            }
+        }
+        span = key_span<KT>(a, q, s.tokens, tile);
+        cut();
+        return true;
+    }
+    __device__ __forceinline__ bool whole() const { return count == span.units; }
+    // Of a tile that is not whole: where this CTA leaves its partial, and who else has one.  A piece that begins the range goes to the CTA's first place, one that ends it to
+    // the second.
+    __device__ __forceinline__ unsigned long long tile_unit() const { return unit - at; }
+};
+// The place of CTA c's partial of the tile that starts at unit `tile_unit`
+__device__ __forceinline__ uint32_t paged_place(const PagedRange &g, unsigned long long tile_unit, uint32_t c) { return 2 * c + (g.first_unit(c) < tile_unit ? 1u : 0u); }
+
+__device__ __forceinline__ bool paged_sees(const PagedAttn &a, long long p, long long j) {
+    return j >= 0 && j <= p && (a.window == 0 || p - j < (long long)a.window || j < (long long)a.sinks);
+}
+
+__device__ __forceinline__ float paged_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// A row's power of two for its f16 halves: q * 2^-e is below 2 in magnitude, whatever q's range (no scaling for rows that hold no numbers)
+__device__ __forceinline__ int paged_exponent(float most) {
+    const int e = (int)(__float_as_uint(most) >> 23) - 127;   // most >= 0
+    return e > 127 || most == 0.f ? 0 : (e < -100 ? -100 : e);
+}
+
+// ---- rows that hold something that is not a finite number ----
+// A masked position's weight is 0, but 0 times an infinity or NaN in its row of V is not, and the tiles' products run over all of a tile's positions (those that no
+// row of the tile sees are zeroed on their way); a weight's remainder may be 0 or negative where the weight is not.  So a row with such a result is computed anew, position by position, with
+// the row's largest score (rounded up, in units of log2) known - unless its sum of weights is none either: then it sees a key, or is a query, that is none, and all of the row is rightly
+// so.  Called by a whole warp.
+template <typename T>
+__device__ __noinline__ void paged_repair(const PagedAttn &a, uint32_t KT, uint32_t request, uint32_t kv_head, const KeySpan span, long long p, float most, const float *q, float *out, uint32_t hs) {
+    const uint32_t lane = threadIdx.x & 31, E = hs / 32;
+    const float scale = 1.4426950408889634f / sqrtf((float)hs);
+    float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t u = 0; u < span.units; u++) {
+        const long long base = (long long)key_tile(span, u) * KT;
+        for (long long j = base; j < min(base + KT, (long long)span.end); j++) {
+            if (!paged_sees(a, p, j)) continue;
+            const int32_t page = a.table[(size_t)request * a.max_pages + ((uint32_t)j >> a.page_log2)];
+            if (page < 0 || (uint32_t)page >= a.n_pages) continue;
+            const uint64_t at = (uint64_t)page * a.page_stride + (uint64_t)((uint32_t)j & ((1u << a.page_log2) - 1)) * a.kv_dim + kv_head * hs + lane;
+            const T *k = static_cast<const T *>(a.k) + at, *v = static_cast<const T *>(a.v) + at;
+            float s = 0.f;
+            for (uint32_t e = 0; e < E; e++) s += q[lane + 32 * e] * (float)k[32 * e];
+#pragma unroll
+            for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            const float x = fmaxf(paged_ex2(s * scale - most), 1e-38f);   // (not nothing: an infinity that is seen counts, however small its weight)
+            l += x;
+            for (uint32_t e = 0; e < E; e++) acc[e] += x * (float)v[32 * e];
+        }
+    }
+    for (uint32_t e = 0; e < E; e++) out[lane + 32 * e] = acc[e] / l;
+}
+
+// paged_decode.cu
+constexpr uint32_t PAGED_DECODE_ROWS = 8;
+size_t paged_decode_scratch_floats(const ib_ctx *ctx, uint32_t head_size);
+uint32_t paged_decode_ctas(const ib_ctx *ctx);
+int32_t launch_paged_decode(ib_ctx *ctx, cudaStream_t s, PagedAttn a, uint32_t head_size, int kv_dtype);
+
+}  // namespace ib

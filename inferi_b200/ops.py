@@ -15,7 +15,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import AttnParams, InferiError, KV_F16, KV_F32, ROPE_NEOX, ROPE_ORIGINAL, check  # noqa: F401
+from ._lib import AttnParams, InferiError, KV_F16, KV_F32, PagedAppendArgs, PagedAttnArgs, PagedCache, PagePlanArgs, ROPE_NEOX, ROPE_ORIGINAL, check  # noqa: F401
 from .build import binding_stamp
 from .quant import BLOCK_BYTES, BLOCK_ELEMS, F32, NAMES, Q4_K, Q5_K, Q6_K, Q8_0, row_bytes  # noqa: F401
 
@@ -365,3 +365,128 @@ class Sampler:
                                          float(coin), out.data_ptr()))
         return out
 
+
+# ---- a batch of requests over a paged cache (no counterpart in the reference, which holds one sequence) ----
+PLAN_OK, PLAN_NO_PAGES, PLAN_TABLE_FULL, PLAN_NO_ROOM, PLAN_INVALID = range(5)   # what PagePlan says of a request
+
+
+def _on_device(backend: Backend, *named) -> None:
+    for name, t in named:
+        if not isinstance(t, _tensor) or not t.is_cuda or t.device.index != backend.device:
+            raise InferiError(1, f"{name}: expected a tensor on device cuda:{backend.device}")
+
+
+def _i32_dev(t: torch.Tensor, name: str, numel: int | None = None) -> int:
+    if t.dtype is not torch.int32 or not t.is_contiguous() or (numel is not None and t.numel() != numel):
+        raise InferiError(1, f"{name}: expected a contiguous int32 tensor" + (f" of {numel} elements" if numel is not None else ""))
+    return t.data_ptr()
+
+
+def _u32(v: int, name: str) -> int:
+    if not 0 <= v < 1 << 32:
+        raise InferiError(1, f"{name}: {v} is not a 32-bit count")
+    return v
+
+
+def _f32_rows(t: torch.Tensor, name: str, n: int | None = None, dim: int | None = None) -> tuple[int, int]:
+    """Address and stride of a [n, dim] float32 tensor whose rows are contiguous."""
+    if t.dtype is not _f32 or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (n is not None and t.shape[0] != n) or (dim is not None and t.shape[1] != dim):
+        raise InferiError(1, f"{name}: expected a [{'n' if n is None else n}, {'dim' if dim is None else dim}] float32 tensor with contiguous rows, got {tuple(t.shape)} {t.dtype}")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _paged_cache(key_cache: torch.Tensor, value_cache: torch.Tensor) -> PagedCache:
+    k, v = key_cache, value_cache
+    if k.dtype is not v.dtype or (k.dtype is not _f16 and k.dtype is not _f32):
+        raise InferiError(1, "paged cache: the caches must both be float16 or both float32")
+    if k.dim() != 3 or k.shape != v.shape or k.stride() != v.stride() or k.stride(2) != 1 or k.stride(1) != k.shape[2]:
+        raise InferiError(1, f"paged cache: expected two [pages, page_size, kv_dim] tensors with contiguous pages, got {tuple(k.shape)} and {tuple(v.shape)}")
+    return PagedCache(k.data_ptr(), v.data_ptr(), k.stride(0) if k.shape[0] > 1 else k.shape[1] * k.shape[2], k.shape[0], k.shape[1], k.shape[2], KV_F16 if k.dtype is _f16 else KV_F32)
+
+
+class PagePlan:
+    """Block tables, positions and slots of a step, from the requests' lengths (`ib_page_plan`: what each array holds, and who gets pages)."""
+
+    def __init__(self, backend: Backend):
+        self.backend = backend
+
+    from_backend = classmethod(lambda cls, backend: cls(backend))
+
+    def launch(self, page_size: int, cached_len: torch.Tensor, new_len: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, n_free: torch.Tensor, kv_len: torch.Tensor,
+               row_start: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, n_free_out: torch.Tensor, status: torch.Tensor) -> None:
+        """int32 CUDA tensors: lengths and status [n], block_table [n, max_pages], free_pages [pages of the cache], row_start [n + 1], positions and slots [room for
+        tokens], n_free and n_free_out [1].  kv_len may be cached_len and n_free_out n_free."""
+        b, n = self.backend, cached_len.numel()
+        _on_device(b, ("cached_len", cached_len), ("new_len", new_len), ("block_table", block_table), ("free_pages", free_pages), ("n_free", n_free), ("kv_len", kv_len), ("row_start", row_start),
+                   ("positions", positions), ("slots", slots), ("n_free_out", n_free_out), ("status", status))
+        if block_table.dim() != 2 or block_table.shape[0] != n:
+            raise InferiError(1, f"page plan: {n} requests but a block table of {tuple(block_table.shape)}")
+        a = PagePlanArgs(n, block_table.shape[1], _u32(slots.numel(), "slots"), _u32(free_pages.numel(), "free_pages"), _u32(page_size, "page_size"), _i32_dev(cached_len, "cached_len"), _i32_dev(new_len, "new_len", n), _i32_dev(n_free, "n_free", 1),
+                         _i32_dev(block_table, "block_table"), _i32_dev(free_pages, "free_pages"), _i32_dev(kv_len, "kv_len", n), _i32_dev(row_start, "row_start", n + 1),
+                         _i32_dev(positions, "positions", slots.numel()), _i32_dev(slots, "slots"), _i32_dev(n_free_out, "n_free_out", 1), _i32_dev(status, "status", n))
+        check(b.lib.ib_page_plan(b.handle, _stream_ptr(), C.byref(a)))
+
+
+@dataclass
+class PagedAppendConfig:
+    """The part of `RoPEConfig` that does not change from row to row."""
+    head_size: int
+    base_freq: float
+
+
+class PagedAppend:
+    """`RoPE.launch` for rows at positions of their own, and their keys and values into their slots of a paged cache (`ib_paged_append`)."""
+
+    def __init__(self, backend: Backend):
+        self.backend = backend
+
+    from_backend = classmethod(lambda cls, backend: cls(backend))
+
+    def launch(self, variant: int, config: PagedAppendConfig, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, q_out: torch.Tensor,
+               key_cache: torch.Tensor, value_cache: torch.Tensor) -> None:
+        """q, q_out: [n, q_dim], k, v: [n, kv_dim] float32 with contiguous rows (q_out may be q); caches [pages, page_size, kv_dim] float16 or float32; positions and
+        slots [n] int32.  Rows with slots outside the cache are left out."""
+        b = self.backend
+        _on_device(b, ("q", q), ("k", k), ("v", v), ("positions", positions), ("slots", slots), ("q_out", q_out), ("key_cache", key_cache), ("value_cache", value_cache))
+        c = _paged_cache(key_cache, value_cache)
+        (pq, sq), (n, q_dim) = _f32_rows(q, "q"), q.shape
+        (pk, sk), (pv, sv), (po, so) = _f32_rows(k, "k", n, c.kv_dim), _f32_rows(v, "v", n, c.kv_dim), _f32_rows(q_out, "q_out", n, q_dim)
+        a = PagedAppendArgs(pq, pk, pv, po, sq, sk, sv, so, _i32_dev(positions, "positions", n), _i32_dev(slots, "slots", n), _u32(n, "rows"), _u32(q_dim, "q_dim"), _u32(config.head_size, "head_size"), variant, config.base_freq)
+        check(b.lib.ib_paged_append(b.handle, _stream_ptr(), C.byref(a), C.byref(c)))
+
+
+@dataclass
+class PagedAttentionConfig:
+    """window: positions that a token sees up to its own, 0: all of them; sinks: first positions that it sees besides.  longest_new: the most new tokens that a
+    request of the call has, where the host knows it, else 0; results do not depend on it."""
+    n_heads: int
+    kv_mul: int
+    head_size: int
+    window: int = 0
+    sinks: int = 0
+    longest_new: int = 0
+
+
+class PagedAttention:
+    """Attention of the new tokens of several requests, single ones and chunks of prompts, over a paged cache that holds their keys and values (`ib_paged_attention`)."""
+
+    def __init__(self, backend: Backend):
+        self.backend = backend
+
+    from_backend = classmethod(lambda cls, backend: cls(backend))
+
+    def launch(self, config: PagedAttentionConfig, q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_table: torch.Tensor, row_start: torch.Tensor, kv_len: torch.Tensor,
+               out: torch.Tensor) -> None:
+        """q, out: [rows, n_heads * head_size] float32 with contiguous rows; caches [pages, page_size, kv_dim] float16 or float32; block_table [n, max_pages], row_start
+        [n + 1], kv_len [n] int32.  Rows behind row_start[n] stay as they are."""
+        b, n = self.backend, kv_len.numel()
+        _on_device(b, ("q", q), ("key_cache", key_cache), ("value_cache", value_cache), ("block_table", block_table), ("row_start", row_start), ("kv_len", kv_len), ("out", out))
+        c = _paged_cache(key_cache, value_cache)
+        dim = config.n_heads * config.head_size
+        (pq, sq), (po, so) = _f32_rows(q, "q", None, dim), _f32_rows(out, "out", q.shape[0], dim)
+        if block_table.dim() != 2 or block_table.shape[0] != n:
+            raise InferiError(1, f"paged attention: {n} requests but a block table of {tuple(block_table.shape)}")
+        counts = [_u32(getattr(config, f), f) for f in ("n_heads", "kv_mul", "head_size", "window", "sinks", "longest_new")]
+        a = PagedAttnArgs(pq, po, sq, so, _i32_dev(block_table, "block_table"), _i32_dev(row_start, "row_start", n + 1), _i32_dev(kv_len, "kv_len"), n, _u32(q.shape[0], "rows"),
+                          block_table.shape[1], *counts)
+        check(b.lib.ib_paged_attention(b.handle, _stream_ptr(), C.byref(a), C.byref(c)))

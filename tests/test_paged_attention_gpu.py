@@ -1,0 +1,335 @@
+"""Attention over a paged cache against its definition in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from inferi_b200.ops import Backend, FusedAttention, AttnParams, InferiError, PagedAttention, PagedAttentionConfig
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(a):
+    return torch.tensor(a, dtype=torch.int32, device="cuda")
+
+
+class Batch:
+    """Requests with `cached` positions behind them and `new` tokens each, their pages shuffled over a cache whose unused rows hold NaN."""
+
+    def __init__(self, cached, new, heads, mul, hs, P=16, dtype=torch.float16, pad=0, gap=0, q_pad=0, offset=0, seed=1, q_scale=1.0, spare=2):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        self.cached, self.new, self.heads, self.mul, self.hs, self.P, self.gap = cached, new, heads, mul, hs, P, gap
+        self.kv = [c + n for c, n in zip(cached, new)]
+        kv_dim, n = heads // mul * hs, len(cached)
+        pages = [-(-max(k, 0) // P) for k in self.kv]
+        self.n_pages, width = sum(pages) + spare, max(pages) + 1
+        ids = torch.randperm(self.n_pages, generator=torch.Generator().manual_seed(seed)).tolist()
+        self.store = torch.full((2, self.n_pages * (P * kv_dim + gap)), float("nan"), dtype=dtype, device="cuda")
+        self.kc, self.vc = (s.as_strided((self.n_pages, P, kv_dim), (P * kv_dim + gap, kv_dim, 1)) for s in self.store)
+        self.table = torch.full((n, width), 1 << 30, dtype=torch.int32)   # entries behind a request's pages are not looked at
+        self.rows = []   # per request: [kv, kv_dim] of K and V as the cache holds them
+        for r in range(n):
+            mine, ids = ids[: pages[r]], ids[pages[r]:]
+            self.table[r, : pages[r]] = torch.tensor(mine, dtype=torch.int32)
+            k, v = (torch.randn(max(self.kv[r], 0), kv_dim, generator=g, device="cuda").to(dtype) for _ in range(2))
+            for i, page in enumerate(mine):
+                part = slice(i * P, min((i + 1) * P, self.kv[r]))
+                self.kc[page, : part.stop - part.start], self.vc[page, : part.stop - part.start] = k[part], v[part]
+            self.rows.append((k, v))
+        self.table = self.table.cuda()
+        self.start = [0]
+        for c in new:
+            self.start.append(self.start[-1] + c)
+        self.row_start, self.kv_len = i32(self.start), i32(self.kv)
+        tokens = self.start[-1] + pad
+
+        def rows():
+            return torch.randn(tokens * (heads * hs + q_pad) + offset, generator=g, device="cuda")[offset:].view(tokens, heads * hs + q_pad)[:, : heads * hs]
+
+        self.q, self.out = rows(), rows()
+        self.q *= q_scale
+
+    def put(self, r, j, which, value):
+        """Sets a position's row of K (0) or V (1), in the cache and in the copy."""
+        self.rows[r][which][j] = value
+        (self.kc, self.vc)[which][self.table[r, j // self.P].item(), j % self.P] = value
+
+    def run(self, backend, window=0, sinks=0, longest_new=0):
+        PagedAttention(backend).launch(PagedAttentionConfig(self.heads, self.mul, self.hs, window, sinks, longest_new), self.q, self.kc, self.vc, self.table, self.row_start, self.kv_len, self.out)
+        return self.out
+
+    def exact(self, r, window=0, sinks=0):
+        """([new, heads, hs] of request r, how far a result may be off)"""
+        n, kv, hs, G = self.new[r], self.kv[r], self.hs, self.mul
+        k, v = (x.double().view(kv, self.heads // G, hs).permute(1, 0, 2) for x in self.rows[r])       # [kv heads, kv, hs]
+        q = self.q[self.start[r]: self.start[r] + n].double().view(n, self.heads // G, G, hs).permute(1, 2, 0, 3)   # [kv heads, G, n, hs]
+        p = torch.arange(kv - n, kv, device="cuda")[:, None]
+        j = torch.arange(kv, device="cuda")[None, :]
+        seen = j <= p
+        if window:
+            seen = seen & ((p - j < window) | (j < sinks))
+        s = torch.einsum("hgnd,hkd->hgnk", q, k) / math.sqrt(hs)
+        s = torch.where(seen, s, -math.inf)
+        w = torch.exp(s - s.amax(-1, keepdim=True).clamp(min=-1e300))
+        w = w / w.sum(-1, keepdim=True)
+        w = torch.where(seen, w, 0.0)   # (rows that see nothing)
+        # positions that a row does not see count for nothing, whatever they hold
+        finite = torch.where(torch.isfinite(v), v, 0.0)
+        out = torch.einsum("hgnk,hkd->hgnd", w, finite)
+        odd = ~torch.isfinite(v).all(-1)
+        for h, at in odd.nonzero().tolist():
+            sees = seen[:, at]
+            out[h][:, sees] = out[h][:, sees] + w[h][:, sees, at][..., None] * torch.where(torch.isfinite(v[h, at]), 0.0, v[h, at])
+        # A score is off by at most the split of q (2^-23 of its terms' absolute sum A), hs / 8 truncated additions of two products (2^-23 of A each) and three roundings; a weight by twice that
+        # (its own and the sum's) and the exponential's 2^-22, its split's 2^-22; the sum over positions adds 2^-23 per 16 of them and a rounding per step: all of it relative to the weighted sum of |v|.
+        A = float(torch.einsum("hgnd,hkd->hgnk", q.abs(), torch.where(torch.isfinite(k), k, 0.0).abs()).max()) / math.sqrt(hs)
+        tol = 2 * A * (hs / 8 + 4) * 2**-23 + (8 + kv / 16) * 2**-23
+        return out.permute(2, 0, 1, 3).reshape(n, -1), tol * float(finite.abs().max()) + 1e-30
+
+    def check(self, backend, window=0, sinks=0, longest_new=0, requests=None):
+        before = self.out.clone()
+        self.run(backend, window, sinks, longest_new)
+        for r in requests if requests is not None else range(len(self.new)):
+            if self.new[r] and self.kv[r] >= self.new[r]:
+                want, tol = self.exact(r, window, sinks)
+                got = self.out[self.start[r]: self.start[r + 1]].double()
+                fine = torch.isfinite(want)
+                assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got[~fine & ~torch.isnan(want)], want[~fine & ~torch.isnan(want)]), f"request {r}: other values that are no numbers"
+                off = (got - want)[fine].abs().max() if fine.any() else 0.0
+                assert off <= tol, f"request {r}: off by {float(off):.3e} > {tol:.1e}"
+        assert torch.equal(self.out[self.start[-1]:], before[self.start[-1]:])   # rows behind the last request's stay
+        return self.out.clone()
+
+
+HEADS = [(32, 4, 64), (32, 4, 128), (4, 1, 64), (6, 2, 128), (16, 8, 64), (14, 7, 128), (12, 12, 64), (24, 24, 128), (64, 64, 64), (9, 3, 128), (20, 5, 64)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("heads,mul,hs", HEADS)
+def test_single_tokens(backend, heads, mul, hs, dtype):
+    Batch([0, 1, 15, 16, 17, 63, 64, 65, 300, 1000], [1] * 10, heads, mul, hs, dtype=dtype, pad=3).check(backend)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("heads,mul,hs", HEADS)
+def test_chunks(backend, heads, mul, hs, dtype):
+    for longest in (0, 1, 129):
+        Batch([0, 0, 7, 130, 64, 500, 31], [1, 70, 2, 129, 0, 33, 5], heads, mul, hs, P=32, dtype=dtype, pad=2).check(backend, longest_new=longest)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("cached,new,P", [(0, 1, 16), (0, 2, 1024), (5000, 1, 128), (0, 1000, 64), (3000, 300, 16), (17000, 9, 256), (0, 257, 16), (127, 128, 16), (128, 256, 16), (1, 255, 16)])
+def test_one_request(backend, cached, new, P, dtype):
+    Batch([cached], [new], 8, 4, 128, P=P, dtype=dtype).check(backend)
+    Batch([cached], [new], 4, 2, 64, P=P, dtype=dtype).check(backend, longest_new=new)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (2, 300), (16, 4), (63, 0), (64, 64), (100, 5), (129, 70), (400, 0), (1000, 200), (1 << 31, 0), (0xFFFFFFFF, 0xFFFFFFFF), (50, 0xFFFFFFFF)])
+def test_windows_and_sinks(backend, window, sinks, dtype):
+    Batch([0, 10, 700, 1500, 64, 333], [300, 1, 1, 65, 200, 8], 8, 4, 64, dtype=dtype).check(backend, window, sinks)
+    Batch([900, 2100], [140, 1], 8, 4, 128, P=64, dtype=dtype).check(backend, window, sinks)
+
+
+@pytest.mark.parametrize("gap,q_pad,offset", [(512, 0, 0), (64, 64, 0), (0, 3, 0), (0, 0, 1), (1024, 5, 2)])
+def test_strides_and_alignment(backend, gap, q_pad, offset):
+    for dtype in (torch.float16, torch.float32):
+        Batch([5, 100, 40], [3, 1, 150], 8, 2, 64, dtype=dtype, gap=gap, q_pad=q_pad, offset=offset, pad=2).check(backend)
+        Batch([5, 100], [1, 40], 4, 4, 128, dtype=dtype, gap=gap, q_pad=q_pad, offset=offset).check(backend, window=30, sinks=2)
+
+
+def test_agrees_with_the_contiguous_op(backend):
+    b = Batch([700], [1], 32, 4, 128)
+    b.run(backend)
+    k, v = b.rows[0]
+    out = torch.empty(32 * 128, device="cuda")
+    FusedAttention(backend).launch(AttnParams(701, 1024, 4, 32, 128, 700), b.q[0].contiguous(), k, v, out)
+    assert (out - b.out[0]).abs().max() <= 2e-6
+
+
+@pytest.mark.parametrize("n", [40, 127, 129, 200, 1000])
+def test_many_requests(backend, n):
+    """More requests than a CTA has threads, some without tokens; few units each and some long ones."""
+    g = torch.Generator().manual_seed(n)
+    cached, new = torch.randint(0, 60, (n,), generator=g).tolist(), torch.randint(0, 3, (n,), generator=g).tolist()
+    cached[n // 3], new[n // 2], new[0], new[-1] = 4000, 90, 0, 1
+    b = Batch(cached, new, 4, 2, 64)
+    assert n < 1000 or len(cached) > 320
+    b.check(backend, requests=[i for i in range(n) if i % 7 == 0 or new[i] > 3 or cached[i] > 100 or i == n - 1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("scale", [1e-12, 1e-3, 30.0, 1e6])
+def test_queries_of_any_size(backend, scale, dtype):
+    """(At 1e6 the softmax is a choice of the largest score: the bound on a weight grows with the scores, and the check is of the choice where that is clear.)"""
+    b = Batch([200, 64], [1, 70], 8, 4, 64, dtype=dtype, q_scale=scale)
+    if scale < 1e5:
+        b.check(backend)
+    else:
+        b.run(backend)
+        for r in range(2):
+            want, _ = b.exact(r)
+            k = b.rows[r][0].double().view(b.kv[r], 2, 64)
+            q = b.q[b.start[r]: b.start[r + 1]].double().view(-1, 8, 64)
+            for h in range(8):
+                s = q[:, h] @ k[:, h // 4].T
+                s = s.masked_fill(torch.arange(b.kv[r], device="cuda")[None] > torch.arange(b.cached[r], b.kv[r], device="cuda")[:, None], -math.inf)
+                top = s.topk(2, -1).values
+                clear = (top[:, 0] - top[:, 1]) / 8.0 > top[:, 0].abs() * 1e-5 + 30
+                got = b.out[b.start[r]: b.start[r + 1]].view(-1, 8, 64)[:, h]
+                assert clear.any() and (got.double() - want.view(-1, 8, 64)[:, h])[clear].abs().max() <= 1e-5
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("hs", [64, 128])
+def test_masked_positions_may_hold_anything(backend, hs, dtype):
+    """Infinities and NaN in rows of K and V that some rows of a tile see and others do not; the type's lowest and largest values."""
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    for new in (2, 40, 300):
+        b = Batch([50, 90], [new, 1], 8, 4, hs, dtype=dtype, seed=new)
+        b.put(0, 50 + new - 1, 1, float("nan"))       # the last token's V: only the last token sees it
+        b.put(0, 50 + new // 2, 1, float("inf"))
+        b.put(0, 50 + new // 2 + 1 if new > 2 else 0, 0, 0.0)
+        b.check(backend)
+        b = Batch([50, 90], [new, 1], 8, 4, hs, dtype=dtype, seed=new)
+        b.put(0, 50 + new - 1, 0, float("nan"))       # ... and its K
+        want, tol = b.exact(0)
+        b.run(backend)
+        assert torch.isnan(b.out[new - 1]).all() and (b.out[: new - 1].double() - want[: new - 1]).abs().max() <= tol
+        # behind the window
+        b = Batch([500], [new], 8, 4, hs, dtype=dtype, seed=new)
+        for j, value in ((3, float("inf")), (200, float("nan")), (380, -float("inf")), (500 - 101, float("nan"))):
+            b.put(0, j, 1, value)
+        b.check(backend, window=100, sinks=2)
+        # lowest and largest values: no overflow on the way where the result has none
+        b = Batch([40], [new], 8, 4, hs, dtype=dtype, seed=new)
+        b.put(0, 5, 1, high / 4)
+        b.put(0, 40 + new - 1, 1, low / 4)
+        b.check(backend)
+
+
+def test_lengths_that_do_not_fit_together(backend):
+    """Fewer cached positions than new tokens: the tokens at positions below 0 see nothing and get 0; rows never leave q."""
+    b = Batch([4, 4], [6, 3], 8, 4, 64)
+    b.kv_len = i32([2, 7])   # request 0: positions -4 .. 1
+    b.out.fill_(5.0)
+    b.run(backend)
+    assert (b.out[:4] == 0).all() and torch.isfinite(b.out).all() and (b.out[4:6] != 0).any()
+    assert torch.allclose(b.out[6:9].double(), b.exact(1)[0], atol=1e-5)
+    for starts, kv in (([0, 9, 4], [10, 7]), ([-5, 6, 900], [10, 7]), ([3, 3, 3], [10, 7]), ([0, 6, 9], [-4, 1 << 30])):
+        b.row_start, b.kv_len = i32(starts), i32(kv)
+        b.run(backend)
+    torch.cuda.synchronize()
+
+
+def test_pages_outside_the_cache_do_not_reach_other_requests(backend):
+    for longest in (0, 1, 50):
+        b = Batch([200, 300, 90], [1, 50, 1], 8, 4, 128)
+        for page in (-1, b.n_pages, 1 << 30, -(1 << 31)):
+            b.table[0, 3] = page
+            b.table[0, 0] = page
+            b.check(backend, longest_new=longest, requests=[1, 2])
+
+
+def test_nothing_to_do(backend):
+    b = Batch([5, 6], [0, 0], 8, 4, 64, pad=4)
+    b.check(backend)
+    before = backend.launch_count()
+    e = torch.zeros(0, 512, device="cuda")
+    PagedAttention(backend).launch(PagedAttentionConfig(8, 4, 64), e, b.kc, b.vc, b.table, b.row_start, b.kv_len, e)
+    PagedAttention(backend).launch(PagedAttentionConfig(8, 4, 64), b.q, b.kc, b.vc, b.table[:0], i32([0]), i32([]), b.out)
+    assert backend.launch_count() == before
+
+
+def test_results_repeat_bit_for_bit(backend):
+    b = Batch([3000, 77, 900, 12000], [1, 300, 40, 1], 32, 4, 128, P=64)
+    first = b.check(backend)
+    for _ in range(5):
+        assert torch.equal(b.run(backend), first)
+
+
+def test_captured_first_call_and_replay_with_other_lengths(backend):
+    """A context's first call while a stream is being captured; then lengths change and the graph is replayed."""
+    own = Backend(0)
+    b = Batch([800, 90, 0], [1, 60, 30], 8, 4, 64, pad=10)
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        b.run(own)
+    graph.replay()
+    torch.cuda.synchronize()
+    for r in range(3):
+        want, tol = b.exact(r)
+        assert (b.out[b.start[r]: b.start[r + 1]].double() - want).abs().max() <= tol
+    b.new, b.kv, b.start = [2, 1, 20], [500, 80, 25], [0, 2, 3, 23]
+    b.rows = [(k[:n], v[:n]) for (k, v), n in zip(b.rows, b.kv)]
+    b.row_start.copy_(i32(b.start))
+    b.kv_len.copy_(i32(b.kv))
+    before = b.out.clone()
+    graph.replay()
+    torch.cuda.synchronize()
+    for r in range(3):
+        want, tol = b.exact(r)
+        assert (b.out[b.start[r]: b.start[r + 1]].double() - want).abs().max() <= tol
+    assert torch.equal(b.out[23:], before[23:])
+    del graph
+    own.close()
+
+
+def test_two_contexts_side_by_side(backend):
+    """Calls on two streams, a context each."""
+    other = Backend(0)
+    batches = [Batch([3000, 500], [1, 70], 8, 4, 128, seed=s) for s in (1, 2)]
+    want = [b.check(backend) for b in batches]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for b, c, s in zip(batches, (backend, other), streams):
+            with torch.cuda.stream(s):
+                b.run(c)
+    torch.cuda.synchronize()
+    for b, w in zip(batches, want):
+        assert torch.equal(b.out, w)
+    other.close()
+
+
+def test_a_cache_beyond_32_bit_offsets(backend):
+    """Pages whose elements lie behind 2^32 bytes and 2^31 elements."""
+    P, kv_dim, n_pages = 1024, 1024, 2200   # 2.3e9 elements
+    kc = torch.empty(n_pages, P, kv_dim, dtype=torch.float16, device="cuda")
+    vc = torch.empty(n_pages, P, kv_dim, dtype=torch.float16, device="cuda")
+    for cached, new in ((1500, 1), (1100, 200)):
+        b = Batch([cached], [new], 32, 4, 128, P=P)
+        b.table[0, :2] = i32([n_pages - 1, n_pages - 2])
+        for c, rows in ((kc, b.rows[0][0]), (vc, b.rows[0][1])):
+            c[n_pages - 1], c[n_pages - 2, : b.kv[0] - P] = rows[:P], rows[P:]
+        b.kc, b.vc, b.n_pages = kc, vc, n_pages
+        b.check(backend)
+
+
+def test_refusals(backend):
+    b = Batch([20, 30], [1, 2], 8, 4, 64)
+
+    def refused(message, heads=8, mul=4, hs=64, window=0, sinks=0, q=b.q, kc=b.kc, vc=b.vc, table=b.table, starts=b.row_start, kv=b.kv_len, out=b.out):
+        with pytest.raises(InferiError, match=message):
+            PagedAttention(backend).launch(PagedAttentionConfig(heads, mul, hs, window, sinks), q, kc, vc, table, starts, kv, out)
+
+    refused("kv_mul=3", mul=3)
+    refused("kv_mul=0", mul=0)
+    refused("kv_mul=128", heads=128, mul=128, q=torch.zeros(3, 128 * 64, device="cuda"), out=torch.zeros(3, 128 * 64, device="cuda"))
+    refused("q: expected", hs=128)
+    refused("head_size=32", hs=32, q=torch.zeros(3, 256, device="cuda"), out=torch.zeros(3, 256, device="cuda"))
+    refused("kv_dim=128", mul=8)
+    refused("q: expected", q=b.q.half())
+    refused("out: expected", out=b.out[:2])
+    refused("window: -1", window=-1)
+    refused("sinks", sinks=1 << 32)
+    refused("row_start", starts=b.row_start[:2])
+    refused("row_start", starts=b.row_start.long())
+    refused("block_table: expected", table=b.table.T.contiguous().T)
+    refused("block table", table=b.table[:1])
+    refused("on device", kv=b.kv_len.cpu())
+    refused("float16 or both float32", vc=b.vc.float())
+    refused("contiguous pages", kc=b.kc.transpose(0, 1), vc=b.vc.transpose(0, 1))
+    assert backend.lib.ib_paged_attention(backend.handle, None, None, None) == 1
