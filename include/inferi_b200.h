@@ -243,6 +243,29 @@ typedef struct ib_paged_attn_args {
 } ib_paged_attn_args;
 IB_API int32_t ib_paged_attention(ib_ctx *ctx, void *stream, const ib_paged_attn_args *args, const ib_paged_cache *cache);
 
+/* A token for every row of logits [rows][vocab] (`stride` floats apart), each with settings of its own.  All arrays are on the device, one element per row:
+ *   temperature   above 0; others, NaN among them: the arg-max, lowest index on ties
+ *   top_k         the k largest logits (ties: lowest index); others than 1 .. vocab - 1: no limit.  NULL: none for any row
+ *   top_p         the fewest of those whose sum exceeds top_p times their sum; outside (0, 1): no limit.  NULL: none
+ *   min_p         tokens with at least min_p times the largest probability; 0 and below: no limit.  NULL: none.  (One token is always left.)
+ *   coin          the caller's random number in [0, 1)
+ *   token         which token it is: in the order of probabilities, ties by index, the first at which the running sum of what is left exceeds coin times its sum; rows
+ *                 without a limit: the same in the order of indices.  (ib_sample's rules, where it offers the same.)
+ *   prob          the token's share of what was left (1 for the arg-max).  May be NULL
+ * Logits are not modified; NaN counts as -infinity, which is never drawn, and +infinity as the largest float; a row without a number gives token 0.  Sums are exact in units of 2^-44 of the
+ * largest probability, and weights are good to 2^-31.  vocab up to 524288. */
+typedef struct ib_sample_batch_args {
+    const float *logits_dev;
+    uint64_t stride;
+    uint32_t rows, vocab;
+    const float *temperature;
+    const int32_t *top_k;
+    const float *top_p, *min_p, *coin;
+    int32_t *token;
+    float *prob;
+} ib_sample_batch_args;
+IB_API int32_t ib_sample_batch(ib_ctx *ctx, void *stream, const ib_sample_batch_args *args);
+
 /* = `Llama2Config` (crates/inferi/src/models/llama2/cpu.rs:46-66). */
 typedef struct ib_llama_config {
     uint32_t hidden_size;

@@ -54,6 +54,12 @@ class PagedAttnArgs(C.Structure):
         (n, C.c_uint32) for n in ("n_requests", "n_tokens", "max_pages", "n_heads", "kv_mul", "head_size", "window", "sinks", "longest_new")]
 
 
+class SampleBatchArgs(C.Structure):
+    """= ib_sample_batch_args"""
+    _fields_ = [("logits_dev", C.c_void_p), ("stride", C.c_uint64), ("rows", C.c_uint32), ("vocab", C.c_uint32)] + [
+        (n, C.c_void_p) for n in ("temperature", "top_k", "top_p", "min_p", "coin", "token", "prob")]
+
+
 class LlamaConfig(C.Structure):
     """= Llama2Config (crates/inferi/src/models/llama2/cpu.rs:46-66)."""
     _fields_ = [(n, C.c_uint32) for n in ("hidden_size", "intermediate_size", "num_hidden_layers", "num_attention_heads",
@@ -110,6 +116,7 @@ SIGNATURES = {
     "ib_page_plan": (_i32, [_vp, _vp, C.POINTER(PagePlanArgs)]),
     "ib_paged_append": (_i32, [_vp, _vp, C.POINTER(PagedAppendArgs), C.POINTER(PagedCache)]),
     "ib_paged_attention": (_i32, [_vp, _vp, C.POINTER(PagedAttnArgs), C.POINTER(PagedCache)]),
+    "ib_sample_batch": (_i32, [_vp, _vp, C.POINTER(SampleBatchArgs)]),
     "ib_llama_set_sampler": (_i32, [_vp, _f, _f, _u64]),
     "ib_llama_generate_until": (_i32, [_vp, _vp, _vp, _u32, _u32, _u32, _u32, _vp, C.POINTER(_u32)]),
     "ib_llama_chat": (_i32, [_vp, _vp, _vp, _u32, _u32, _u32, _u32, TOKEN_EVENT_FN, _vp, C.POINTER(_u32)]),

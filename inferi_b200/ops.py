@@ -15,7 +15,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import AttnParams, InferiError, KV_F16, KV_F32, PagedAppendArgs, PagedAttnArgs, PagedCache, PagePlanArgs, ROPE_NEOX, ROPE_ORIGINAL, check  # noqa: F401
+from ._lib import AttnParams, InferiError, KV_F16, KV_F32, PagedAppendArgs, PagedAttnArgs, PagedCache, PagePlanArgs, ROPE_NEOX, ROPE_ORIGINAL, SampleBatchArgs, check  # noqa: F401
 from .build import binding_stamp
 from .quant import BLOCK_BYTES, BLOCK_ELEMS, F32, NAMES, Q4_K, Q5_K, Q6_K, Q8_0, row_bytes  # noqa: F401
 
@@ -490,3 +490,33 @@ class PagedAttention:
         a = PagedAttnArgs(pq, po, sq, so, _i32_dev(block_table, "block_table"), _i32_dev(row_start, "row_start", n + 1), _i32_dev(kv_len, "kv_len"), n, _u32(q.shape[0], "rows"),
                           block_table.shape[1], *counts)
         check(b.lib.ib_paged_attention(b.handle, _stream_ptr(), C.byref(a), C.byref(c)))
+
+
+class BatchSampler:
+    """`Sampler` for a batch of rows with settings of their own (`ib_sample_batch`: the rules)."""
+
+    def __init__(self, backend: Backend, vocab_size: int):
+        self.backend, self.vocab_size = backend, vocab_size
+
+    def sample(self, logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor | None, top_p: torch.Tensor | None, min_p: torch.Tensor | None, coin: torch.Tensor,
+               token: torch.Tensor | None = None, prob: torch.Tensor | None = None) -> torch.Tensor:
+        """logits: [n, vocab_size] float32 with contiguous rows; temperature, top_p, min_p and coin: [n] float32, top_k: [n] int32 (None: no row has that limit).  token [n] int32 (made
+        if None) and, if given, prob [n] float32 are written; returns token."""
+        b, n = self.backend, logits.shape[0]
+        token = token if token is not None else torch.empty(n, dtype=torch.int32, device=logits.device)
+        given = [(name, t) for name, t in (("logits", logits), ("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p), ("coin", coin), ("token", token), ("prob", prob))
+                 if t is not None]
+        _on_device(b, *given)
+        x, stride = _f32_rows(logits, "logits", None, self.vocab_size)
+
+        def f32(t, name):
+            if t is None:
+                return None
+            if t.dtype is not _f32 or not t.is_contiguous() or t.numel() != n:
+                raise InferiError(1, f"{name}: expected a contiguous float32 tensor of {n} elements")
+            return t.data_ptr()
+
+        a = SampleBatchArgs(x, stride, _u32(n, "rows"), self.vocab_size, f32(temperature, "temperature"), _i32_dev(top_k, "top_k", n) if top_k is not None else None, f32(top_p, "top_p"),
+                            f32(min_p, "min_p"), f32(coin, "coin"), _i32_dev(token, "token", n), f32(prob, "prob"))
+        check(b.lib.ib_sample_batch(b.handle, _stream_ptr(), C.byref(a)))
+        return token

@@ -1,0 +1,218 @@
+"""Sampling of a batch of rows with settings of their own, against the definition in 64 bits."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from inferi_b200.ops import BatchSampler, InferiError, Sampler
+
+pytestmark = pytest.mark.gpu
+
+
+def choose(x, T, k, top_p, min_p, coin):
+    """(token, probability) of one row, in 64 bits (weights exact to 2^-52 here, to 2^-31 in the kernel: a border would have to be that near to a coin)."""
+    x = np.where(np.isnan(x), -np.inf, np.minimum(x.astype(np.float64), np.finfo(np.float32).max))
+    if not T > 0 or x.max() == -np.inf:
+        return int(np.argmax(x)), 1.0
+    with np.errstate(over="ignore", under="ignore"):
+        w = np.exp((x - x.max()) / float(np.float32(T)))
+    n = len(x)
+    by_k, by_p, by_min = 0 < k < n, 0 < top_p < 1, min_p > 0
+    order = np.lexsort((np.arange(n), -x)) if by_k or by_p or by_min else np.arange(n)
+    w = w[order]
+    m = k if by_k else n
+    sums = np.cumsum(w)
+    if by_min:
+        least = max(1, int((w >= float(np.float32(min_p))).sum()))
+    if by_p:
+        m = min(m, int((sums[:m] <= float(np.float32(top_p)) * sums[m - 1]).sum()) + 1)
+    if by_min:
+        m = min(m, least)
+    at = min(int((sums[:m] <= float(np.float32(coin)) * sums[m - 1]).sum()), m - 1)
+    return int(order[at]), float(w[at] / sums[m - 1])
+
+
+def run(backend, logits, T, k, top_p, min_p, coin):
+    """Lists, or None where no row has that limit."""
+    f = lambda v: None if v is None else torch.tensor(v, dtype=torch.float32, device="cuda")   # noqa: E731
+    n = logits.shape[0]
+    token, prob = torch.full((n,), -7, dtype=torch.int32, device="cuda"), torch.full((n,), -7.0, device="cuda")
+    BatchSampler(backend, logits.shape[1]).sample(logits, f(T), None if k is None else torch.tensor(k, dtype=torch.int32, device="cuda"), f(top_p), f(min_p), f(coin), token, prob)
+    return token.tolist(), prob.tolist()
+
+
+def check(backend, logits, T, k, top_p, min_p, coin):
+    tokens, probs = run(backend, logits, T, k, top_p, min_p, coin)
+    x = logits.cpu().numpy()
+    for r in range(len(tokens)):
+        want, p = choose(x[r], T[r], k[r] if k else 0, top_p[r] if top_p else 1.0, min_p[r] if min_p else 0.0, coin[r])
+        assert tokens[r] == want, f"row {r}: token {tokens[r]} instead of {want} (T {T[r]}, k {k and k[r]}, top_p {top_p and top_p[r]}, min_p {min_p and min_p[r]}, coin {coin[r]})"
+        # a weight and a sum, each to 2^-31 and 2^-44 of the largest weight per token, rounded to 32 bits
+        assert abs(probs[r] - p) <= p * (2**-24 + 2**-29) + x.shape[1] * 2**-44, (r, probs[r], p)
+
+
+def settings(n, seed):
+    rng = np.random.default_rng(seed)
+    pick = np.arange(n) % 8
+    T = (0.3 + 1.4 * rng.random(n)).astype(np.float32).tolist()
+    k = np.where(pick & 1, rng.integers(1, 300, n), 0).tolist()
+    top_p = np.where(pick & 2, 0.3 + 0.69 * rng.random(n), 1.0).tolist()
+    min_p = np.where(pick & 4, 0.3 * rng.random(n) ** 2, 0.0).tolist()
+    return T, k, top_p, min_p, rng.random(n).astype(np.float32).clip(max=1 - 2**-24).tolist()
+
+
+@pytest.mark.parametrize("sharp", [0.01, 0.7, 3.0, 30.0])
+@pytest.mark.parametrize("vocab", [1, 2, 31, 512, 1000, 4096, 4097, 32003, 128256])
+def test_against_the_definition(backend, vocab, sharp):
+    n = 24
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    logits = torch.randn(n, vocab, generator=g, device="cuda") * sharp
+    check(backend, logits, *settings(n, vocab))
+    if vocab > 100:   # one filter alone, and none
+        T, k, top_p, min_p, coin = settings(n, vocab + 1)
+        for use in (0, 1, 2, 3):
+            check(backend, logits, T, [5] * n if use == 1 else None, [0.9] * n if use == 2 else None, [0.02] * n if use == 3 else None, coin)
+
+
+@pytest.mark.parametrize("vocab", [371000, 524288])
+def test_vocabularies_that_shared_memory_does_not_hold(backend, vocab):
+    logits = torch.randn(8, vocab, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda") * 2
+    check(backend, logits, *settings(8, 3))
+
+
+@pytest.mark.parametrize("vocab", [50, 5000, 40000])
+def test_ties(backend, vocab):
+    """Equal logits: weights are equal, and index order decides.  Rows of one value, of two, of a few; a largest one that many tokens share."""
+    rng = np.random.default_rng(vocab)
+    rows = [np.zeros(vocab), np.where(np.arange(vocab) % 3 == 0, 1.0, 0.0), rng.integers(0, 4, vocab).astype(float), np.where(rng.random(vocab) < 0.5, 2.0, -np.inf),
+            np.where(np.arange(vocab) >= vocab - 3, 0.0, -40.0)]
+    logits = torch.tensor(np.stack(rows * 8), dtype=torch.float32, device="cuda")
+    n = logits.shape[0]
+    T, k, top_p, min_p, coin = settings(n, 7)
+    pick = np.arange(n) // 5   # every kind of row with every combination of limits
+    k, top_p, min_p = [np.where(pick & b, on, off).tolist() for b, on, off in ((1, vocab // 3 + 1, 0), (2, 0.6, 1.0), (4, 0.5, 0.0))]
+    check(backend, logits, T, k, top_p, min_p, coin)
+    check(backend, logits, [1.0] * n, [1] * n, None, None, coin)          # the first of the largest
+    check(backend, logits, [1.0] * n, None, None, [1.0] * n, coin)        # all of the largest
+    check(backend, logits, [1.0] * n, None, None, [1.5] * n, coin)        # the first alone
+    check(backend, logits, [1.0] * n, [vocab - 1] * n, None, None, coin)
+
+
+def test_coins_at_the_ends(backend):
+    """Coin 0 is the first token that can come, a coin just below 1 the last one that is left."""
+    logits = torch.tensor([[-math.inf, 0.0, -1.0, -math.inf, -50.0, -math.inf]] * 4, device="cuda")
+    for coin, index, ranked in ((0.0, 1, 1), (1 - 2**-24, 2, 2)):
+        tokens, _ = run(backend, logits, [1.0] * 4, [0, 2, 0, 0], [1.0, 1.0, 0.99, 1.0], [0.0, 0.0, 0.0, 0.1], [coin] * 4)
+        assert tokens == [index, ranked, ranked, ranked]
+
+
+def test_limits_that_are_none(backend):
+    logits = torch.randn(8, 3000, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda")
+    coin = [0.1, 0.5, 0.9, 0.99, 0.3, 0.7, 0.2, 0.05]
+    want = run(backend, logits, [0.8] * 8, None, None, None, coin)
+    nan, inf = float("nan"), float("inf")
+    assert run(backend, logits, [0.8] * 8, [0, -1, 3000, 3001, 2**31 - 1, -2**31, 0, 0], [1.0, 0.0, -1.0, nan, 2.0, inf, -inf, 1.0], [0.0, -1.0, nan, -inf, 0.0, -0.0, nan, 0.0], coin) == want
+    # a row with a limit that keeps all of it, in the order of probabilities
+    check(backend, logits, [0.8] * 8, [2999] * 8, [1 - 2**-24] * 8, [1e-30] * 8, coin)
+
+
+def test_temperatures(backend):
+    logits = torch.randn(9, 5000, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda") * 3
+    logits[:, 77] = logits[:, 4000] = logits.max() + 1
+    T = [0.0, -1.0, float("nan"), -float("inf"), 1e-6, 1e-30, 100.0, 1e6, 1e-2]
+    tokens, probs = run(backend, logits, T, [0] * 9, [0.9] * 9, [0.0] * 9, [0.75] * 9)
+    assert tokens[:4] == [77] * 4 and probs[:4] == [1.0] * 4
+    assert tokens[4:6] == [4000] * 2 and probs[4:6] == [0.5] * 2    # two largest ones share everything
+    check(backend, logits[6:], T[6:], None, [0.9] * 3, None, [0.75] * 3)
+    check(backend, logits[6:], T[6:], None, None, None, [0.75] * 3)
+
+
+def test_logits_that_are_no_numbers(backend):
+    x = torch.randn(6, 700, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda")
+    x[0] = float("nan")
+    x[1] = -math.inf
+    x[2, ::2] = float("nan")
+    x[3, 50] = x[3, 60] = math.inf
+    x[4, 1:] = -math.inf
+    x[5] = torch.finfo(torch.float32).min
+    x[5, 9] = torch.finfo(torch.float32).max
+    coin = [0.6] * 6
+    for limits in ((None, None, None), ([3] * 6, [0.9] * 6, [0.1] * 6)):
+        check(backend, x, [1.0] * 6, *limits, coin)
+    assert run(backend, x, [0.0] * 6, None, None, None, coin)[0] == [0, 0, int(torch.where(x[2].isnan(), -math.inf, x[2]).argmax()), 50, 0, 9]
+
+
+def test_agrees_with_the_sampler_of_one_row(backend):
+    """Temperature and top-p are what `Sampler` makes of them (32-bit probabilities there: coins are kept away from borders)."""
+    logits = torch.randn(1, 8000, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda") * 4
+    for T, top_p in ((0.9, 0.8), (0.7, 1.0), (1.3, 0.95)):
+        x = logits[0].double().cpu().numpy()
+        w = np.exp((x - x.max()) / float(np.float32(T)))
+        order = np.argsort(-x, kind="stable") if top_p < 1 else np.arange(8000)
+        w = w[order]
+        m = int((np.cumsum(w) <= top_p * w.sum()).sum()) + 1 if top_p < 1 else 8000
+        sums = np.cumsum(w[:m]) / w[:m].sum()
+        for at in np.argsort(-w[:m])[:6]:
+            coin = float(np.float32(sums[at] - w[at] / w[:m].sum() / 2))
+            one = Sampler(backend, 8000, T, top_p).sample(logits[0], coin).item()
+            assert run(backend, logits, [T], None, [top_p], None, [coin])[0] == [one] == [order[at]]
+
+
+def test_strided_rows_and_no_probabilities(backend):
+    store = torch.randn(5, 1300, generator=torch.Generator(device="cuda").manual_seed(6), device="cuda")
+    for cut in (store[:, :1000], store[:, 3:1004], store[1:2, 7:900]):
+        n = cut.shape[0]
+        T, coin = torch.full((n,), 0.9, device="cuda"), torch.full((n,), 0.4, device="cuda")
+        k = torch.full((n,), 20, dtype=torch.int32, device="cuda")
+        s = BatchSampler(backend, cut.shape[1])
+        got = s.sample(cut, T, k, None, None, coin)
+        assert got.dtype == torch.int32 and torch.equal(got, s.sample(cut.contiguous(), T, k, None, None, coin, torch.empty_like(got), torch.empty_like(T)))
+        check(backend, cut, [0.9] * n, [20] * n, None, None, [0.4] * n)
+
+
+def test_many_rows_captured(backend):
+    n, vocab = 700, 9000
+    logits = torch.randn(n, vocab, generator=torch.Generator(device="cuda").manual_seed(8), device="cuda") * 3
+    T, k, top_p, min_p, coin = settings(n, 8)
+    check(backend, logits, T, k, top_p, min_p, coin)
+    f = lambda v: torch.tensor(v, dtype=torch.float32, device="cuda")   # noqa: E731
+    args = (f(T), torch.tensor(k, dtype=torch.int32, device="cuda"), f(top_p), f(min_p), f(coin))
+    token = torch.empty(n, dtype=torch.int32, device="cuda")
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        BatchSampler(backend, vocab).sample(logits, *args, token)
+    args[-1].copy_(f(coin[::-1]))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert token.tolist() == run(backend, logits, T, k, top_p, min_p, coin[::-1])[0]
+
+
+def test_no_rows(backend):
+    e, before = torch.zeros(0, device="cuda"), backend.launch_count()
+    assert BatchSampler(backend, 100).sample(torch.zeros(0, 100, device="cuda"), e, None, None, None, e).numel() == 0
+    assert backend.launch_count() == before
+
+
+def test_refusals(backend):
+    x, one, i = torch.zeros(3, 100, device="cuda"), torch.zeros(3, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+
+    def refused(message, vocab=100, x=x, T=one, k=i, p=one, m=one, coin=one, token=i, prob=one):
+        with pytest.raises(InferiError, match=message):
+            BatchSampler(backend, vocab).sample(x, T, k, p, m, coin, token, prob)
+
+    refused("logits: expected", vocab=101)
+    refused("logits: expected", x=x.half())
+    refused("logits: expected", x=torch.zeros(3, 200, device="cuda")[:, ::2])
+    refused("temperature", T=one[:2])
+    refused("top_k", k=one)
+    refused("top_p", p=one.double())
+    refused("min_p", m=torch.zeros(6, device="cuda")[::2])
+    refused("coin", coin=i)
+    refused("token", token=i.long())
+    refused("prob", prob=i)
+    refused("on device", coin=one.cpu())
+    refused("524289 tokens", vocab=524289, x=torch.zeros(3, 524289, device="cuda"))
+    refused("0 tokens", vocab=0, x=torch.zeros(3, 0, device="cuda"))
+    assert backend.lib.ib_sample_batch(backend.handle, None, None) == 1
