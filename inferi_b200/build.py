@@ -16,7 +16,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libinferi_b200.so")
 BINDING_PATH = os.path.join(PKG_DIR, "_binding" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))   # (another interpreter does not find it)
 BINDING_SOURCES = [os.path.join(CSRC, "binding.cpp"), os.path.join(PKG_DIR, "..", "include", "inferi_b200.h"), os.path.abspath(__file__)]
-SOURCES = ["api.cu", "gemv.cu", "gemv_stream.cu", "ops.cu", "attention.cu", "prefill.cu", "prefill_gemm.cu", "prefill_attention.cu", "llama.cu", "gguf.cu", "sampler.cu", "paged.cu", "paged_attention.cu", "paged_decode.cu", "batch_sampler.cu", "tokenizer.cu"]
+SOURCES = ["api.cu", "gemv.cu", "gemv_stream.cu", "ops.cu", "attention.cu", "prefill.cu", "prefill_gemm.cu", "prefill_attention.cu", "llama.cu", "gguf.cu", "sampler.cu", "paged.cu", "paged_attention.cu", "paged_decode.cu", "paged_chunk.cu", "batch_sampler.cu", "tokenizer.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr",

@@ -28,7 +28,8 @@ int32_t check_device_error(ib_ctx *ctx) {
                                        "another rank's partial sums never arrived", "another rank's arg-max candidate never arrived",
                                        "the consumer warps never finished a tile", "the input's sum of squares never completed",
                                        "this rank's reduction of the partial sums never completed", "a GEMM stage was never released by the tensor core",
-                                       "a GEMM stage was never filled", "the GEMM accumulator never completed"};
+                                       "a GEMM stage was never filled", "the GEMM accumulator never completed", "a tile of the paged cache never arrived in shared memory",
+                                       "the products of an attention tile never completed"};
     return set_error(IB_ERR_TIMEOUT, "a kernel gave up waiting (%s); results of that launch are invalid", e < sizeof(what) / sizeof(what[0]) ? what[e] : "unknown wait");
 }
 

@@ -6,11 +6,13 @@ namespace ib {
 int32_t check_paged_cache(const char *who, const ib_paged_cache *c);   // paged.cu
 uint32_t log2_of(uint32_t power);
 
+constexpr uint32_t PAGED_FEW_ROWS = 16;
+
 // Scratch of a context, of one size whatever the arguments: made once and never moved, so a captured launch may be replayed at any time.  (Made while a stream is being
 // captured, it is cleared on a stream of its own: the capture does not get the clearing as a node.)
 static int32_t ensure_paged_scratch(ib_ctx *ctx) {
     if (ctx->paged_scratch) return IB_OK;
-    const size_t floats = paged_decode_scratch_floats(ctx, 128), counters = paged_decode_ctas(ctx);
+    const size_t of_decode = paged_decode_scratch_floats(ctx, 128), floats = of_decode + paged_chunk_scratch_floats(ctx, 128), counters = paged_decode_ctas(ctx) + 2 * paged_chunk_ctas(ctx);
     BesideCaptures beside;
     float *scratch = nullptr;
     cudaStream_t own = nullptr;
@@ -58,9 +60,24 @@ extern "C" int32_t ib_paged_attention(ib_ctx *ctx, void *stream, const ib_paged_
     a.kv_heads = p.n_heads / p.kv_mul; a.kv_mul = p.kv_mul; a.kv_dim = cache->kv_dim;
     a.window = p.window; a.sinks = p.sinks;
     a.vec = (uintptr_t)p.q_dev % 16 == 0 && (uintptr_t)p.out_dev % 16 == 0 && p.q_stride % 4 == 0 && p.out_stride % 4 == 0;
-    a.scratch = ctx->paged_scratch; a.counters = ctx->paged_counters;
     a.err = ctx->err_dev; a.wait_ns = ctx->wait_limit_ns;
-    a.rows_from = 1;
+    // Requests with few rows go through tiles of 8, the others through tiles of 256.  The host knows no lengths: where requests of either kind can be there, both kernels are launched, each for
+    // its own.  One that is alone takes all of them, whatever they turn out to be.
+    const uint64_t most = (uint64_t)(p.longest_new && p.longest_new < p.n_tokens ? p.longest_new : p.n_tokens) * p.kv_mul;
+    const bool chunks = most > PAGED_FEW_ROWS && paged_chunk_takes(a, cache->kv_dtype), few = !chunks || p.n_requests > 1;
+    const uint32_t border = chunks && few ? PAGED_FEW_ROWS : (chunks ? 0u : 0xFFFFFFFFu);
+    if (few) {
+        a.scratch = ctx->paged_scratch;
+        a.counters = ctx->paged_counters;
+        a.rows_from = 1;
+        a.rows_to = border;
+        rc = launch_paged_decode(ctx, (cudaStream_t)stream, a, p.head_size, cache->kv_dtype);
+        if (rc) return rc;
+    }
+    if (!chunks) return IB_OK;
+    a.scratch = ctx->paged_scratch + paged_decode_scratch_floats(ctx, 128);
+    a.counters = ctx->paged_counters + paged_decode_ctas(ctx);
+    a.rows_from = border + 1;
     a.rows_to = 0xFFFFFFFFu;
-    return launch_paged_decode(ctx, (cudaStream_t)stream, a, p.head_size, cache->kv_dtype);
+    return launch_paged_chunk(ctx, (cudaStream_t)stream, a, p.head_size);
 }

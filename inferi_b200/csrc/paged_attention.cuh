@@ -276,27 +276,36 @@ __device__ __forceinline__ int paged_exponent(float most) {
 // the row's largest score (rounded up, in units of log2) known - unless its sum of weights is none either: then it sees a key, or is a query, that is none, and all of the row is rightly
 // so.  Called by a whole warp.
 template <typename T>
-__device__ __noinline__ void paged_repair(const PagedAttn &a, uint32_t KT, uint32_t request, uint32_t kv_head, const KeySpan span, long long p, float most, const float *q, float *out, uint32_t hs) {
+static __device__ __noinline__ void paged_repair(const PagedAttn &a, uint32_t KT, uint32_t request, uint32_t kv_head, const KeySpan span, long long p, float most, const float *q, float *out, uint32_t hs) {
     const uint32_t lane = threadIdx.x & 31, E = hs / 32;
     const float scale = 1.4426950408889634f / sqrtf((float)hs);
     float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t u = 0; u < span.units; u++) {
-        const long long base = (long long)key_tile(span, u) * KT;
-        for (long long j = base; j < min(base + KT, (long long)span.end); j++) {
-            if (!paged_sees(a, p, j)) continue;
-            const int32_t page = a.table[(size_t)request * a.max_pages + ((uint32_t)j >> a.page_log2)];
-            if (page < 0 || (uint32_t)page >= a.n_pages) continue;
-            const uint64_t at = (uint64_t)page * a.page_stride + (uint64_t)((uint32_t)j & ((1u << a.page_log2) - 1)) * a.kv_dim + kv_head * hs + lane;
-            const T *k = static_cast<const T *>(a.k) + at, *v = static_cast<const T *>(a.v) + at;
-            float s = 0.f;
-            for (uint32_t e = 0; e < E; e++) s += q[lane + 32 * e] * (float)k[32 * e];
-#pragma unroll
-            for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            const float x = fmaxf(paged_ex2(s * scale - most), 1e-38f);   // (not nothing: an infinity that is seen counts, however small its weight)
-            l += x;
-            for (uint32_t e = 0; e < E; e++) acc[e] += x * (float)v[32 * e];
+    for (uint32_t u = 0; u < span.units; u++)
+        for (uint32_t j0 = key_tile(span, u) * KT; j0 < min(key_tile(span, u) * KT + KT, span.end); j0 += 32) {
+            // a lane's position: its weight, then everybody's elements of all 32
+            const uint32_t j = j0 + lane;
+            uint64_t at = ~0ull;
+            float x = 0.f;
+            if (j < span.end && paged_sees(a, p, j)) {
+                const int32_t page = a.table[(size_t)request * a.max_pages + (j >> a.page_log2)];
+                if (page >= 0 && (uint32_t)page < a.n_pages) {
+                    at = (uint64_t)page * a.page_stride + (uint64_t)(j & ((1u << a.page_log2) - 1)) * a.kv_dim + kv_head * hs;
+                    const T *k = static_cast<const T *>(a.k) + at;
+                    float s = 0.f;
+#pragma unroll 8
+                    for (uint32_t e = 0; e < hs; e++) s += q[e] * (float)k[e];
+                    x = fmaxf(paged_ex2(s * scale - most), 1e-38f);   // (not nothing: an infinity that is seen counts, however small its weight)
+                }
+            }
+#pragma unroll 4
+            for (int i = 0; i < 32; i++) {
+                const uint64_t from = __shfl_sync(0xffffffffu, at, i);
+                const float y = __shfl_sync(0xffffffffu, x, i);
+                if (from == ~0ull) continue;
+                l += y;
+                for (uint32_t e = 0; e < E; e++) acc[e] += y * (float)static_cast<const T *>(a.v)[from + lane + 32 * e];
+            }
         }
-    }
     for (uint32_t e = 0; e < E; e++) out[lane + 32 * e] = acc[e] / l;
 }
 
@@ -305,5 +314,12 @@ constexpr uint32_t PAGED_DECODE_ROWS = 8;
 size_t paged_decode_scratch_floats(const ib_ctx *ctx, uint32_t head_size);
 uint32_t paged_decode_ctas(const ib_ctx *ctx);
 int32_t launch_paged_decode(ib_ctx *ctx, cudaStream_t s, PagedAttn a, uint32_t head_size, int kv_dtype);
+
+
+// paged_chunk.cu
+uint32_t paged_chunk_ctas(const ib_ctx *ctx);
+size_t paged_chunk_scratch_floats(const ib_ctx *ctx, uint32_t head_size);
+bool paged_chunk_takes(const PagedAttn &a, int kv_dtype);
+int32_t launch_paged_chunk(ib_ctx *ctx, cudaStream_t s, PagedAttn a, uint32_t head_size);
 
 }  // namespace ib

@@ -1,0 +1,536 @@
+// Attention over a paged cache (f16) for requests with many rows: chunks of a prompt, on the 5th-generation tensor cores.
+//
+// A query tile is 256 rows (tokens x heads of a kv head), two halves of 128 rows; a key tile is 128 positions.  Per half and key tile:
+//     S[128 x 128] = Q K^T        Q from shared memory (two operands, hi and lo), K from shared memory; f32 sums in tensor memory
+//     P = 2^(S f - m)             a thread per row; P replaces S in tensor memory, as two f16 operands, hi and lo
+//     O[128 x HS] = P V           P from tensor memory, V from shared memory, f32 sums in tensor memory
+//     acc = 2^(m' - m) acc + O    in registers, HS of them per thread
+// q = hi + lo and P = hi + lo hold about 22 bits, K and V are exact, so the result is as good as 32-bit arithmetic makes it; each product is two MMAs.  The sums of a tile go from tensor
+// memory to registers before the next one's: the tensor core truncates, and a chain of its additions over a long context would shrink the result.  With whole numbers m rescaling is exact.
+//
+// What bounds it: the MMAs.  Twice 4 * 128 * 128 * HS operations per half and key tile are 2048 clocks (HS 128); the exponentials are 1024 of the SM's special function units, and the
+// remaining work of a thread's 128 scores about 1000.  The halves take turns: while one is in softmax, the tensor cores do the other's products.  Two halves share a key tile's 64 KB, 16
+// bytes a clock and SM; a tile of 128 rows would take twice as much from L2, which is all that L2 has.
+//
+// Who does what (12 warps, one CTA per SM):
+//   warps 0-3, 4-7   a half each: thread = row.  Loads and splits q, softmax, fold, result
+//   warp 8           MMA issue
+//   warp 9           TMA copies of K and V: a ring of tiles, a copy per page and 64 columns, swizzled by 128 bytes
+//   warps 10, 11     nothing (registers change hands by groups of four warps)
+// They hand over through mbarriers.  Order of the MMAs: S0 S1 | O0 S0' O1 S1' | O0' S0'' ...: a half's softmax has the time of the other's two products.
+// Tensor memory (512 columns): S0 / P0, S1 / P1, O0, O1 of 128 columns each.  P's operands are interleaved by 16 positions, hi then lo, so that a thread overwrites only scores that it has read.
+//
+// Every wait is bounded; a wait that gives up raises the context's error word, and the kernel returns after freeing its tensor memory.
+#include "paged_attention.cuh"
+#include "tensor_core.cuh"
+
+namespace ib {
+
+constexpr uint32_t PC_THREADS = 384, PC_KT = 128, PC_ROWS = 256, PC_W_MMA = 8, PC_W_TMA = 9;
+// Registers: 384 threads at 168 are what the block is launched with; the halves' warps take 208 of them, the others keep 88 (2 * 128 * 208 + 128 * 88 = 384 * 168).
+constexpr uint32_t PC_REGS_HALF = 208, PC_REGS_OTHER = 88;
+constexpr uint32_t PC_S = 0, PC_O = 256;   // tensor memory columns; the halves' are 128 apart
+constexpr uint32_t PC_SMEM_LIMIT = 227 * 1024;
+constexpr float PC_SHIFT = 14.f;           // probabilities are held times 2^14 (the remainders of small ones stay above f16's smallest step)
+constexpr uint32_t pc_half(uint32_t hs) { return 128 * hs * 2; }       // bytes of 128 rows: a half's hi (= lo) operand, a tile of K or V
+constexpr uint32_t pc_slots(uint32_t hs) { return hs == 128 ? 3u : 8u; }
+constexpr uint32_t pc_smem(uint32_t hs) { return 1024 + (4 + pc_slots(hs)) * pc_half(hs) + 256; }
+static_assert(pc_smem(128) <= PC_SMEM_LIMIT && pc_smem(64) <= PC_SMEM_LIMIT, "shared memory");
+constexpr uint32_t pc_partial_floats(uint32_t hs) { return 128 * (hs + 2); }   // of a half
+
+// Descriptors of operands in shared memory: rows of 64 f16 (128 bytes), eight of them 1024 bytes, swizzled by 128 bytes.  K-major: further columns lie behind all rows, so a descriptor covers 64
+// columns.  MN-major (V: the product's columns run along the rows): `next` bytes to the following 64 columns, 1024 to the following 8 positions.
+__device__ __forceinline__ uint64_t pc_desc_k(uint32_t addr) { return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61; }
+__device__ __forceinline__ uint64_t pc_desc_mn(uint32_t addr, uint32_t next) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)(next >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// D[128 x N] (+)= A x B, both in shared memory
+__device__ __forceinline__ void pc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc),
+                 "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void pc_tma3d(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, int32_t z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)),
+                 "r"(x), "r"(y), "r"(z), "r"(bar)
+                 : "memory");
+}
+
+// The wait for loads from tensor memory, with the registers that they fill: nothing that reads those can be moved ahead of it
+__device__ __forceinline__ void pc_wait_ld(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
+                   "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void pc_sync_half(uint32_t half) {
+    if (half) asm volatile("bar.sync 2, 128;" ::: "memory");
+    else asm volatile("bar.sync 1, 128;" ::: "memory");
+}
+
+// Bounded wait without a function call: ptxas does not keep a caller's registers beyond the launch's number across one
+__device__ __forceinline__ bool pc_wait(uint32_t bar, uint32_t parity, const PagedAttn &a, uint32_t code) {
+    unsigned long long t0 = 0;
+    for (uint32_t tries = 1; !pg_try(bar, parity); tries++) {
+        if (tries & 1023) continue;   // (the clock takes a microsecond to read)
+        const unsigned long long t = pg_ns();
+        if (t0 == 0) t0 = t;
+        else if (t - t0 > a.wait_ns) {
+            *(volatile uint32_t *)a.err = code;
+            __threadfence_system();
+            return false;
+        }
+    }
+    return true;
+}
+
+struct PcMaps { CUtensorMap k, v; };
+
+template <int HS>
+__global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid_constant__ PagedAttn a, const TileShape shape, const __grid_constant__ PcMaps maps) {
+    constexpr uint32_t HALF = pc_half(HS), SLOTS = pc_slots(HS), COLS = HS / 64;   // column blocks of 64
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    __shared__ PagedRangeShared range_sh;
+    __shared__ uint32_t sm_last[2];
+    __shared__ PagedWalk<PC_KT> sm_walk[8];   // the halves' warps' walks, while their registers hold a tile's sums
+    const uint32_t q0 = pg_smem(smem), ring = q0 + 4 * HALF, bars = ring + SLOTS * HALF;   // Q: [half][hi, lo]
+    const uint32_t b_full = bars, b_empty = b_full + 8 * SLOTS, b_q = b_empty + 8 * SLOTS, b_s = b_q + 16, b_p = b_s + 16, b_o = b_p + 16, b_free = b_o + 16, s_tmem = b_free + 16;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const PagedRange range = paged_range<PC_KT, PC_THREADS>(a, shape, range_sh);
+    if (range.total == 0 || blockIdx.x >= range.ranges) return;
+    if (warp == 0 && lane == 0) {
+        for (uint32_t i = 0; i < 2 * SLOTS; i++) pg_bar_init(b_full + 8 * i, 1);
+        for (uint32_t h = 0; h < 2; h++) {
+            pg_bar_init(b_q + 8 * h, 4);      // a half's warps
+            pg_bar_init(b_s + 8 * h, 1);      // the MMAs' completion
+            pg_bar_init(b_p + 8 * h, 4);
+            pg_bar_init(b_o + 8 * h, 1);
+            pg_bar_init(b_free + 8 * h, 4);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == PC_W_MMA) pg_alloc<false>(s_tmem);
+    pg_fence_before();
+    __syncthreads();
+    pg_fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(s_tmem));
+    bool ok = true;
+    auto wait = [&](uint32_t bar, uint32_t parity, uint32_t code) {
+        ok = __all_sync(0xffffffffu, pc_wait(bar, parity, a, code));
+        return ok;
+    };
+    PagedWalk<PC_KT> w;
+    w.begin(a, shape, range);
+    auto rows_of = [&]() { return min(shape.tokens, w.q.n - w.tile * shape.tokens) * a.kv_mul; };
+
+    if (warp < PC_W_MMA) {
+        // ===== a half: thread = row =====
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PC_REGS_HALF));
+        const uint32_t half = warp >> 2, row = tid & 127, tl = tmem + ((warp & 3) << 21);   // the warp's 32 lanes of tensor memory
+        const uint32_t t_s = tl + PC_S + 128 * half, t_o = tl + PC_O + 128 * half;
+        const uint32_t bs = b_s + 8 * half, bp = b_p + 8 * half, bo = b_o + 8 * half, bf = b_free + 8 * half;
+        uint32_t ps = 0, po = 0;   // parities
+        do {
+            if (half == 1 && rows_of() <= 128) continue;
+            const uint32_t r = 128 * half + row, tt = r / a.kv_mul;
+            const int32_t p = w.q.p0 + (int32_t)(w.tile * shape.tokens + tt);
+            float acc[HS], f;
+            {
+                const bool there = w.tile * shape.tokens + tt < w.q.n && tt < shape.tokens;
+                const float *q = a.q + (uint64_t)(w.q.start + w.tile * shape.tokens + tt) * a.q_stride + (uint64_t)(w.group * a.kv_mul + r % a.kv_mul) * HS;
+                float most = 0.f;
+#pragma unroll
+                for (int i = 0; i < HS; i += 4) {
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (there) {
+                        if (a.vec) v = *reinterpret_cast<const float4 *>(q + i);
+                        else v = make_float4(q[i], q[i + 1], q[i + 2], q[i + 3]);
+                    }
+                    acc[i] = v.x; acc[i + 1] = v.y; acc[i + 2] = v.z; acc[i + 3] = v.w;
+                    most = fmaxf(fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+                }
+                const int e2 = paged_exponent(most);
+                const float down = exp2f((float)-e2);
+                f = exp2f((float)e2) * (1.4426950408889634f / sqrtf((float)HS));
+                // 16-byte piece c of a row lies at piece c ^ (row % 8)
+                const uint32_t to = q0 + half * 2 * HALF + row * 128;
+#pragma unroll
+                for (uint32_t c = 0; c < HS / 8; c++) {
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float x = acc[8 * c + 2 * e] * down, y = acc[8 * c + 2 * e + 1] * down;
+                        const __half2 h = __floats2half2_rn(x, y);
+                        const float2 g = __half22float2(h);
+                        const __half2 l = __floats2half2_rn(x - g.x, y - g.y);
+                        hi[e] = *reinterpret_cast<const uint32_t *>(&h);
+                        lo[e] = *reinterpret_cast<const uint32_t *>(&l);
+                    }
+                    const uint32_t at = to + (c / 8) * 16384 + (((c & 7) ^ (row & 7)) << 4);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + HALF), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) pg_arrive(b_q + 8 * half);
+            }
+#pragma unroll
+            for (int i = 0; i < HS; i++) acc[i] = 0.f;
+            float m = -INFINITY, l = 0.f, alpha = 1.f;
+            const int32_t p_lo = w.q.p0 + (int32_t)(w.tile * shape.tokens + 128 * half / a.kv_mul), p_hi = w.q.p0 + (int32_t)min((w.tile + 1) * shape.tokens, w.q.n) - 1;
+            const uint32_t first_unit = w.at, units = w.count, sink_tiles = w.span.sink_tiles, first_tile = w.span.first;
+            if (lane == 0) sm_walk[warp] = w;
+            __syncwarp();
+            auto fold = [&]() {   // acc = alpha acc + O
+                if (!wait(bo, po, 12)) return;
+                po ^= 1;
+                pg_fence_after();
+                uint32_t o[2][16];
+                pg_ld16(t_o, o[0]);
+                pc_wait_ld(o[0]);
+#pragma unroll
+                for (int c = 0; c < HS / 16; c++) {
+                    if (c + 1 < HS / 16) pg_ld16(t_o + 16 * (c + 1), o[(c + 1) & 1]);
+#pragma unroll
+                    for (int e = 0; e < 16; e++) acc[16 * c + e] = fmaf(acc[16 * c + e], alpha, __uint_as_float(o[c & 1][e]));
+                    if (c + 1 < HS / 16) pc_wait_ld(o[(c + 1) & 1]);
+                }
+                pg_fence_before();
+                __syncwarp();
+                if (lane == 0) pg_arrive(bf);
+            };
+            for (uint32_t i = 0; i < units && ok; i++) {
+                if (!wait(bs, ps, 12)) break;
+                ps ^= 1;
+                pg_fence_after();
+                const int32_t base = (int32_t)(key_tile({sink_tiles, first_tile, 0, 0}, first_unit + i) * PC_KT);
+                // which columns the row sees: up to `last`, and of those from `from` on or ahead of `sinks`
+                const bool masked = base + (int32_t)PC_KT - 1 > p_lo || (a.window && (int64_t)base + a.window <= p_hi);
+                const int32_t last = p - base;
+                const int32_t from = a.window ? (int32_t)max((int64_t)p - a.window + 1 - base, (int64_t)-1) : -1, sinks = (int32_t)min((int64_t)a.sinks - base, (int64_t)PC_KT);
+                auto sees = [&](int32_t c) { return c <= last && (c >= from || c < sinks); };
+                float top = -INFINITY;
+                uint32_t s[2][16];
+                pg_ld16(t_s, s[0]);
+                pc_wait_ld(s[0]);
+                if (!masked) {
+#pragma unroll
+                    for (int c = 0; c < 8; c++) {
+                        pg_ld16(t_s + 16 * ((c + 1) & 7), s[(c + 1) & 1]);   // (the last one fetches the first for the next pass)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) top = fmaxf(top, __uint_as_float(s[c & 1][e]));
+                        pc_wait_ld(s[(c + 1) & 1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 8; c++) {
+                        pg_ld16(t_s + 16 * ((c + 1) & 7), s[(c + 1) & 1]);
+#pragma unroll
+                        for (int e = 0; e < 16; e++) top = fmaxf(top, sees(16 * c + e) ? __uint_as_float(s[c & 1][e]) : -INFINITY);
+                        pc_wait_ld(s[(c + 1) & 1]);
+                    }
+                }
+                const float m1 = fmaxf(m, ceilf(top * f)), bottom = m1 == -INFINITY ? 0.f : m1, alpha1 = paged_ex2(m - bottom), shift = PC_SHIFT - bottom;
+                m = m1;
+                float sum = 0.f;
+#pragma unroll
+                for (int c = 0; c < 8; c++) {
+                    uint32_t o[16];
+                    if (c < 7) pg_ld16(t_s + 16 * (c + 1), s[(c + 1) & 1]);
+                    if (masked) {
+#pragma unroll
+                        for (int e = 0; e < 16; e++)
+                            if (!sees(16 * c + e)) s[c & 1][e] = 0xFF800000u;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const float x = paged_ex2(fmaf(__uint_as_float(s[c & 1][e]), f, shift)), y = paged_ex2(fmaf(__uint_as_float(s[c & 1][e + 1]), f, shift));
+                        sum += x + y;
+                        const __half2 h = __floats2half2_rn(x, y);
+                        const float2 g = __half22float2(h);
+                        const __half2 d = __floats2half2_rn(x - g.x, y - g.y);
+                        o[e / 2] = *reinterpret_cast<const uint32_t *>(&h);
+                        o[8 + e / 2] = *reinterpret_cast<const uint32_t *>(&d);
+                    }
+                    if (c < 7) pc_wait_ld(s[(c + 1) & 1]);
+                    pg_st16(t_s + 16 * c, o);
+                }
+                l = fmaf(l, alpha1, sum);
+                pg_wait_st();
+                pg_fence_before();
+                __syncwarp();
+                if (lane == 0) pg_arrive(bp);
+                if (i) fold();   // of the tile before: its products were done before these scores
+                alpha = alpha1;
+            }
+            if (ok) fold();
+            if (!ok) break;
+            w = *const_cast<const PagedWalk<PC_KT> *>(&sm_walk[warp]);
+
+            // ---- the half's result, or its part of it ----
+            bool finish = w.whole();
+            if (!finish) {
+                const uint32_t c0 = range.range_of(w.tile_unit()), c1 = range.range_of(w.tile_unit() + w.span.units - 1);
+                float *part = a.scratch + ((size_t)paged_place(range, w.tile_unit(), blockIdx.x) * 2 + half) * pc_partial_floats(HS);
+#pragma unroll
+                for (int i = 0; i < HS; i++) __stcg(part + 128 * i + row, acc[i]);
+                __stcg(part + 128 * HS + row, m);
+                __stcg(part + 128 * (HS + 1) + row, l);
+                __threadfence();
+                pc_sync_half(half);
+                if (row == 0) {
+                    const uint32_t is_last = atomicAdd(a.counters + 2 * c0 + half, 1u) == c1 - c0;
+                    if (is_last) a.counters[2 * c0 + half] = 0u;   // for the next launch
+                    __threadfence();
+                    sm_last[half] = is_last;
+                }
+                pc_sync_half(half);
+                finish = sm_last[half] != 0;
+                pc_sync_half(half);   // (the word is written again at the next tile)
+                if (finish) {
+                    m = -INFINITY;
+                    l = 0.f;
+#pragma unroll
+                    for (int i = 0; i < HS; i++) acc[i] = 0.f;
+                    for (uint32_t k = c0; k <= c1; k++) m = fmaxf(m, __ldcg(a.scratch + ((size_t)paged_place(range, w.tile_unit(), k) * 2 + half) * pc_partial_floats(HS) + 128 * HS + row));
+                    for (uint32_t k = c0; k <= c1; k++) {
+                        const float *from = a.scratch + ((size_t)paged_place(range, w.tile_unit(), k) * 2 + half) * pc_partial_floats(HS) + row;
+                        const float wt = m == -INFINITY ? 0.f : paged_ex2(__ldcg(from + 128 * HS) - m);
+                        l += wt * __ldcg(from + 128 * (HS + 1));
+#pragma unroll
+                        for (int i = 0; i < HS; i++) acc[i] = fmaf(wt, __ldcg(from + 128 * i), acc[i]);
+                    }
+                }
+            }
+            if (finish) {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                const bool there = w.tile * shape.tokens + tt < w.q.n && tt < shape.tokens;
+                const uint64_t q_row = w.q.start + w.tile * shape.tokens + tt;
+                const uint32_t head = w.group * a.kv_mul + r % a.kv_mul;
+                const float *q = a.q + q_row * a.q_stride + (uint64_t)head * HS;
+                float *out = a.out + q_row * a.out_stride + (uint64_t)head * HS;
+                bool odd = false;
+#pragma unroll
+                for (int i = 0; i < HS; i++) {
+                    acc[i] *= inv;
+                    odd |= !isfinite(acc[i]);
+                }
+                if (there) {
+                    if (a.vec)
+#pragma unroll
+                        for (int i = 0; i < HS; i += 4) *reinterpret_cast<float4 *>(out + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+                    else
+#pragma unroll
+                        for (int i = 0; i < HS; i++) out[i] = acc[i];
+                }
+                for (uint32_t who = __ballot_sync(0xffffffffu, odd && there && isfinite(l)); who; who &= who - 1) {
+                    const int b = __ffs(who) - 1;
+                    __syncwarp();
+                    paged_repair<__half>(a, PC_KT, w.request, w.group, w.span, __shfl_sync(0xffffffffu, p, b), __shfl_sync(0xffffffffu, m, b),
+                                         reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, (unsigned long long)q, b)), reinterpret_cast<float *>(__shfl_sync(0xffffffffu, (unsigned long long)out, b)), HS);
+                }
+            }
+        } while (w.next(a, shape));
+    } else {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PC_REGS_OTHER));
+      if (warp == PC_W_MMA) {
+        // ===== MMA issue =====
+        const uint32_t id_s = pg_idesc(128, 128), id_o = pg_idesc(128, HS) | 1u << 16;   // (V: MN-major)
+        uint32_t slot = 0, phase = 0;                                                     // of the ring
+        uint32_t pq[2] = {0, 0}, pp[2] = {0, 0}, n[2] = {0, 0};                            // parities; key tiles that a half has been given
+        auto take = [&]() {   // the next tile of the ring
+            const uint32_t at = slot;
+            if (!wait(b_full + 8 * slot, phase, 11)) return at;
+            if (++slot == SLOTS) { slot = 0; phase ^= 1; }
+            return at;
+        };
+        auto scores = [&](uint32_t h, uint32_t k_slot) {
+            if (pg_elect()) {
+                const uint64_t qd = pc_desc_k(q0 + h * 2 * HALF), kd = pc_desc_k(ring + k_slot * HALF);
+#pragma unroll
+                for (uint32_t lo = 0; lo < 2; lo++)
+#pragma unroll
+                    for (uint32_t k = 0; k < HS / 16; k++) {
+                        const uint64_t at = (k / 4) * (16384 >> 4) + (k % 4) * (32 >> 4);
+                        pc_mma_ss(tmem + PC_S + 128 * h, qd + lo * (HALF >> 4) + at, kd + at, id_s, lo | k);
+                    }
+                pg_commit<false>(b_s + 8 * h);
+            }
+            __syncwarp();
+        };
+        auto products = [&](uint32_t h, uint32_t v_slot) {
+            if (pg_elect()) {
+                const uint64_t vd = pc_desc_mn(ring + v_slot * HALF, 16384);
+#pragma unroll
+                for (uint32_t k = 0; k < 8; k++)
+#pragma unroll
+                    for (uint32_t lo = 0; lo < 2; lo++)
+                        pg_mma<false>(tmem + PC_O + 128 * h, tmem + PC_S + 128 * h + 16 * k + 8 * lo, vd + k * (2048 >> 4), id_o, lo | k);
+                pg_commit<false>(b_o + 8 * h);
+            }
+            __syncwarp();
+        };
+        auto release = [&](uint32_t s) {
+            if (pg_elect()) pg_commit<false>(b_empty + 8 * s);
+            __syncwarp();
+        };
+        auto begin_half = [&](uint32_t h) {   // its q has arrived
+            if (!wait(b_q + 8 * h, pq[h], 12)) return false;
+            pq[h] ^= 1;
+            pg_fence_after();
+            return true;
+        };
+        auto probabilities = [&](uint32_t h) {   // P is there, and O's place is free
+            if (!wait(b_p + 8 * h, pp[h], 12)) return false;
+            pp[h] ^= 1;
+            if (n[h] && !wait(b_free + 8 * h, (n[h] - 1) & 1, 12)) return false;
+            n[h]++;
+            pg_fence_after();
+            return true;
+        };
+        bool two = rows_of() > 128;
+        uint32_t ks = take();
+        if (ok && begin_half(0)) {
+            scores(0, ks);
+            if (two && begin_half(1)) scores(1, ks);
+            if (ok) release(ks);
+        }
+        for (bool more = true; more && ok;) {
+            uint32_t i = w.at;
+            const uint32_t end = w.at + w.count;
+            const int32_t kv_end = w.q.p0 + (int32_t)w.q.n;   // positions behind it: rows of the last page that hold nothing
+            const KeySpan span = w.span;
+            for (; i < end && ok; i++) {
+                const uint32_t vs = take();
+                if (!ok) break;
+                const int32_t base = (int32_t)(key_tile(span, i) * PC_KT);
+                if (base + (int32_t)PC_KT > kv_end) {
+                    const uint32_t first = (uint32_t)max(kv_end - base, 0);
+                    for (uint32_t c = 0; c < COLS; c++)
+                        for (uint32_t at = first * 128 + lane * 16; at < 16384; at += 512)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(ring + vs * HALF + c * 16384 + at), "r"(0u) : "memory");
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+                const bool was_two = two, fresh = i + 1 == end;   // fresh: the next key tile is another query tile's
+                if (fresh) {
+                    more = w.next(a, shape);
+                    if (more) two = rows_of() > 128;
+                }
+                if (!probabilities(0)) break;
+                products(0, vs);
+                if (!was_two) release(vs);
+                if (more) {
+                    ks = take();
+                    if (!ok || (fresh && !begin_half(0))) break;
+                    scores(0, ks);
+                    if (!two) release(ks);
+                }
+                if (was_two) {
+                    if (!probabilities(1)) break;
+                    products(1, vs);
+                    release(vs);
+                }
+                if (more && two) {
+                    if (fresh && !begin_half(1)) break;
+                    scores(1, ks);
+                    release(ks);
+                }
+            }
+        }
+        if (ok) {   // the last commits arrive in shared memory: let them, before the CTA ends
+            const uint32_t last = (slot + SLOTS - 1) % SLOTS;
+            wait(b_empty + 8 * last, slot == 0 ? phase ^ 1 : phase, 12);
+        }
+      } else if (warp == PC_W_TMA) {
+        // ===== TMA: K and V of a key tile, one slot of the ring each =====
+        const uint32_t page_size = 1u << a.page_log2, box = page_size < PC_KT ? page_size : PC_KT, boxes = PC_KT / box;
+        uint32_t slot = 0, use = 0;
+        do {
+            const int32_t *table = a.table + (size_t)w.request * a.max_pages;
+            const int32_t kv_end = w.q.p0 + (int32_t)w.q.n;
+            for (uint32_t i = 0; i < w.count && ok; i++) {
+                const uint32_t j = key_tile(w.span, w.at + i) * PC_KT + lane * box;   // a lane per page
+                int32_t page = -1;
+                if (lane < boxes && (int32_t)j < kv_end) page = table[j >> a.page_log2];
+                const bool there = page >= 0 && (uint32_t)page < a.n_pages;
+                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, there)) * box * HS * 2;
+#pragma unroll
+                for (uint32_t v = 0; v < 2; v++) {
+                    if (use && !wait(b_empty + 8 * slot, (use - 1) & 1, 12)) break;
+                    const uint32_t full = b_full + 8 * slot, dst = ring + slot * HALF + lane * box * 128;
+                    if (lane == 0) pg_expect(full, bytes);
+                    __syncwarp();
+                    if (there)
+                        for (uint32_t c = 0; c < COLS; c++)
+                            pc_tma3d(dst + c * 16384, v ? &maps.v : &maps.k, (int32_t)(w.group * HS + 64 * c), (int32_t)(j & (page_size - 1)), page, full);
+                    __syncwarp();
+                    if (++slot == SLOTS) { slot = 0; use++; }
+                }
+            }
+        } while (ok && w.next(a, shape));
+      }
+    }
+    if (!ok) {   // a wait gave up: copies and products of this CTA may still be in flight; give them time to land before the CTA ends
+        const unsigned long long t0 = pg_ns();
+        while (pg_ns() - t0 < 100000ull) {}
+    }
+    __syncwarp();
+    pg_fence_before();
+    __syncthreads();
+    if (warp == PC_W_MMA) pg_dealloc<false>(tmem);
+}
+
+uint32_t paged_chunk_ctas(const ib_ctx *ctx) { return (uint32_t)ctx->sm_count; }
+size_t paged_chunk_scratch_floats(const ib_ctx *ctx, uint32_t head_size) { return (size_t)paged_chunk_ctas(ctx) * 4 * pc_partial_floats(head_size); }
+
+// Pages of a cache as boxes of up to 128 rows x 64 columns
+static int32_t pc_encode(const PagedAttn &a, const void *cache, CUtensorMap *map) {
+    EncodeTiledFn encode = encode_tiled();
+    IB_REQUIRE(encode, "ib_paged_attention: the driver does not export cuTensorMapEncodeTiled");
+    const cuuint32_t page_size = 1u << a.page_log2, box[3] = {64, page_size < PC_KT ? page_size : PC_KT, 1}, estr[3] = {1, 1, 1};
+    const cuuint64_t dims[3] = {a.kv_dim, page_size, a.n_pages}, strides[2] = {(cuuint64_t)a.kv_dim * 2, a.page_stride * 2};
+    const CUresult cr = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(cache), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    IB_REQUIRE(cr == CUDA_SUCCESS, "ib_paged_attention: cuTensorMapEncodeTiled failed with %d", (int)cr);
+    return IB_OK;
+}
+
+bool paged_chunk_takes(const PagedAttn &a, int kv_dtype) { return kv_dtype == IB_KV_F16 && a.page_stride * 2 < (1ull << 40); }
+
+int32_t launch_paged_chunk(ib_ctx *ctx, cudaStream_t s, PagedAttn a, uint32_t head_size) {
+    const TileShape shape = {a.kv_mul, 1, PC_ROWS / a.kv_mul};
+    a.least_units = 1;
+    PcMaps maps;
+    int32_t rc = pc_encode(a, a.k, &maps.k);
+    if (rc == IB_OK) rc = pc_encode(a, a.v, &maps.v);
+    if (rc) return rc;
+    void (*kernel)(PagedAttn, TileShape, PcMaps) = head_size == 128 ? paged_chunk_kernel<128> : paged_chunk_kernel<64>;
+    static bool attr_set[16] = {false};
+    const bool beyond = ctx->device >= 16;
+    if (beyond || !attr_set[ctx->device]) {
+        IB_CHECK_CUDA(cudaFuncSetAttribute(paged_chunk_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pc_smem(128)));
+        IB_CHECK_CUDA(cudaFuncSetAttribute(paged_chunk_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pc_smem(64)));
+        if (!beyond) attr_set[ctx->device] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(paged_chunk_ctas(ctx));
+    cfg.blockDim = dim3(PC_THREADS);
+    cfg.dynamicSmemBytes = pc_smem(head_size);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    IB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, shape, maps));
+    ctx->launches++;
+    return IB_OK;
+}
+
+}  // namespace ib
