@@ -12,11 +12,12 @@
 // remaining work of a thread's 128 scores about 1000.  The halves take turns: while one is in softmax, the tensor cores do the other's products.  Two halves share a key tile's 64 KB, 16
 // bytes a clock and SM; a tile of 128 rows would take twice as much from L2, which is all that L2 has.
 //
-// Who does what (12 warps, one CTA per SM):
-//   warps 0-3, 4-7   a half each: thread = row.  Loads and splits q, softmax, fold, result
-//   warp 8           MMA issue
-//   warp 9           TMA copies of K and V: a ring of tiles, a copy per page and 64 columns, swizzled by 128 bytes
-//   warps 10, 11     nothing (registers change hands by groups of four warps)
+// Who does what (20 warps, one CTA per SM):
+//   warps 0-7, 8-15  a half each: two threads per row, each with half of the key tile's scores and of the result's columns.  Load and split q, softmax, fold, result.  (A thread per row
+//                    had a chain of 4600 clocks from the scores to the next product, 128 sums in registers and no room for the rest)
+//   warp 16          MMA issue
+//   warp 17          TMA copies of K and V: a ring of tiles, a copy per page and 64 columns, swizzled by 128 bytes
+//   warps 18, 19     nothing (registers change hands by groups of four warps)
 // They hand over through mbarriers.  Order of the MMAs: S0 S1 | O0 S0' O1 S1' | O0' S0'' ...: a half's softmax has the time of the other's two products.
 // Tensor memory (512 columns): S0 / P0, S1 / P1, O0, O1 of 128 columns each.  P's operands are interleaved by 16 positions, hi then lo, so that a thread overwrites only scores that it has read.
 //
@@ -26,16 +27,24 @@
 
 namespace ib {
 
-constexpr uint32_t PC_THREADS = 384, PC_KT = 128, PC_ROWS = 256, PC_W_MMA = 8, PC_W_TMA = 9;
-// Registers: 384 threads at 168 are what the block is launched with; the halves' warps take 208 of them, the others keep 88 (2 * 128 * 208 + 128 * 88 = 384 * 168).
-constexpr uint32_t PC_REGS_HALF = 208, PC_REGS_OTHER = 88;
+constexpr uint32_t PC_THREADS = 640, PC_KT = 128, PC_ROWS = 256, PC_W_MMA = 16, PC_W_TMA = 17;
+// Registers: 640 threads at 96 are what the block is launched with; the halves' warps take 104 of them, the others keep 64 (512 * 104 + 128 * 64 = 640 * 96).
+constexpr uint32_t PC_REGS_HALF = 104, PC_REGS_OTHER = 64;
 constexpr uint32_t PC_S = 0, PC_O = 256;   // tensor memory columns; the halves' are 128 apart
 constexpr uint32_t PC_SMEM_LIMIT = 227 * 1024;
 constexpr float PC_SHIFT = 14.f;           // probabilities are held times 2^14 (the remainders of small ones stay above f16's smallest step)
 constexpr uint32_t pc_half(uint32_t hs) { return 128 * hs * 2; }       // bytes of 128 rows: a half's hi (= lo) operand, a tile of K or V
 constexpr uint32_t pc_slots(uint32_t hs) { return hs == 128 ? 3u : 8u; }
-constexpr uint32_t pc_smem(uint32_t hs) { return 1024 + (4 + pc_slots(hs)) * pc_half(hs) + 256; }
-static_assert(pc_smem(128) <= PC_SMEM_LIMIT && pc_smem(64) <= PC_SMEM_LIMIT, "shared memory");
+constexpr uint32_t PC_MAX_SLOTS = 8;
+struct PcShared {   // behind Q and the ring
+    uint64_t bars[2 * PC_MAX_SLOTS + 10];
+    uint32_t tmem, last[2], odd[2][2][4];
+    float x[2][2][128];            // what the two threads of a row tell one another
+    PagedWalk<PC_KT> walk[4];      // the walks of the halves, of the MMA warp and of the TMA warp, while registers have other things to hold
+    PagedRangeShared range;
+};
+constexpr uint32_t pc_smem(uint32_t hs) { return (4 + pc_slots(hs)) * pc_half(hs) + (uint32_t)sizeof(PcShared); }
+static_assert(pc_smem(128) <= PC_SMEM_LIMIT && pc_smem(64) <= PC_SMEM_LIMIT && pc_slots(64) <= PC_MAX_SLOTS, "shared memory");
 constexpr uint32_t pc_partial_floats(uint32_t hs) { return 128 * (hs + 2); }   // of a half
 
 // Descriptors of operands in shared memory: rows of 64 f16 (128 bytes), eight of them 1024 bytes, swizzled by 128 bytes.  K-major: further columns lie behind all rows, so a descriptor covers 64
@@ -65,8 +74,8 @@ __device__ __forceinline__ void pc_wait_ld(uint32_t (&r)[16]) {
                  : "memory");
 }
 __device__ __forceinline__ void pc_sync_half(uint32_t half) {
-    if (half) asm volatile("bar.sync 2, 128;" ::: "memory");
-    else asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (half) asm volatile("bar.sync 2, 256;" ::: "memory");
+    else asm volatile("bar.sync 1, 256;" ::: "memory");
 }
 
 // Bounded wait without a function call: ptxas does not keep a caller's registers beyond the launch's number across one
@@ -90,35 +99,31 @@ struct PcMaps { CUtensorMap k, v; };
 template <int HS>
 __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid_constant__ PagedAttn a, const TileShape shape, const __grid_constant__ PcMaps maps) {
     constexpr uint32_t HALF = pc_half(HS), SLOTS = pc_slots(HS), COLS = HS / 64;   // column blocks of 64
-    extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    __shared__ PagedRangeShared range_sh;
-    __shared__ uint32_t sm_last[2];
-    __shared__ PagedWalk<PC_KT> sm_walk[8];   // the halves' warps' walks, while their registers hold a tile's sums
-    const uint32_t q0 = pg_smem(smem), ring = q0 + 4 * HALF, bars = ring + SLOTS * HALF;   // Q: [half][hi, lo]
-    const uint32_t b_full = bars, b_empty = b_full + 8 * SLOTS, b_q = b_empty + 8 * SLOTS, b_s = b_q + 16, b_p = b_s + 16, b_o = b_p + 16, b_free = b_o + 16, s_tmem = b_free + 16;
+    extern __shared__ __align__(1024) uint8_t smem[];   // (the swizzle's alignment; there is no static shared memory ahead of it)
+    PcShared &S = *reinterpret_cast<PcShared *>(smem + (4 + SLOTS) * HALF);
+    const uint32_t q0 = pg_smem(smem), ring = q0 + 4 * HALF, bars = pg_smem(S.bars);   // Q: [half][hi, lo]
+    const uint32_t b_full = bars, b_empty = b_full + 8 * SLOTS, b_q = b_empty + 8 * SLOTS, b_s = b_q + 16, b_p = b_s + 16, b_o = b_p + 16, b_free = b_o + 16;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const PagedRange range = paged_range<PC_KT, PC_THREADS>(a, shape, range_sh);
+    const PagedRange range = paged_range<PC_KT, PC_THREADS>(a, shape, S.range);
     if (range.total == 0 || blockIdx.x >= range.ranges) return;
     if (warp == 0 && lane == 0) {
         for (uint32_t i = 0; i < 2 * SLOTS; i++) pg_bar_init(b_full + 8 * i, 1);
         for (uint32_t h = 0; h < 2; h++) {
-            pg_bar_init(b_q + 8 * h, 4);      // a half's warps
+            pg_bar_init(b_q + 8 * h, 8);      // a half's warps
             pg_bar_init(b_s + 8 * h, 1);      // the MMAs' completion
-            pg_bar_init(b_p + 8 * h, 4);
+            pg_bar_init(b_p + 8 * h, 8);
             pg_bar_init(b_o + 8 * h, 1);
-            pg_bar_init(b_free + 8 * h, 4);
+            pg_bar_init(b_free + 8 * h, 8);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == PC_W_MMA) pg_alloc<false>(s_tmem);
+    if (warp == PC_W_MMA) pg_alloc<false>(pg_smem(&S.tmem));
     pg_fence_before();
     __syncthreads();
     pg_fence_after();
-    uint32_t tmem;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(s_tmem));
+    const uint32_t tmem = *const_cast<volatile uint32_t *>(&S.tmem);
     bool ok = true;
     auto wait = [&](uint32_t bar, uint32_t parity, uint32_t code) {
         ok = __all_sync(0xffffffffu, pc_wait(bar, parity, a, code));
@@ -126,26 +131,41 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
     };
     PagedWalk<PC_KT> w;
     w.begin(a, shape, range);
+    PagedWalk<PC_KT> &kept = S.walk[warp < PC_W_MMA ? warp >> 3 : 2 + (warp & 1)];
+    auto park = [&]() {
+        __syncwarp();
+        if (lane == 0) kept = w;
+        __syncwarp();
+    };
+    auto unpark = [&]() { w = *const_cast<const PagedWalk<PC_KT> *>(&kept); };
     auto rows_of = [&]() { return min(shape.tokens, w.q.n - w.tile * shape.tokens) * a.kv_mul; };
 
     if (warp < PC_W_MMA) {
-        // ===== a half: thread = row =====
+        // ===== a half: two threads per row =====
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PC_REGS_HALF));
-        const uint32_t half = warp >> 2, row = tid & 127, tl = tmem + ((warp & 3) << 21);   // the warp's 32 lanes of tensor memory
-        const uint32_t t_s = tl + PC_S + 128 * half, t_o = tl + PC_O + 128 * half;
+        constexpr uint32_t D = HS / 2;   // a thread's columns of the result
+        const uint32_t half = warp >> 3, side = (warp >> 2) & 1, row = tid & 127, tl = tmem + ((warp & 3) << 21);   // the warp's 32 lanes of tensor memory
+        const uint32_t t_s = tl + PC_S + 128 * half + 64 * side, t_o = tl + PC_O + 128 * half + D * side;
         const uint32_t bs = b_s + 8 * half, bp = b_p + 8 * half, bo = b_o + 8 * half, bf = b_free + 8 * half;
+        // The value of the row's other thread.  (Between an exchange and the next one there is a barrier that every warp of the half arrives at only when it is through with this one: of the
+        // scores, of the products, or the half's own.)
+        auto other = [&](float x) {
+            S.x[half][side][row] = x;
+            pc_sync_half(half);
+            return S.x[half][side ^ 1][row];
+        };
         uint32_t ps = 0, po = 0;   // parities
         do {
             if (half == 1 && rows_of() <= 128) continue;
             const uint32_t r = 128 * half + row, tt = r / a.kv_mul;
             const int32_t p = w.q.p0 + (int32_t)(w.tile * shape.tokens + tt);
-            float acc[HS], f;
+            float acc[D], f;
             {
                 const bool there = w.tile * shape.tokens + tt < w.q.n && tt < shape.tokens;
-                const float *q = a.q + (uint64_t)(w.q.start + w.tile * shape.tokens + tt) * a.q_stride + (uint64_t)(w.group * a.kv_mul + r % a.kv_mul) * HS;
+                const float *q = a.q + (uint64_t)(w.q.start + w.tile * shape.tokens + tt) * a.q_stride + (uint64_t)(w.group * a.kv_mul + r % a.kv_mul) * HS + D * side;
                 float most = 0.f;
 #pragma unroll
-                for (int i = 0; i < HS; i += 4) {
+                for (int i = 0; i < (int)D; i += 4) {
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (there) {
                         if (a.vec) v = *reinterpret_cast<const float4 *>(q + i);
@@ -154,24 +174,25 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                     acc[i] = v.x; acc[i + 1] = v.y; acc[i + 2] = v.z; acc[i + 3] = v.w;
                     most = fmaxf(fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
                 }
+                most = fmaxf(most, other(most));
                 const int e2 = paged_exponent(most);
                 const float down = exp2f((float)-e2);
                 f = exp2f((float)e2) * (1.4426950408889634f / sqrtf((float)HS));
                 // 16-byte piece c of a row lies at piece c ^ (row % 8)
                 const uint32_t to = q0 + half * 2 * HALF + row * 128;
 #pragma unroll
-                for (uint32_t c = 0; c < HS / 8; c++) {
+                for (uint32_t i = 0; i < D / 8; i++) {
                     uint32_t hi[4], lo[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const float x = acc[8 * c + 2 * e] * down, y = acc[8 * c + 2 * e + 1] * down;
+                        const float x = acc[8 * i + 2 * e] * down, y = acc[8 * i + 2 * e + 1] * down;
                         const __half2 h = __floats2half2_rn(x, y);
                         const float2 g = __half22float2(h);
                         const __half2 l = __floats2half2_rn(x - g.x, y - g.y);
                         hi[e] = *reinterpret_cast<const uint32_t *>(&h);
                         lo[e] = *reinterpret_cast<const uint32_t *>(&l);
                     }
-                    const uint32_t at = to + (c / 8) * 16384 + (((c & 7) ^ (row & 7)) << 4);
+                    const uint32_t c = side * (D / 8) + i, at = to + (c / 8) * 16384 + (((c & 7) ^ (row & 7)) << 4);
                     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
                     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + HALF), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
                 }
@@ -180,12 +201,11 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                 if (lane == 0) pg_arrive(b_q + 8 * half);
             }
 #pragma unroll
-            for (int i = 0; i < HS; i++) acc[i] = 0.f;
+            for (int i = 0; i < (int)D; i++) acc[i] = 0.f;
             float m = -INFINITY, l = 0.f, alpha = 1.f;
             const int32_t p_lo = w.q.p0 + (int32_t)(w.tile * shape.tokens + 128 * half / a.kv_mul), p_hi = w.q.p0 + (int32_t)min((w.tile + 1) * shape.tokens, w.q.n) - 1;
             const uint32_t first_unit = w.at, units = w.count, sink_tiles = w.span.sink_tiles, first_tile = w.span.first;
-            if (lane == 0) sm_walk[warp] = w;
-            __syncwarp();
+            if (side == 0 && (warp & 3) == 0) park();   // (read again behind the half's barrier below)
             auto fold = [&]() {   // acc = alpha acc + O
                 if (!wait(bo, po, 12)) return;
                 po ^= 1;
@@ -194,11 +214,11 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                 pg_ld16(t_o, o[0]);
                 pc_wait_ld(o[0]);
 #pragma unroll
-                for (int c = 0; c < HS / 16; c++) {
-                    if (c + 1 < HS / 16) pg_ld16(t_o + 16 * (c + 1), o[(c + 1) & 1]);
+                for (int c = 0; c < (int)D / 16; c++) {
+                    if (c + 1 < (int)D / 16) pg_ld16(t_o + 16 * (c + 1), o[(c + 1) & 1]);
 #pragma unroll
                     for (int e = 0; e < 16; e++) acc[16 * c + e] = fmaf(acc[16 * c + e], alpha, __uint_as_float(o[c & 1][e]));
-                    if (c + 1 < HS / 16) pc_wait_ld(o[(c + 1) & 1]);
+                    if (c + 1 < (int)D / 16) pc_wait_ld(o[(c + 1) & 1]);
                 }
                 pg_fence_before();
                 __syncwarp();
@@ -208,40 +228,36 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                 if (!wait(bs, ps, 12)) break;
                 ps ^= 1;
                 pg_fence_after();
-                const int32_t base = (int32_t)(key_tile({sink_tiles, first_tile, 0, 0}, first_unit + i) * PC_KT);
-                // which columns the row sees: up to `last`, and of those from `from` on or ahead of `sinks`
-                const bool masked = base + (int32_t)PC_KT - 1 > p_lo || (a.window && (int64_t)base + a.window <= p_hi);
+                const int32_t base = (int32_t)(key_tile({sink_tiles, first_tile, 0, 0}, first_unit + i) * PC_KT) + 64 * (int32_t)side;
+                // which of its 64 columns the row sees: up to `last`, and of those from `from` on or ahead of `sinks`
+                const bool masked = base + 63 > p_lo || (a.window && (int64_t)base + a.window <= p_hi);
                 const int32_t last = p - base;
-                const int32_t from = a.window ? (int32_t)max((int64_t)p - a.window + 1 - base, (int64_t)-1) : -1, sinks = (int32_t)min((int64_t)a.sinks - base, (int64_t)PC_KT);
+                const int32_t from = a.window ? (int32_t)max((int64_t)p - a.window + 1 - base, (int64_t)-1) : -1, sinks = (int32_t)min((int64_t)a.sinks - base, (int64_t)64);
                 auto sees = [&](int32_t c) { return c <= last && (c >= from || c < sinks); };
-                float top = -INFINITY;
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 uint32_t s[2][16];
                 pg_ld16(t_s, s[0]);
                 pc_wait_ld(s[0]);
-                if (!masked) {
 #pragma unroll
-                    for (int c = 0; c < 8; c++) {
-                        pg_ld16(t_s + 16 * ((c + 1) & 7), s[(c + 1) & 1]);   // (the last one fetches the first for the next pass)
+                for (int c = 0; c < 4; c++) {
+                    pg_ld16(t_s + 16 * ((c + 1) & 3), s[(c + 1) & 1]);   // (the last one fetches the first for the next pass)
+                    if (masked) {
 #pragma unroll
-                        for (int e = 0; e < 16; e++) top = fmaxf(top, __uint_as_float(s[c & 1][e]));
-                        pc_wait_ld(s[(c + 1) & 1]);
+                        for (int e = 0; e < 16; e++) tops[e & 3] = fmaxf(tops[e & 3], sees(16 * c + e) ? __uint_as_float(s[c & 1][e]) : -INFINITY);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; e++) tops[e & 3] = fmaxf(tops[e & 3], __uint_as_float(s[c & 1][e]));
                     }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 8; c++) {
-                        pg_ld16(t_s + 16 * ((c + 1) & 7), s[(c + 1) & 1]);
-#pragma unroll
-                        for (int e = 0; e < 16; e++) top = fmaxf(top, sees(16 * c + e) ? __uint_as_float(s[c & 1][e]) : -INFINITY);
-                        pc_wait_ld(s[(c + 1) & 1]);
-                    }
+                    pc_wait_ld(s[(c + 1) & 1]);
                 }
+                const float own = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), top = fmaxf(own, other(own));
                 const float m1 = fmaxf(m, ceilf(top * f)), bottom = m1 == -INFINITY ? 0.f : m1, alpha1 = paged_ex2(m - bottom), shift = PC_SHIFT - bottom;
                 m = m1;
-                float sum = 0.f;
+                float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int c = 0; c < 8; c++) {
+                for (int c = 0; c < 4; c++) {
                     uint32_t o[16];
-                    if (c < 7) pg_ld16(t_s + 16 * (c + 1), s[(c + 1) & 1]);
+                    if (c < 3) pg_ld16(t_s + 16 * (c + 1), s[(c + 1) & 1]);
                     if (masked) {
 #pragma unroll
                         for (int e = 0; e < 16; e++)
@@ -250,17 +266,18 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
                         const float x = paged_ex2(fmaf(__uint_as_float(s[c & 1][e]), f, shift)), y = paged_ex2(fmaf(__uint_as_float(s[c & 1][e + 1]), f, shift));
-                        sum += x + y;
+                        sums[e & 2] += x;
+                        sums[(e & 2) + 1] += y;
                         const __half2 h = __floats2half2_rn(x, y);
                         const float2 g = __half22float2(h);
                         const __half2 d = __floats2half2_rn(x - g.x, y - g.y);
                         o[e / 2] = *reinterpret_cast<const uint32_t *>(&h);
                         o[8 + e / 2] = *reinterpret_cast<const uint32_t *>(&d);
                     }
-                    if (c < 7) pc_wait_ld(s[(c + 1) & 1]);
                     pg_st16(t_s + 16 * c, o);
+                    if (c < 3) pc_wait_ld(s[(c + 1) & 1]);
                 }
-                l = fmaf(l, alpha1, sum);
+                l = fmaf(l, alpha1, (sums[0] + sums[1]) + (sums[2] + sums[3]));
                 pg_wait_st();
                 pg_fence_before();
                 __syncwarp();
@@ -270,7 +287,8 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
             }
             if (ok) fold();
             if (!ok) break;
-            w = *const_cast<const PagedWalk<PC_KT> *>(&sm_walk[warp]);
+            l += other(l);   // (also: the kept walk is there)
+            unpark();
 
             // ---- the half's result, or its part of it ----
             bool finish = w.whole();
@@ -278,63 +296,68 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                 const uint32_t c0 = range.range_of(w.tile_unit()), c1 = range.range_of(w.tile_unit() + w.span.units - 1);
                 float *part = a.scratch + ((size_t)paged_place(range, w.tile_unit(), blockIdx.x) * 2 + half) * pc_partial_floats(HS);
 #pragma unroll
-                for (int i = 0; i < HS; i++) __stcg(part + 128 * i + row, acc[i]);
-                __stcg(part + 128 * HS + row, m);
-                __stcg(part + 128 * (HS + 1) + row, l);
+                for (int i = 0; i < (int)D; i++) __stcg(part + 128 * (D * side + i) + row, acc[i]);
+                if (side == 0) {
+                    __stcg(part + 128 * HS + row, m);
+                    __stcg(part + 128 * (HS + 1) + row, l);
+                }
                 __threadfence();
                 pc_sync_half(half);
-                if (row == 0) {
+                if (row == 0 && side == 0) {
                     const uint32_t is_last = atomicAdd(a.counters + 2 * c0 + half, 1u) == c1 - c0;
                     if (is_last) a.counters[2 * c0 + half] = 0u;   // for the next launch
                     __threadfence();
-                    sm_last[half] = is_last;
+                    S.last[half] = is_last;
                 }
                 pc_sync_half(half);
-                finish = sm_last[half] != 0;
-                pc_sync_half(half);   // (the word is written again at the next tile)
+                finish = S.last[half] != 0;
                 if (finish) {
                     m = -INFINITY;
                     l = 0.f;
 #pragma unroll
-                    for (int i = 0; i < HS; i++) acc[i] = 0.f;
+                    for (int i = 0; i < (int)D; i++) acc[i] = 0.f;
                     for (uint32_t k = c0; k <= c1; k++) m = fmaxf(m, __ldcg(a.scratch + ((size_t)paged_place(range, w.tile_unit(), k) * 2 + half) * pc_partial_floats(HS) + 128 * HS + row));
                     for (uint32_t k = c0; k <= c1; k++) {
                         const float *from = a.scratch + ((size_t)paged_place(range, w.tile_unit(), k) * 2 + half) * pc_partial_floats(HS) + row;
                         const float wt = m == -INFINITY ? 0.f : paged_ex2(__ldcg(from + 128 * HS) - m);
                         l += wt * __ldcg(from + 128 * (HS + 1));
+                        from += 128 * D * side;
 #pragma unroll
-                        for (int i = 0; i < HS; i++) acc[i] = fmaf(wt, __ldcg(from + 128 * i), acc[i]);
+                        for (int i = 0; i < (int)D; i++) acc[i] = fmaf(wt, __ldcg(from + 128 * i), acc[i]);
                     }
                 }
             }
-            if (finish) {
+            if (finish) {   // (the same for all of the half)
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 const bool there = w.tile * shape.tokens + tt < w.q.n && tt < shape.tokens;
-                const uint64_t q_row = w.q.start + w.tile * shape.tokens + tt;
-                const uint32_t head = w.group * a.kv_mul + r % a.kv_mul;
-                const float *q = a.q + q_row * a.q_stride + (uint64_t)head * HS;
-                float *out = a.out + q_row * a.out_stride + (uint64_t)head * HS;
+                const uint64_t q_row = w.q.start + w.tile * shape.tokens + tt, column = (uint64_t)(w.group * a.kv_mul + r % a.kv_mul) * HS;
+                float *out = a.out + q_row * a.out_stride + column;
                 bool odd = false;
 #pragma unroll
-                for (int i = 0; i < HS; i++) {
+                for (int i = 0; i < (int)D; i++) {
                     acc[i] *= inv;
                     odd |= !isfinite(acc[i]);
                 }
                 if (there) {
                     if (a.vec)
 #pragma unroll
-                        for (int i = 0; i < HS; i += 4) *reinterpret_cast<float4 *>(out + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+                        for (int i = 0; i < (int)D; i += 4) *reinterpret_cast<float4 *>(out + D * side + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
                     else
 #pragma unroll
-                        for (int i = 0; i < HS; i++) out[i] = acc[i];
+                        for (int i = 0; i < (int)D; i++) out[D * side + i] = acc[i];
                 }
-                for (uint32_t who = __ballot_sync(0xffffffffu, odd && there && isfinite(l)); who; who &= who - 1) {
+                const uint32_t mine = __ballot_sync(0xffffffffu, odd && there && isfinite(l));
+                if (lane == 0) S.odd[half][side][warp & 3] = mine;
+                pc_sync_half(half);
+                const float *q = a.q + q_row * a.q_stride + column;
+                for (uint32_t who = (mine | S.odd[half][side ^ 1][warp & 3]) & (side ? 0xFFFF0000u : 0xFFFFu); who; who &= who - 1) {   // (the two warps of the rows share them)
                     const int b = __ffs(who) - 1;
                     __syncwarp();
                     paged_repair<__half>(a, PC_KT, w.request, w.group, w.span, __shfl_sync(0xffffffffu, p, b), __shfl_sync(0xffffffffu, m, b),
                                          reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, (unsigned long long)q, b)), reinterpret_cast<float *>(__shfl_sync(0xffffffffu, (unsigned long long)out, b)), HS);
                 }
             }
+            pc_sync_half(half);   // (what is shared may be written again)
         } while (w.next(a, shape));
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PC_REGS_OTHER));
@@ -353,11 +376,11 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
             if (pg_elect()) {
                 const uint64_t qd = pc_desc_k(q0 + h * 2 * HALF), kd = pc_desc_k(ring + k_slot * HALF);
 #pragma unroll
-                for (uint32_t lo = 0; lo < 2; lo++)
+                for (uint32_t i = 0; i < 2; i++)   // the remainders first: the sums are small then, and what their additions drop too
 #pragma unroll
                     for (uint32_t k = 0; k < HS / 16; k++) {
                         const uint64_t at = (k / 4) * (16384 >> 4) + (k % 4) * (32 >> 4);
-                        pc_mma_ss(tmem + PC_S + 128 * h, qd + lo * (HALF >> 4) + at, kd + at, id_s, lo | k);
+                        pc_mma_ss(tmem + PC_S + 128 * h, qd + (1 - i) * (HALF >> 4) + at, kd + at, id_s, i | k);
                     }
                 pg_commit<false>(b_s + 8 * h);
             }
@@ -367,10 +390,9 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
             if (pg_elect()) {
                 const uint64_t vd = pc_desc_mn(ring + v_slot * HALF, 16384);
 #pragma unroll
-                for (uint32_t k = 0; k < 8; k++)
+                for (uint32_t i = 0; i < 2; i++)
 #pragma unroll
-                    for (uint32_t lo = 0; lo < 2; lo++)
-                        pg_mma<false>(tmem + PC_O + 128 * h, tmem + PC_S + 128 * h + 16 * k + 8 * lo, vd + k * (2048 >> 4), id_o, lo | k);
+                    for (uint32_t k = 0; k < 8; k++) pg_mma<false>(tmem + PC_O + 128 * h, tmem + PC_S + 128 * h + 16 * k + 8 * (1 - i), vd + k * (2048 >> 4), id_o, i | k);
                 pg_commit<false>(b_o + 8 * h);
             }
             __syncwarp();
@@ -394,6 +416,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
             return true;
         };
         bool two = rows_of() > 128;
+        park();
         uint32_t ks = take();
         if (ok && begin_half(0)) {
             scores(0, ks);
@@ -401,14 +424,15 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
             if (ok) release(ks);
         }
         for (bool more = true; more && ok;) {
-            uint32_t i = w.at;
-            const uint32_t end = w.at + w.count;
-            const int32_t kv_end = w.q.p0 + (int32_t)w.q.n;   // positions behind it: rows of the last page that hold nothing
-            const KeySpan span = w.span;
+            const PagedWalk<PC_KT> &now = kept;
+            uint32_t i = now.at;
+            const uint32_t end = now.at + now.count;
+            const int32_t kv_end = now.q.p0 + (int32_t)now.q.n;   // positions behind it: rows of the last page that hold nothing
+            const uint32_t sink_tiles = now.span.sink_tiles, first_tile = now.span.first;
             for (; i < end && ok; i++) {
                 const uint32_t vs = take();
                 if (!ok) break;
-                const int32_t base = (int32_t)(key_tile(span, i) * PC_KT);
+                const int32_t base = (int32_t)(key_tile({sink_tiles, first_tile, 0, 0}, i) * PC_KT);
                 if (base + (int32_t)PC_KT > kv_end) {
                     const uint32_t first = (uint32_t)max(kv_end - base, 0);
                     for (uint32_t c = 0; c < COLS; c++)
@@ -419,8 +443,10 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                 }
                 const bool was_two = two, fresh = i + 1 == end;   // fresh: the next key tile is another query tile's
                 if (fresh) {
+                    unpark();
                     more = w.next(a, shape);
                     if (more) two = rows_of() > 128;
+                    park();
                 }
                 if (!probabilities(0)) break;
                 products(0, vs);
@@ -451,11 +477,14 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
         // ===== TMA: K and V of a key tile, one slot of the ring each =====
         const uint32_t page_size = 1u << a.page_log2, box = page_size < PC_KT ? page_size : PC_KT, boxes = PC_KT / box;
         uint32_t slot = 0, use = 0;
+        bool more = true;
         do {
             const int32_t *table = a.table + (size_t)w.request * a.max_pages;
-            const int32_t kv_end = w.q.p0 + (int32_t)w.q.n;
-            for (uint32_t i = 0; i < w.count && ok; i++) {
-                const uint32_t j = key_tile(w.span, w.at + i) * PC_KT + lane * box;   // a lane per page
+            const int32_t kv_end = w.q.p0 + (int32_t)w.q.n, x = (int32_t)(w.group * HS);
+            const uint32_t at = w.at, end = w.at + w.count, sink_tiles = w.span.sink_tiles, first_tile = w.span.first;
+            park();
+            for (uint32_t i = at; i < end && ok; i++) {
+                const uint32_t j = key_tile({sink_tiles, first_tile, 0, 0}, i) * PC_KT + lane * box;   // a lane per page
                 int32_t page = -1;
                 if (lane < boxes && (int32_t)j < kv_end) page = table[j >> a.page_log2];
                 const bool there = page >= 0 && (uint32_t)page < a.n_pages;
@@ -468,12 +497,14 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                     __syncwarp();
                     if (there)
                         for (uint32_t c = 0; c < COLS; c++)
-                            pc_tma3d(dst + c * 16384, v ? &maps.v : &maps.k, (int32_t)(w.group * HS + 64 * c), (int32_t)(j & (page_size - 1)), page, full);
+                            pc_tma3d(dst + c * 16384, v ? &maps.v : &maps.k, x + (int32_t)(64 * c), (int32_t)(j & (page_size - 1)), page, full);
                     __syncwarp();
                     if (++slot == SLOTS) { slot = 0; use++; }
                 }
             }
-        } while (ok && w.next(a, shape));
+            unpark();
+            more = ok && w.next(a, shape);
+        } while (more);
       }
     }
     if (!ok) {   // a wait gave up: copies and products of this CTA may still be in flight; give them time to land before the CTA ends
