@@ -65,14 +65,21 @@ __device__ __forceinline__ void pc_tma3d(uint32_t dst, const CUtensorMap *map, i
                  : "memory");
 }
 
-// The wait for loads from tensor memory, with the registers that they fill: nothing that reads those can be moved ahead of it
-__device__ __forceinline__ void pc_wait_ld(uint32_t (&r)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
-                   "+r"(r[14]), "+r"(r[15])
-                 :
-                 : "memory");
+// 32 consecutive tensor-memory columns of the warp's 32 lanes.  The wait names the registers that the load fills: nothing that reads those can be moved ahead of it.
+#define PC_REGS32(C, r) \
+    C(r[0]), C(r[1]), C(r[2]), C(r[3]), C(r[4]), C(r[5]), C(r[6]), C(r[7]), C(r[8]), C(r[9]), C(r[10]), C(r[11]), C(r[12]), C(r[13]), C(r[14]), C(r[15]), C(r[16]), C(r[17]), C(r[18]), \
+        C(r[19]), C(r[20]), C(r[21]), C(r[22]), C(r[23]), C(r[24]), C(r[25]), C(r[26]), C(r[27]), C(r[28]), C(r[29]), C(r[30]), C(r[31])
+#define PC_NAMES32 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}"
+#define PC_OUT(x) "=r"(x)
+#define PC_BOTH(x) "+r"(x)
+__device__ __forceinline__ void pc_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 " PC_NAMES32 ", [%32];" : PC_REGS32(PC_OUT, r) : "r"(taddr) : "memory");
 }
+__device__ __forceinline__ void pc_wait_ld(uint32_t (&r)[32]) { asm volatile("tcgen05.wait::ld.sync.aligned;" : PC_REGS32(PC_BOTH, r) : : "memory"); }
+#undef PC_REGS32
+#undef PC_NAMES32
+#undef PC_OUT
+#undef PC_BOTH
 __device__ __forceinline__ void pc_sync_half(uint32_t half) {
     if (half) asm volatile("bar.sync 2, 256;" ::: "memory");
     else asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -210,22 +217,21 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                 if (!wait(bo, po, 12)) return;
                 po ^= 1;
                 pg_fence_after();
-                uint32_t o[2][16];
-                pg_ld16(t_o, o[0]);
-                pc_wait_ld(o[0]);
 #pragma unroll
-                for (int c = 0; c < (int)D / 16; c++) {
-                    if (c + 1 < (int)D / 16) pg_ld16(t_o + 16 * (c + 1), o[(c + 1) & 1]);
+                for (int c = 0; c < (int)D / 32; c++) {
+                    uint32_t o[32];
+                    pc_ld32(t_o + 32 * c, o);
+                    pc_wait_ld(o);
 #pragma unroll
-                    for (int e = 0; e < 16; e++) acc[16 * c + e] = fmaf(acc[16 * c + e], alpha, __uint_as_float(o[c & 1][e]));
-                    if (c + 1 < (int)D / 16) pc_wait_ld(o[(c + 1) & 1]);
+                    for (int e = 0; e < 32; e++) acc[32 * c + e] = fmaf(acc[32 * c + e], alpha, __uint_as_float(o[e]));
                 }
                 pg_fence_before();
                 __syncwarp();
                 if (lane == 0) pg_arrive(bf);
             };
             for (uint32_t i = 0; i < units && ok; i++) {
-                if (!wait(bs, ps, 12)) break;
+                if (i) fold();   // of the tile before: its products are done before this one's scores
+                if (!ok || !wait(bs, ps, 12)) break;
                 ps ^= 1;
                 pg_fence_after();
                 const int32_t base = (int32_t)(key_tile({sink_tiles, first_tile, 0, 0}, first_unit + i) * PC_KT) + 64 * (int32_t)side;
@@ -234,55 +240,62 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                 const int32_t last = p - base;
                 const int32_t from = a.window ? (int32_t)max((int64_t)p - a.window + 1 - base, (int64_t)-1) : -1, sinks = (int32_t)min((int64_t)a.sinks - base, (int64_t)64);
                 auto sees = [&](int32_t c) { return c <= last && (c >= from || c < sinks); };
+                // A load from tensor memory takes 300 clocks whatever its size (while products run), so it is of 32 columns, as many as there are registers for; the columns that are looked at last for
+                // the maximum are the first to become weights.
                 float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                uint32_t s[2][16];
-                pg_ld16(t_s, s[0]);
-                pc_wait_ld(s[0]);
+                uint32_t s[32];
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    pg_ld16(t_s + 16 * ((c + 1) & 3), s[(c + 1) & 1]);   // (the last one fetches the first for the next pass)
+                for (int c = 0; c < 2; c++) {
+                    pc_ld32(t_s + 32 * c, s);
+                    pc_wait_ld(s);
                     if (masked) {
 #pragma unroll
-                        for (int e = 0; e < 16; e++) tops[e & 3] = fmaxf(tops[e & 3], sees(16 * c + e) ? __uint_as_float(s[c & 1][e]) : -INFINITY);
+                        for (int e = 0; e < 32; e++) {
+                            if (!sees(32 * c + e)) s[e] = 0xFF800000u;
+                            tops[e & 3] = fmaxf(tops[e & 3], __uint_as_float(s[e]));
+                        }
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 16; e++) tops[e & 3] = fmaxf(tops[e & 3], __uint_as_float(s[c & 1][e]));
+                        for (int e = 0; e < 32; e++) tops[e & 3] = fmaxf(tops[e & 3], __uint_as_float(s[e]));
                     }
-                    pc_wait_ld(s[(c + 1) & 1]);
                 }
                 const float own = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), top = fmaxf(own, other(own));
                 const float m1 = fmaxf(m, ceilf(top * f)), bottom = m1 == -INFINITY ? 0.f : m1, alpha1 = paged_ex2(m - bottom), shift = PC_SHIFT - bottom;
                 m = m1;
                 float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    uint32_t o[16];
-                    if (c < 3) pg_ld16(t_s + 16 * (c + 1), s[(c + 1) & 1]);
-                    if (masked) {
+                for (int c = 1; c >= 0; c--) {
+                    if (c == 0) {
+                        pc_ld32(t_s, s);
+                        pc_wait_ld(s);
+                        if (masked) {
 #pragma unroll
-                        for (int e = 0; e < 16; e++)
-                            if (!sees(16 * c + e)) s[c & 1][e] = 0xFF800000u;
+                            for (int e = 0; e < 32; e++)
+                                if (!sees(e)) s[e] = 0xFF800000u;
+                        }
                     }
 #pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        const float x = paged_ex2(fmaf(__uint_as_float(s[c & 1][e]), f, shift)), y = paged_ex2(fmaf(__uint_as_float(s[c & 1][e + 1]), f, shift));
-                        sums[e & 2] += x;
-                        sums[(e & 2) + 1] += y;
-                        const __half2 h = __floats2half2_rn(x, y);
-                        const float2 g = __half22float2(h);
-                        const __half2 d = __floats2half2_rn(x - g.x, y - g.y);
-                        o[e / 2] = *reinterpret_cast<const uint32_t *>(&h);
-                        o[8 + e / 2] = *reinterpret_cast<const uint32_t *>(&d);
+                    for (int b = 0; b < 32; b += 16) {   // by 16 positions: their upper parts, then their remainders
+                        uint32_t o[16];
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) {
+                            const float x = paged_ex2(fmaf(__uint_as_float(s[b + e]), f, shift)), y = paged_ex2(fmaf(__uint_as_float(s[b + e + 1]), f, shift));
+                            sums[e & 2] += x;
+                            sums[(e & 2) + 1] += y;
+                            const __half2 h = __floats2half2_rn(x, y);
+                            const float2 g = __half22float2(h);
+                            const __half2 d = __floats2half2_rn(x - g.x, y - g.y);
+                            o[e / 2] = *reinterpret_cast<const uint32_t *>(&h);
+                            o[8 + e / 2] = *reinterpret_cast<const uint32_t *>(&d);
+                        }
+                        pg_st16(t_s + 32 * c + b, o);
                     }
-                    pg_st16(t_s + 16 * c, o);
-                    if (c < 3) pc_wait_ld(s[(c + 1) & 1]);
                 }
                 l = fmaf(l, alpha1, (sums[0] + sums[1]) + (sums[2] + sums[3]));
                 pg_wait_st();
                 pg_fence_before();
                 __syncwarp();
                 if (lane == 0) pg_arrive(bp);
-                if (i) fold();   // of the tile before: its products were done before these scores
                 alpha = alpha1;
             }
             if (ok) fold();
