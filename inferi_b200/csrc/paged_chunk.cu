@@ -39,6 +39,7 @@ constexpr uint32_t PC_MAX_SLOTS = 8;
 struct PcShared {   // behind Q and the ring
     uint64_t bars[2 * PC_MAX_SLOTS + 10];
     uint32_t tmem, last[2], odd[2][2][4];
+    int32_t lo[2], hi[2];          // positions of the halves' first tokens, and of their query tile's last one
     float x[2][2][128];            // what the two threads of a row tell one another
     PagedWalk<PC_KT> walk[4];      // the walks of the halves, of the MMA warp and of the TMA warp, while registers have other things to hold
     PagedRangeShared range;
@@ -166,6 +167,13 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
             if (half == 1 && rows_of() <= 128) continue;
             const uint32_t r = 128 * half + row, tt = r / a.kv_mul;
             const int32_t p = w.q.p0 + (int32_t)(w.tile * shape.tokens + tt);
+            if (side == 0 && (warp & 3) == 0) {   // (read behind the exchanges)
+                park();
+                if (lane == 0) {
+                    S.lo[half] = w.q.p0 + (int32_t)(w.tile * shape.tokens + 128 * half / a.kv_mul);
+                    S.hi[half] = w.q.p0 + (int32_t)min((w.tile + 1) * shape.tokens, w.q.n) - 1;
+                }
+            }
             float acc[D], f;
             {
                 const bool there = w.tile * shape.tokens + tt < w.q.n && tt < shape.tokens;
@@ -210,9 +218,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
 #pragma unroll
             for (int i = 0; i < (int)D; i++) acc[i] = 0.f;
             float m = -INFINITY, l = 0.f, alpha = 1.f;
-            const int32_t p_lo = w.q.p0 + (int32_t)(w.tile * shape.tokens + 128 * half / a.kv_mul), p_hi = w.q.p0 + (int32_t)min((w.tile + 1) * shape.tokens, w.q.n) - 1;
-            const uint32_t first_unit = w.at, units = w.count, sink_tiles = w.span.sink_tiles, first_tile = w.span.first;
-            if (side == 0 && (warp & 3) == 0) park();   // (read again behind the half's barrier below)
+            const volatile PagedWalk<PC_KT> &now = kept;   // (registers are short: what is read once per key tile is read from there)
             auto fold = [&]() {   // acc = alpha acc + O
                 if (!wait(bo, po, 12)) return;
                 po ^= 1;
@@ -229,14 +235,15 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                 __syncwarp();
                 if (lane == 0) pg_arrive(bf);
             };
-            for (uint32_t i = 0; i < units && ok; i++) {
+            for (uint32_t i = 0; i < now.count && ok; i++) {
                 if (i) fold();   // of the tile before: its products are done before this one's scores
+                const uint32_t unit = now.at + i, sink_tiles = now.span.sink_tiles;
+                const int32_t base = (int32_t)((unit < sink_tiles ? unit : now.span.first + unit - sink_tiles) * PC_KT + 64 * side);
+                const bool masked = base + 63 > *const_cast<volatile int32_t *>(&S.lo[half]) || (a.window && (int64_t)base + a.window <= *const_cast<volatile int32_t *>(&S.hi[half]));
                 if (!ok || !wait(bs, ps, 12)) break;
                 ps ^= 1;
                 pg_fence_after();
-                const int32_t base = (int32_t)(key_tile({sink_tiles, first_tile, 0, 0}, first_unit + i) * PC_KT) + 64 * (int32_t)side;
                 // which of its 64 columns the row sees: up to `last`, and of those from `from` on or ahead of `sinks`
-                const bool masked = base + 63 > p_lo || (a.window && (int64_t)base + a.window <= p_hi);
                 const int32_t last = p - base;
                 const int32_t from = a.window ? (int32_t)max((int64_t)p - a.window + 1 - base, (int64_t)-1) : -1, sinks = (int32_t)min((int64_t)a.sinks - base, (int64_t)64);
                 auto sees = [&](int32_t c) { return c <= last && (c >= from || c < sinks); };
@@ -376,111 +383,106 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PC_REGS_OTHER));
       if (warp == PC_W_MMA) {
         // ===== MMA issue =====
+        // Every product stands here once, in a loop: this warp's code competes with the halves' for the instruction caches, and code that has fallen out of them costs 12 clocks an
+        // instruction (written out for each place where a product is issued, an MMA took 75 clocks to issue).
         const uint32_t id_s = pg_idesc(128, 128), id_o = pg_idesc(128, HS) | 1u << 16;   // (V: MN-major)
-        uint32_t slot = 0, phase = 0;                                                     // of the ring
-        uint32_t pq[2] = {0, 0}, pp[2] = {0, 0}, n[2] = {0, 0};                            // parities; key tiles that a half has been given
+        uint32_t slot = 0, phase = 0;       // of the ring
+        uint32_t pq = 0, pp = 0, pf = 3;     // parities, a bit per half: of q's arrival, of P's, of O's release (which nobody has to wait for at first)
         auto take = [&]() {   // the next tile of the ring
             const uint32_t at = slot;
-            if (!wait(b_full + 8 * slot, phase, 11)) return at;
-            if (++slot == SLOTS) { slot = 0; phase ^= 1; }
+            if (wait(b_full + 8 * slot, phase, 11) && ++slot == SLOTS) { slot = 0; phase ^= 1; }
             return at;
         };
-        auto scores = [&](uint32_t h, uint32_t k_slot) {
-            if (pg_elect()) {
-                const uint64_t qd = pc_desc_k(q0 + h * 2 * HALF), kd = pc_desc_k(ring + k_slot * HALF);
-#pragma unroll
-                for (uint32_t i = 0; i < 2; i++)   // the remainders first: the sums are small then, and what their additions drop too
-#pragma unroll
-                    for (uint32_t k = 0; k < HS / 16; k++) {
-                        const uint64_t at = (k / 4) * (16384 >> 4) + (k % 4) * (32 >> 4);
-                        pc_mma_ss(tmem + PC_S + 128 * h, qd + (1 - i) * (HALF >> 4) + at, kd + at, id_s, i | k);
-                    }
-                pg_commit<false>(b_s + 8 * h);
-            }
+        auto release = [&](uint32_t at) {
+            if (pg_elect()) pg_commit<false>(b_empty + 8 * at);
             __syncwarp();
         };
-        auto products = [&](uint32_t h, uint32_t v_slot) {
-            if (pg_elect()) {
-                const uint64_t vd = pc_desc_mn(ring + v_slot * HALF, 16384);
-#pragma unroll
-                for (uint32_t i = 0; i < 2; i++)
-#pragma unroll
-                    for (uint32_t k = 0; k < 8; k++) pg_mma<false>(tmem + PC_O + 128 * h, tmem + PC_S + 128 * h + 16 * k + 8 * (1 - i), vd + k * (2048 >> 4), id_o, i | k);
-                pg_commit<false>(b_o + 8 * h);
-            }
-            __syncwarp();
+        bool was_two = false, two = rows_of() > 128, more = true, fresh = true;   // the query tile has rows in both halves: of this key tile, of the next one
+        uint32_t i = 0, end = 0, vs = 0, ks = 0;
+        int32_t kv_end = 0;
+        uint32_t sink_tiles = 0, first_tile = 0;
+        auto load = [&]() {
+            i = w.at;
+            end = w.at + w.count;
+            kv_end = w.q.p0 + (int32_t)w.q.n;   // positions behind it: rows of the last page that hold nothing
+            sink_tiles = w.span.sink_tiles;
+            first_tile = w.span.first;
         };
-        auto release = [&](uint32_t s) {
-            if (pg_elect()) pg_commit<false>(b_empty + 8 * s);
-            __syncwarp();
-        };
-        auto begin_half = [&](uint32_t h) {   // its q has arrived
-            if (!wait(b_q + 8 * h, pq[h], 12)) return false;
-            pq[h] ^= 1;
-            pg_fence_after();
-            return true;
-        };
-        auto probabilities = [&](uint32_t h) {   // P is there, and O's place is free
-            if (!wait(b_p + 8 * h, pp[h], 12)) return false;
-            pp[h] ^= 1;
-            if (n[h] && !wait(b_free + 8 * h, (n[h] - 1) & 1, 12)) return false;
-            n[h]++;
-            pg_fence_after();
-            return true;
-        };
-        bool two = rows_of() > 128;
-        park();
-        uint32_t ks = take();
-        if (ok && begin_half(0)) {
-            scores(0, ks);
-            if (two && begin_half(1)) scores(1, ks);
-            if (ok) release(ks);
-        }
-        for (bool more = true; more && ok;) {
-            const PagedWalk<PC_KT> &now = kept;
-            uint32_t i = now.at;
-            const uint32_t end = now.at + now.count;
-            const int32_t kv_end = now.q.p0 + (int32_t)now.q.n;   // positions behind it: rows of the last page that hold nothing
-            const uint32_t sink_tiles = now.span.sink_tiles, first_tile = now.span.first;
-            for (; i < end && ok; i++) {
-                const uint32_t vs = take();
+        bool began = false;   // the first round has scores to make only
+#pragma unroll 1
+        while (ok) {
+            if (began) {
+                vs = take();
                 if (!ok) break;
                 const int32_t base = (int32_t)(key_tile({sink_tiles, first_tile, 0, 0}, i) * PC_KT);
                 if (base + (int32_t)PC_KT > kv_end) {
                     const uint32_t first = (uint32_t)max(kv_end - base, 0);
                     for (uint32_t c = 0; c < COLS; c++)
+#pragma unroll 1
                         for (uint32_t at = first * 128 + lane * 16; at < 16384; at += 512)
                             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(ring + vs * HALF + c * 16384 + at), "r"(0u) : "memory");
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                 }
-                const bool was_two = two, fresh = i + 1 == end;   // fresh: the next key tile is another query tile's
+                was_two = two;
+                fresh = ++i == end;   // the next key tile is another query tile's
                 if (fresh) {
                     unpark();
                     more = w.next(a, shape);
                     if (more) two = rows_of() > 128;
-                    park();
-                }
-                if (!probabilities(0)) break;
-                products(0, vs);
-                if (!was_two) release(vs);
-                if (more) {
-                    ks = take();
-                    if (!ok || (fresh && !begin_half(0))) break;
-                    scores(0, ks);
-                    if (!two) release(ks);
-                }
-                if (was_two) {
-                    if (!probabilities(1)) break;
-                    products(1, vs);
-                    release(vs);
-                }
-                if (more && two) {
-                    if (fresh && !begin_half(1)) break;
-                    scores(1, ks);
-                    release(ks);
                 }
             }
+            if (fresh && more) {
+                load();
+                park();
+            }
+#pragma unroll 1
+            for (uint32_t h = 0; h < 2 && ok; h++) {
+                if (began && (h == 0 || was_two)) {   // O = P V, once P is there and O's place is free
+                    if (!wait(b_p + 8 * h, (pp >> h) & 1, 12) || !wait(b_free + 8 * h, (pf >> h) & 1, 12)) break;
+                    pp ^= 1u << h;
+                    pf ^= 1u << h;
+                    pg_fence_after();
+                    if (pg_elect()) {
+                        uint64_t vd = pc_desc_mn(ring + vs * HALF, 16384);
+                        const uint32_t d = tmem + PC_O + 128 * h, p = tmem + PC_S + 128 * h;
+#pragma unroll 1
+                        for (uint32_t hi = 0; hi < 2; hi++)   // the remainders first: the sums are small then, and what their additions drop too
+#pragma unroll
+                            for (uint32_t k = 0; k < 8; k++) pg_mma<false>(d, p + 8 - 8 * hi + 16 * k, vd + k * (2048 >> 4), id_o, hi | k);
+                        pg_commit<false>(b_o + 8 * h);
+                    }
+                    __syncwarp();
+                    if (h == (was_two ? 1u : 0u)) release(vs);
+                }
+                if (more && (h == 0 || two)) {   // S = Q K^T of the next key tile
+                    if (h == 0) ks = take();
+                    if (!ok) break;
+                    if (fresh) {
+                        if (!wait(b_q + 8 * h, (pq >> h) & 1, 12)) break;
+                        pq ^= 1u << h;
+                        pg_fence_after();
+                    }
+                    if (pg_elect()) {
+                        const uint64_t kd = pc_desc_k(ring + ks * HALF), qd = pc_desc_k(q0 + h * 2 * HALF);
+                        const uint32_t d = tmem + PC_S + 128 * h;
+#pragma unroll 1
+                        for (uint32_t hi = 0; hi < 2; hi++) {
+                            const uint64_t q1 = qd + (1 - hi) * (HALF >> 4);
+#pragma unroll
+                            for (uint32_t k = 0; k < HS / 16; k++) {
+                                const uint32_t at = (k / 4) * (16384 >> 4) + (k % 4) * (32 >> 4);
+                                pc_mma_ss(d, q1 + at, kd + at, id_s, hi | k);
+                            }
+                        }
+                        pg_commit<false>(b_s + 8 * h);
+                    }
+                    __syncwarp();
+                    if (h == (two ? 1u : 0u)) release(ks);
+                }
+            }
+            if (!more) break;
+            began = true;
         }
         if (ok) {   // the last commits arrive in shared memory: let them, before the CTA ends
             const uint32_t last = (slot + SLOTS - 1) % SLOTS;
