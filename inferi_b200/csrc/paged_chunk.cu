@@ -15,10 +15,12 @@
 // Who does what (20 warps, one CTA per SM):
 //   warps 0-7, 8-15  a half each: two threads per row, each with half of the key tile's scores and of the result's columns.  Load and split q, softmax, fold, result.  (A thread per row
 //                    had a chain of 4600 clocks from the scores to the next product, 128 sums in registers and no room for the rest)
-//   warp 16          MMA issue
-//   warp 17          TMA copies of K and V: a ring of tiles, a copy per page and 64 columns, swizzled by 128 bytes
-//   warps 18, 19     nothing (registers change hands by groups of four warps)
-// They hand over through mbarriers.  Order of the MMAs: S0 S1 | O0 S0' O1 S1' | O0' S0'' ...: a half's softmax has the time of the other's two products.
+//   warps 16, 17     MMA issue, of a half each
+//   warp 18          TMA copies of K and V: a ring of tiles, a copy per page and 64 columns, swizzled by 128 bytes
+//   warp 19          nothing (registers change hands by groups of four warps)
+// They hand over through mbarriers.  Order of the MMAs: S0 S1 | O0 S0' O1 S1' | O0' S0'' ...: a half's softmax has the time of the other's two products.  The tensor cores take no more than
+// three or four MMAs ahead, so what the issuing warp does between two products is time that they stand still (700 clocks of every 2600 with one warp for both halves): there are two, which take
+// turns, and each waits for its operands while the other one's products run.  From a product with A in shared memory to one with A in tensor memory the tensor cores lose 215 clocks.
 // Tensor memory (512 columns): S0 / P0, S1 / P1, O0, O1 of 128 columns each.  P's operands are interleaved by 16 positions, hi then lo, so that a thread overwrites only scores that it has read.
 //
 // Every wait is bounded; a wait that gives up raises the context's error word, and the kernel returns after freeing its tensor memory.
@@ -27,7 +29,7 @@
 
 namespace ib {
 
-constexpr uint32_t PC_THREADS = 640, PC_KT = 128, PC_ROWS = 256, PC_W_MMA = 16, PC_W_TMA = 17;
+constexpr uint32_t PC_THREADS = 640, PC_KT = 128, PC_ROWS = 256, PC_W_MMA = 16, PC_W_TMA = 18;
 // Registers: 640 threads at 96 are what the block is launched with; the halves' warps take 104 of them, the others keep 64 (512 * 104 + 128 * 64 = 640 * 96).
 constexpr uint32_t PC_REGS_HALF = 104, PC_REGS_OTHER = 64;
 constexpr uint32_t PC_S = 0, PC_O = 256;   // tensor memory columns; the halves' are 128 apart
@@ -37,11 +39,11 @@ constexpr uint32_t pc_half(uint32_t hs) { return 128 * hs * 2; }       // bytes 
 constexpr uint32_t pc_slots(uint32_t hs) { return hs == 128 ? 3u : 8u; }
 constexpr uint32_t PC_MAX_SLOTS = 8;
 struct PcShared {   // behind Q and the ring
-    uint64_t bars[2 * PC_MAX_SLOTS + 10];
+    uint64_t bars[2 * PC_MAX_SLOTS + 12];
     uint32_t tmem, last[2], odd[2][2][4];
     int32_t lo[2], hi[2];          // positions of the halves' first tokens, and of their query tile's last one
     float x[2][2][128];            // what the two threads of a row tell one another
-    PagedWalk<PC_KT> walk[4];      // the walks of the halves, of the MMA warp and of the TMA warp, while registers have other things to hold
+    PagedWalk<PC_KT> walk[5];      // the walks of the halves, of the MMA warps and of the TMA warp, while registers have other things to hold
     PagedRangeShared range;
 };
 constexpr uint32_t pc_smem(uint32_t hs) { return (4 + pc_slots(hs)) * pc_half(hs) + (uint32_t)sizeof(PcShared); }
@@ -102,6 +104,10 @@ __device__ __forceinline__ bool pc_wait(uint32_t bar, uint32_t parity, const Pag
     return true;
 }
 
+// A value that all lanes hold, in a uniform register.  MMAs take their operands from those; of what comes from memory the compiler does not know that it is uniform, nor of what hangs on it, and
+// moves every operand of every MMA over by itself (70 clocks an MMA instead of 20).
+__device__ __forceinline__ uint32_t pc_uniform(uint32_t x) { return __reduce_or_sync(0xffffffffu, x); }
+
 struct PcMaps { CUtensorMap k, v; };
 
 template <int HS>
@@ -110,20 +116,24 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
     extern __shared__ __align__(1024) uint8_t smem[];   // (the swizzle's alignment; there is no static shared memory ahead of it)
     PcShared &S = *reinterpret_cast<PcShared *>(smem + (4 + SLOTS) * HALF);
     const uint32_t q0 = pg_smem(smem), ring = q0 + 4 * HALF, bars = pg_smem(S.bars);   // Q: [half][hi, lo]
-    const uint32_t b_full = bars, b_empty = b_full + 8 * SLOTS, b_q = b_empty + 8 * SLOTS, b_s = b_q + 16, b_p = b_s + 16, b_o = b_p + 16, b_free = b_o + 16;
+    const uint32_t b_full = bars, b_empty = b_full + 8 * SLOTS, b_q = b_empty + 8 * SLOTS, b_s = b_q + 16, b_p = b_s + 16, b_o = b_p + 16, b_free = b_o + 16, b_turn = b_free + 16;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const PagedRange range = paged_range<PC_KT, PC_THREADS>(a, shape, S.range);
     if (range.total == 0 || blockIdx.x >= range.ranges) return;
     if (warp == 0 && lane == 0) {
-        for (uint32_t i = 0; i < 2 * SLOTS; i++) pg_bar_init(b_full + 8 * i, 1);
+        for (uint32_t i = 0; i < SLOTS; i++) {
+            pg_bar_init(b_full + 8 * i, 1);
+            pg_bar_init(b_empty + 8 * i, 2);   // both MMA warps
+        }
         for (uint32_t h = 0; h < 2; h++) {
             pg_bar_init(b_q + 8 * h, 8);      // a half's warps
             pg_bar_init(b_s + 8 * h, 1);      // the MMAs' completion
             pg_bar_init(b_p + 8 * h, 8);
             pg_bar_init(b_o + 8 * h, 1);
             pg_bar_init(b_free + 8 * h, 8);
+            pg_bar_init(b_turn + 8 * h, 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -131,7 +141,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
     pg_fence_before();
     __syncthreads();
     pg_fence_after();
-    const uint32_t tmem = *const_cast<volatile uint32_t *>(&S.tmem);
+    const uint32_t tmem = pc_uniform(*const_cast<volatile uint32_t *>(&S.tmem));
     bool ok = true;
     auto wait = [&](uint32_t bar, uint32_t parity, uint32_t code) {
         ok = __all_sync(0xffffffffu, pc_wait(bar, parity, a, code));
@@ -139,7 +149,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
     };
     PagedWalk<PC_KT> w;
     w.begin(a, shape, range);
-    PagedWalk<PC_KT> &kept = S.walk[warp < PC_W_MMA ? warp >> 3 : 2 + (warp & 1)];
+    PagedWalk<PC_KT> &kept = S.walk[warp < PC_W_MMA ? warp >> 3 : 2 + (warp - PC_W_MMA) % 3];
     auto park = [&]() {
         __syncwarp();
         if (lane == 0) kept = w;
@@ -381,41 +391,33 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
         } while (w.next(a, shape));
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PC_REGS_OTHER));
-      if (warp == PC_W_MMA) {
-        // ===== MMA issue =====
-        // Every product stands here once, in a loop: this warp's code competes with the halves' for the instruction caches, and code that has fallen out of them costs 12 clocks an
-        // instruction (written out for each place where a product is issued, an MMA took 75 clocks to issue).
-        const uint32_t id_s = pg_idesc(128, 128), id_o = pg_idesc(128, HS) | 1u << 16;   // (V: MN-major)
-        uint32_t slot = 0, phase = 0;       // of the ring
-        uint32_t pq = 0, pp = 0, pf = 3;     // parities, a bit per half: of q's arrival, of P's, of O's release (which nobody has to wait for at first)
+      if (warp < PC_W_TMA) {
+        // ===== MMA issue of a half =====
+        // Every product stands here once: this code competes with the halves' for the instruction caches.
+        const uint32_t h = pc_uniform(warp - PC_W_MMA), id_s = pg_idesc(128, 128), id_o = pg_idesc(128, HS) | 1u << 16;   // (V: MN-major)
+        const uint32_t t_s = tmem + PC_S + 128 * h, t_o = tmem + PC_O + 128 * h;
+        const uint64_t q_lo = pc_desc_k(q0 + h * 2 * HALF + HALF);
+        uint32_t slot = 0, phase = 0;                        // of the ring
+        uint32_t pq = 0, pp = 0, po = 0, pf = 1, pt = h ^ 1;  // parities: of q's arrival, of P's, of O, of O's release (nobody has to be waited for at first), of the turn (the first half begins)
         auto take = [&]() {   // the next tile of the ring
             const uint32_t at = slot;
             if (wait(b_full + 8 * slot, phase, 11) && ++slot == SLOTS) { slot = 0; phase ^= 1; }
             return at;
         };
-        auto release = [&](uint32_t at) {
-            if (pg_elect()) pg_commit<false>(b_empty + 8 * at);
-            __syncwarp();
-        };
-        bool was_two = false, two = rows_of() > 128, more = true, fresh = true;   // the query tile has rows in both halves: of this key tile, of the next one
-        uint32_t i = 0, end = 0, vs = 0, ks = 0;
+        // The walk is the same for both; a half without rows passes its turns on.
+        bool now = false, two = pc_uniform(rows_of() > 128), more = true, fresh = true;   // now: the half has rows in this key tile's query tile; two: both have in the next one's
+        uint32_t left = 0, vs = 0, ks = 0;                                               // left: key tiles of the query tile
+        uint32_t unit = 0, sink_tiles = 0, first_tile = 0;
         int32_t kv_end = 0;
-        uint32_t sink_tiles = 0, first_tile = 0;
-        auto load = [&]() {
-            i = w.at;
-            end = w.at + w.count;
-            kv_end = w.q.p0 + (int32_t)w.q.n;   // positions behind it: rows of the last page that hold nothing
-            sink_tiles = w.span.sink_tiles;
-            first_tile = w.span.first;
-        };
         bool began = false;   // the first round has scores to make only
 #pragma unroll 1
         while (ok) {
+            const bool products = began;
             if (began) {
                 vs = take();
                 if (!ok) break;
-                const int32_t base = (int32_t)(key_tile({sink_tiles, first_tile, 0, 0}, i) * PC_KT);
-                if (base + (int32_t)PC_KT > kv_end) {
+                const int32_t base = (int32_t)(key_tile({sink_tiles, first_tile, 0, 0}, unit++) * PC_KT);
+                if (__any_sync(0xffffffffu, base + (int32_t)PC_KT > kv_end)) {   // rows of the last page that hold nothing: zeros (both warps write them)
                     const uint32_t first = (uint32_t)max(kv_end - base, 0);
                     for (uint32_t c = 0; c < COLS; c++)
 #pragma unroll 1
@@ -424,65 +426,79 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                 }
-                was_two = two;
-                fresh = ++i == end;   // the next key tile is another query tile's
+                now = h == 0 || two;
+                fresh = --left == 0;   // the next key tile is another query tile's
                 if (fresh) {
                     unpark();
-                    more = w.next(a, shape);
-                    if (more) two = rows_of() > 128;
+                    more = __any_sync(0xffffffffu, w.next(a, shape));
+                    if (more) two = pc_uniform(rows_of() > 128);
                 }
             }
+            began = true;
             if (fresh && more) {
-                load();
+                left = pc_uniform(w.count);
+                unit = w.at;
+                kv_end = w.q.p0 + (int32_t)w.q.n;
+                sink_tiles = w.span.sink_tiles;
+                first_tile = w.span.first;
                 park();
             }
-#pragma unroll 1
-            for (uint32_t h = 0; h < 2 && ok; h++) {
-                if (began && (h == 0 || was_two)) {   // O = P V, once P is there and O's place is free
-                    if (!wait(b_p + 8 * h, (pp >> h) & 1, 12) || !wait(b_free + 8 * h, (pf >> h) & 1, 12)) break;
-                    pp ^= 1u << h;
-                    pf ^= 1u << h;
-                    pg_fence_after();
-                    if (pg_elect()) {
-                        uint64_t vd = pc_desc_mn(ring + vs * HALF, 16384);
-                        const uint32_t d = tmem + PC_O + 128 * h, p = tmem + PC_S + 128 * h;
-#pragma unroll 1
-                        for (uint32_t hi = 0; hi < 2; hi++)   // the remainders first: the sums are small then, and what their additions drop too
-#pragma unroll
-                            for (uint32_t k = 0; k < 8; k++) pg_mma<false>(d, p + 8 - 8 * hi + 16 * k, vd + k * (2048 >> 4), id_o, hi | k);
-                        pg_commit<false>(b_o + 8 * h);
-                    }
-                    __syncwarp();
-                    if (h == (was_two ? 1u : 0u)) release(vs);
-                }
-                if (more && (h == 0 || two)) {   // S = Q K^T of the next key tile
-                    if (h == 0) ks = take();
-                    if (!ok) break;
-                    if (fresh) {
-                        if (!wait(b_q + 8 * h, (pq >> h) & 1, 12)) break;
-                        pq ^= 1u << h;
-                        pg_fence_after();
-                    }
-                    if (pg_elect()) {
-                        const uint64_t kd = pc_desc_k(ring + ks * HALF), qd = pc_desc_k(q0 + h * 2 * HALF);
-                        const uint32_t d = tmem + PC_S + 128 * h;
-#pragma unroll 1
-                        for (uint32_t hi = 0; hi < 2; hi++) {
-                            const uint64_t q1 = qd + (1 - hi) * (HALF >> 4);
-#pragma unroll
-                            for (uint32_t k = 0; k < HS / 16; k++) {
-                                const uint32_t at = (k / 4) * (16384 >> 4) + (k % 4) * (32 >> 4);
-                                pc_mma_ss(d, q1 + at, kd + at, id_s, hi | k);
-                            }
-                        }
-                        pg_commit<false>(b_s + 8 * h);
-                    }
-                    __syncwarp();
-                    if (h == (two ? 1u : 0u)) release(ks);
-                }
+            const bool next = more && (h == 0 || two);
+            if (more) ks = take();
+            if (!ok) break;
+            if (products && now) {   // P is there, and O's place is free
+                if (!wait(b_p + 8 * h, pp, 12) || !wait(b_free + 8 * h, pf, 12)) break;
+                pp ^= 1;
+                pf ^= 1;
             }
+            if (!wait(b_turn + 8 * h, pt, 12)) break;
+            pt ^= 1;
+            pg_fence_after();
+            if (products && now) {   // O = P V
+                if (pg_elect()) {
+                    const uint64_t vd = pc_desc_mn(ring + vs * HALF, 16384);
+#pragma unroll 1
+                    for (uint32_t hi = 0; hi < 2; hi++)   // the remainders first: the sums are small then, and what their additions drop too
+#pragma unroll
+                        for (uint32_t k = 0; k < 8; k++) pg_mma<false>(t_o, t_s + 8 - 8 * hi + 16 * k, vd + k * (2048 >> 4), id_o, hi | k);
+                    pg_commit<false>(b_o + 8 * h);
+                    pg_commit<false>(b_empty + 8 * vs);
+                }
+                __syncwarp();
+                // The scores take P's place: only when the products are through with it.  (MMAs with different accumulators are not ordered among themselves.)
+                if (!wait(b_o + 8 * h, po, 12)) break;
+                po ^= 1;
+            }
+            if (fresh && products && more) {   // The half has to write this query tile's result before it brings the next one's q; the other half's products do not wait for that.
+                if (pg_elect()) pg_arrive(b_turn + 8 * (h ^ 1));
+                __syncwarp();
+                if (next && !wait(b_q + 8 * h, pq, 12)) break;
+                if (!wait(b_turn + 8 * h, pt, 12)) break;
+                pt ^= 1;
+            } else if (fresh && next && !wait(b_q + 8 * h, pq, 12)) break;   // (the first one)
+            if (fresh && next) pq ^= 1;
+            pg_fence_after();
+            if (pg_elect()) {
+                if (next) {   // S = Q K^T of the next key tile
+                    const uint64_t kd = pc_desc_k(ring + ks * HALF);
+#pragma unroll 1
+                    for (uint32_t hi = 0; hi < 2; hi++) {
+                        const uint64_t qd = q_lo - hi * (HALF >> 4);
+#pragma unroll
+                        for (uint32_t k = 0; k < HS / 16; k++) {
+                            const uint32_t at = (k / 4) * (16384 >> 4) + (k % 4) * (32 >> 4);
+                            pc_mma_ss(t_s, qd + at, kd + at, id_s, hi | k);
+                        }
+                    }
+                    pg_commit<false>(b_s + 8 * h);
+                    pg_commit<false>(b_empty + 8 * ks);
+                }
+                pg_arrive(b_turn + 8 * (h ^ 1));
+                if (products && !now) pg_arrive(b_empty + 8 * vs);   // (without rows: the tiles are not needed)
+                if (more && !next) pg_arrive(b_empty + 8 * ks);
+            }
+            __syncwarp();
             if (!more) break;
-            began = true;
         }
         if (ok) {   // the last commits arrive in shared memory: let them, before the CTA ends
             const uint32_t last = (slot + SLOTS - 1) % SLOTS;
