@@ -68,21 +68,29 @@ __device__ __forceinline__ void pc_tma3d(uint32_t dst, const CUtensorMap *map, i
                  : "memory");
 }
 
-// 32 consecutive tensor-memory columns of the warp's 32 lanes.  The wait names the registers that the load fills: nothing that reads those can be moved ahead of it.
+// 16 or 32 consecutive tensor-memory columns of the warp's 32 lanes.  The wait names the registers that the load fills: nothing that reads those can be moved ahead of it.
 #define PC_REGS32(C, r) \
     C(r[0]), C(r[1]), C(r[2]), C(r[3]), C(r[4]), C(r[5]), C(r[6]), C(r[7]), C(r[8]), C(r[9]), C(r[10]), C(r[11]), C(r[12]), C(r[13]), C(r[14]), C(r[15]), C(r[16]), C(r[17]), C(r[18]), \
         C(r[19]), C(r[20]), C(r[21]), C(r[22]), C(r[23]), C(r[24]), C(r[25]), C(r[26]), C(r[27]), C(r[28]), C(r[29]), C(r[30]), C(r[31])
 #define PC_NAMES32 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}"
 #define PC_OUT(x) "=r"(x)
 #define PC_BOTH(x) "+r"(x)
-__device__ __forceinline__ void pc_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+__device__ __forceinline__ void pc_load(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 " PC_NAMES32 ", [%32];" : PC_REGS32(PC_OUT, r) : "r"(taddr) : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : PC_REGS32(PC_BOTH, r) : : "memory");
 }
-__device__ __forceinline__ void pc_wait_ld(uint32_t (&r)[32]) { asm volatile("tcgen05.wait::ld.sync.aligned;" : PC_REGS32(PC_BOTH, r) : : "memory"); }
 #undef PC_REGS32
 #undef PC_NAMES32
 #undef PC_OUT
 #undef PC_BOTH
+__device__ __forceinline__ void pc_load(uint32_t taddr, uint32_t (&r)[16]) {
+    pg_ld16(taddr, r);
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
+                   "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void pc_sync_half(uint32_t half) {
     if (half) asm volatile("bar.sync 2, 256;" ::: "memory");
     else asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -172,7 +180,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
             pc_sync_half(half);
             return S.x[half][side ^ 1][row];
         };
-        uint32_t ps = 0, po = 0;   // parities
+        uint32_t ps = 0;   // parity of the scores; that of the products before them is the other one
         do {
             if (half == 1 && rows_of() <= 128) continue;
             const uint32_t r = 128 * half + row, tt = r / a.kv_mul;
@@ -230,14 +238,12 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
             float m = -INFINITY, l = 0.f, alpha = 1.f;
             const volatile PagedWalk<PC_KT> &now = kept;   // (registers are short: what is read once per key tile is read from there)
             auto fold = [&]() {   // acc = alpha acc + O
-                if (!wait(bo, po, 12)) return;
-                po ^= 1;
+                if (!wait(bo, ps ^ 1, 12)) return;
                 pg_fence_after();
 #pragma unroll
                 for (int c = 0; c < (int)D / 32; c++) {
                     uint32_t o[32];
-                    pc_ld32(t_o + 32 * c, o);
-                    pc_wait_ld(o);
+                    pc_load(t_o + 32 * c, o);
 #pragma unroll
                     for (int e = 0; e < 32; e++) acc[32 * c + e] = fmaf(acc[32 * c + e], alpha, __uint_as_float(o[e]));
                 }
@@ -257,58 +263,57 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                 const int32_t last = p - base;
                 const int32_t from = a.window ? (int32_t)max((int64_t)p - a.window + 1 - base, (int64_t)-1) : -1, sinks = (int32_t)min((int64_t)a.sinks - base, (int64_t)64);
                 auto sees = [&](int32_t c) { return c <= last && (c >= from || c < sinks); };
-                // A load from tensor memory takes 300 clocks whatever its size (while products run), so it is of 32 columns, as many as there are registers for; the columns that are looked at last for
-                // the maximum are the first to become weights.
-                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                uint32_t s[32];
+                // A load from tensor memory takes 200 clocks and more whatever its size (while products run), so it is of as many columns as there are registers for; those that are looked at
+                // last for the maximum are the first to become weights.
+                constexpr int ST = HS == 128 ? 16 : 32, NC = 64 / ST;   // (HS 128, in pieces of 32: 474 us instead of 464; HS 64, of 16: 165 instead of 155)
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, sums[2];
+                uint32_t s[ST];
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    pc_ld32(t_s + 32 * c, s);
-                    pc_wait_ld(s);
+                for (int c = 0; c < NC; c++) {
+                    pc_load(t_s + ST * c, s);
                     if (masked) {
 #pragma unroll
-                        for (int e = 0; e < 32; e++) {
-                            if (!sees(32 * c + e)) s[e] = 0xFF800000u;
+                        for (int e = 0; e < ST; e++) {
+                            if (!sees(ST * c + e)) s[e] = 0xFF800000u;
                             tops[e & 3] = fmaxf(tops[e & 3], __uint_as_float(s[e]));
                         }
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 32; e++) tops[e & 3] = fmaxf(tops[e & 3], __uint_as_float(s[e]));
+                        for (int e = 0; e < ST; e++) tops[e & 3] = fmaxf(tops[e & 3], __uint_as_float(s[e]));
                     }
                 }
                 const float own = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), top = fmaxf(own, other(own));
                 const float m1 = fmaxf(m, ceilf(top * f)), bottom = m1 == -INFINITY ? 0.f : m1, alpha1 = paged_ex2(m - bottom), shift = PC_SHIFT - bottom;
                 m = m1;
-                float sums[4] = {0.f, 0.f, 0.f, 0.f};
+                sums[0] = sums[1] = 0.f;
 #pragma unroll
-                for (int c = 1; c >= 0; c--) {
-                    if (c == 0) {
-                        pc_ld32(t_s, s);
-                        pc_wait_ld(s);
+                for (int c = NC - 1; c >= 0; c--) {
+                    if (c < NC - 1) {
+                        pc_load(t_s + ST * c, s);
                         if (masked) {
 #pragma unroll
-                            for (int e = 0; e < 32; e++)
-                                if (!sees(e)) s[e] = 0xFF800000u;
+                            for (int e = 0; e < ST; e++)
+                                if (!sees(ST * c + e)) s[e] = 0xFF800000u;
                         }
                     }
 #pragma unroll
-                    for (int b = 0; b < 32; b += 16) {   // by 16 positions: their upper parts, then their remainders
+                    for (int b = 0; b < ST; b += 16) {   // by 16 positions: their upper parts, then their remainders
                         uint32_t o[16];
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) {
                             const float x = paged_ex2(fmaf(__uint_as_float(s[b + e]), f, shift)), y = paged_ex2(fmaf(__uint_as_float(s[b + e + 1]), f, shift));
-                            sums[e & 2] += x;
-                            sums[(e & 2) + 1] += y;
+                            sums[0] += x;
+                            sums[1] += y;
                             const __half2 h = __floats2half2_rn(x, y);
                             const float2 g = __half22float2(h);
                             const __half2 d = __floats2half2_rn(x - g.x, y - g.y);
                             o[e / 2] = *reinterpret_cast<const uint32_t *>(&h);
                             o[8 + e / 2] = *reinterpret_cast<const uint32_t *>(&d);
                         }
-                        pg_st16(t_s + 32 * c + b, o);
+                        pg_st16(t_s + ST * c + b, o);
                     }
                 }
-                l = fmaf(l, alpha1, (sums[0] + sums[1]) + (sums[2] + sums[3]));
+                l = fmaf(l, alpha1, sums[0] + sums[1]);
                 pg_wait_st();
                 pg_fence_before();
                 __syncwarp();
@@ -348,12 +353,11 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                     for (int i = 0; i < (int)D; i++) acc[i] = 0.f;
                     for (uint32_t k = c0; k <= c1; k++) m = fmaxf(m, __ldcg(a.scratch + ((size_t)paged_place(range, w.tile_unit(), k) * 2 + half) * pc_partial_floats(HS) + 128 * HS + row));
                     for (uint32_t k = c0; k <= c1; k++) {
-                        const float *from = a.scratch + ((size_t)paged_place(range, w.tile_unit(), k) * 2 + half) * pc_partial_floats(HS) + row;
-                        const float wt = m == -INFINITY ? 0.f : paged_ex2(__ldcg(from + 128 * HS) - m);
-                        l += wt * __ldcg(from + 128 * (HS + 1));
-                        from += 128 * D * side;
+                        const float *from = a.scratch + ((size_t)paged_place(range, w.tile_unit(), k) * 2 + half) * pc_partial_floats(HS);
+                        const float wt = m == -INFINITY ? 0.f : paged_ex2(__ldcg(from + 128 * HS + row) - m);
+                        l += wt * __ldcg(from + 128 * (HS + 1) + row);
 #pragma unroll
-                        for (int i = 0; i < (int)D; i++) acc[i] = fmaf(wt, __ldcg(from + 128 * i), acc[i]);
+                        for (int i = 0; i < (int)D; i++) acc[i] = fmaf(wt, __ldcg(from + 128 * (D * side + i) + row), acc[i]);
                     }
                 }
             }
