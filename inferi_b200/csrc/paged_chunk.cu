@@ -192,47 +192,53 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                     S.hi[half] = w.q.p0 + (int32_t)min((w.tile + 1) * shape.tokens, w.q.n) - 1;
                 }
             }
-            float acc[D], f;
-            {
-                const bool there = w.tile * shape.tokens + tt < w.q.n && tt < shape.tokens;
-                const float *q = a.q + (uint64_t)(w.q.start + w.tile * shape.tokens + tt) * a.q_stride + (uint64_t)(w.group * a.kv_mul + r % a.kv_mul) * HS + D * side;
-                float most = 0.f;
+            // q: a warp takes rows as they lie in memory (a thread with a row of its own would touch 32 lines with every load), 16 of the half's
+            constexpr uint32_t LANES = HS / 4, AT_ONCE = 32 / LANES, LOADS = 4;   // lanes of a row, rows of a load, loads in flight
+            const uint32_t column = 4 * (lane % LANES);
+#pragma unroll 1
+            for (uint32_t i = 0; i < 16; i += LOADS * AT_ONCE) {
+                float4 v[LOADS];
 #pragma unroll
-                for (int i = 0; i < (int)D; i += 4) {
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (there) {
-                        if (a.vec) v = *reinterpret_cast<const float4 *>(q + i);
-                        else v = make_float4(q[i], q[i + 1], q[i + 2], q[i + 3]);
+                for (uint32_t k = 0; k < LOADS; k++) {
+                    const uint32_t rr = 16 * (warp & 7) + i + k * AT_ONCE + lane / LANES, at = 128 * half + rr, token = at / a.kv_mul;
+                    v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (token < shape.tokens && w.tile * shape.tokens + token < w.q.n) {
+                        const float *q = a.q + (uint64_t)(w.q.start + w.tile * shape.tokens + token) * a.q_stride + (uint64_t)(w.group * a.kv_mul + at % a.kv_mul) * HS + column;
+                        if (a.vec) v[k] = *reinterpret_cast<const float4 *>(q);
+                        else v[k] = make_float4(q[0], q[1], q[2], q[3]);
                     }
-                    acc[i] = v.x; acc[i + 1] = v.y; acc[i + 2] = v.z; acc[i + 3] = v.w;
-                    most = fmaxf(fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
                 }
-                most = fmaxf(most, other(most));
-                const int e2 = paged_exponent(most);
-                const float down = exp2f((float)-e2);
-                f = exp2f((float)e2) * (1.4426950408889634f / sqrtf((float)HS));
-                // 16-byte piece c of a row lies at piece c ^ (row % 8)
-                const uint32_t to = q0 + half * 2 * HALF + row * 128;
 #pragma unroll
-                for (uint32_t i = 0; i < D / 8; i++) {
-                    uint32_t hi[4], lo[4];
+                for (uint32_t k = 0; k < LOADS; k++) {
+                    const uint32_t rr = 16 * (warp & 7) + i + k * AT_ONCE + lane / LANES;
+                    float most = fmaxf(fmaxf(fabsf(v[k].x), fabsf(v[k].y)), fmaxf(fabsf(v[k].z), fabsf(v[k].w)));
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float x = acc[8 * i + 2 * e] * down, y = acc[8 * i + 2 * e + 1] * down;
-                        const __half2 h = __floats2half2_rn(x, y);
+                    for (uint32_t o = LANES / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                    const int e2 = paged_exponent(most);
+                    const float down = exp2f((float)-e2);
+                    if (column == 0) S.x[half][0][rr] = exp2f((float)e2) * (1.4426950408889634f / sqrtf((float)HS));
+                    const float x[4] = {v[k].x * down, v[k].y * down, v[k].z * down, v[k].w * down};
+                    uint32_t hi[2], lo[2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const __half2 h = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
                         const float2 g = __half22float2(h);
-                        const __half2 l = __floats2half2_rn(x - g.x, y - g.y);
+                        const __half2 l = __floats2half2_rn(x[2 * e] - g.x, x[2 * e + 1] - g.y);
                         hi[e] = *reinterpret_cast<const uint32_t *>(&h);
                         lo[e] = *reinterpret_cast<const uint32_t *>(&l);
                     }
-                    const uint32_t c = side * (D / 8) + i, at = to + (c / 8) * 16384 + (((c & 7) ^ (row & 7)) << 4);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + HALF), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
+                    // 16-byte piece c of a row lies at piece c ^ (row % 8)
+                    const uint32_t to = q0 + half * 2 * HALF + (column / 64) * 16384 + rr * 128 + (((column % 64 / 8) ^ (rr & 7)) << 4) + 2 * (column % 8);
+                    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to), "r"(hi[0]), "r"(hi[1]) : "memory");
+                    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + HALF), "r"(lo[0]), "r"(lo[1]) : "memory");
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) pg_arrive(b_q + 8 * half);
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            pc_sync_half(half);
+            float acc[D];
+            const float f = S.x[half][0][row];   // a score's unit, in those of log2
+            __syncwarp();
+            if (lane == 0) pg_arrive(b_q + 8 * half);
 #pragma unroll
             for (int i = 0; i < (int)D; i++) acc[i] = 0.f;
             float m = -INFINITY, l = 0.f, alpha = 1.f;
@@ -362,33 +368,39 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                 }
             }
             if (finish) {   // (the same for all of the half)
+                // through q's place in shared memory, from which warps store whole rows; column c of row r lies at c ^ (r % 32)
+                float *rows = reinterpret_cast<float *>(smem + half * 2 * HALF);
                 const float inv = l == 0.f ? 0.f : 1.f / l;
-                const bool there = w.tile * shape.tokens + tt < w.q.n && tt < shape.tokens;
-                const uint64_t q_row = w.q.start + w.tile * shape.tokens + tt, column = (uint64_t)(w.group * a.kv_mul + r % a.kv_mul) * HS;
-                float *out = a.out + q_row * a.out_stride + column;
                 bool odd = false;
 #pragma unroll
                 for (int i = 0; i < (int)D; i++) {
-                    acc[i] *= inv;
-                    odd |= !isfinite(acc[i]);
+                    const float y = acc[i] * inv;
+                    odd |= !isfinite(y);
+                    rows[row * HS + ((D * side + i) ^ (row & 31))] = y;
                 }
-                if (there) {
-                    if (a.vec)
-#pragma unroll
-                        for (int i = 0; i < (int)D; i += 4) *reinterpret_cast<float4 *>(out + D * side + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
-                    else
-#pragma unroll
-                        for (int i = 0; i < (int)D; i++) out[D * side + i] = acc[i];
-                }
-                const uint32_t mine = __ballot_sync(0xffffffffu, odd && there && isfinite(l));
+                const uint32_t mine = __ballot_sync(0xffffffffu, odd && isfinite(l));
                 if (lane == 0) S.odd[half][side][warp & 3] = mine;
                 pc_sync_half(half);
-                const float *q = a.q + q_row * a.q_stride + column;
-                for (uint32_t who = (mine | S.odd[half][side ^ 1][warp & 3]) & (side ? 0xFFFF0000u : 0xFFFFu); who; who &= who - 1) {   // (the two warps of the rows share them)
-                    const int b = __ffs(who) - 1;
-                    __syncwarp();
-                    paged_repair<__half>(a, PC_KT, w.request, w.group, w.span, __shfl_sync(0xffffffffu, p, b), __shfl_sync(0xffffffffu, m, b),
-                                         reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, (unsigned long long)q, b)), reinterpret_cast<float *>(__shfl_sync(0xffffffffu, (unsigned long long)out, b)), HS);
+#pragma unroll 1
+                for (uint32_t i = 0; i < 16; i++) {
+                    const uint32_t rr = 16 * (warp & 7) + i, at = 128 * half + rr, token = at / a.kv_mul;
+                    if (token >= shape.tokens || w.tile * shape.tokens + token >= w.q.n) break;   // (so are the rows behind it)
+                    float *out = a.out + (uint64_t)(w.q.start + w.tile * shape.tokens + token) * a.out_stride + (uint64_t)(w.group * a.kv_mul + at % a.kv_mul) * HS;
+#pragma unroll
+                    for (uint32_t c = lane; c < HS; c += 32) out[c] = rows[rr * HS + (c ^ (rr & 31))];
+                }
+                uint32_t any = 0;
+                for (uint32_t i = 0; i < 8; i++) any |= S.odd[half][i >> 2][i & 3];
+                if (any) {
+                    pc_sync_half(half);   // (the rows are stored)
+                    for (uint32_t who = (mine | S.odd[half][side ^ 1][warp & 3]) & (side ? 0xFFFF0000u : 0xFFFFu); who; who &= who - 1) {   // (the two warps of the rows share them)
+                        const int b = __ffs(who) - 1;
+                        const uint32_t at = 128 * half + 32 * (warp & 3) + b, token = at / a.kv_mul;
+                        if (token >= shape.tokens || w.tile * shape.tokens + token >= w.q.n) break;
+                        const uint64_t q_row = w.q.start + w.tile * shape.tokens + token, from = (uint64_t)(w.group * a.kv_mul + at % a.kv_mul) * HS;
+                        paged_repair<__half>(a, PC_KT, w.request, w.group, w.span, __shfl_sync(0xffffffffu, p, b), __shfl_sync(0xffffffffu, m, b), a.q + q_row * a.q_stride + from,
+                                             a.out + q_row * a.out_stride + from, HS);
+                    }
                 }
             }
             pc_sync_half(half);   // (what is shared may be written again)
