@@ -58,7 +58,8 @@ extern "C" int32_t ib_paged_attention(ib_ctx *ctx, void *stream, const ib_paged_
     a.k = cache->k_dev; a.v = cache->v_dev; a.page_stride = cache->page_stride;
     a.n_requests = p.n_requests; a.n_tokens = p.n_tokens; a.max_pages = p.max_pages; a.n_pages = cache->n_pages; a.page_log2 = log2_of(cache->page_size);
     a.kv_heads = p.n_heads / p.kv_mul; a.kv_mul = p.kv_mul; a.kv_dim = cache->kv_dim;
-    a.window = p.window; a.sinks = p.sinks;
+    a.window = p.window < (1u << 31) ? (int32_t)p.window : 0;   // (positions are below 2^31: a longer window is none)
+    a.sinks = p.sinks < (1u << 31) ? (int32_t)p.sinks : 0x7FFFFFFF;
     a.vec = (uintptr_t)p.q_dev % 16 == 0 && (uintptr_t)p.out_dev % 16 == 0 && p.q_stride % 4 == 0 && p.out_stride % 4 == 0;
     a.err = ctx->err_dev; a.wait_ns = ctx->wait_limit_ns;
     // Requests with few rows go through tiles of 8, the others through tiles of 256.  The host knows no lengths: where requests of either kind can be there, both kernels are launched, each for

@@ -26,7 +26,7 @@ struct PagedAttn {
     uint64_t page_stride;
     uint32_t n_requests, n_tokens, max_pages, n_pages, page_log2;
     uint32_t kv_heads, kv_mul, kv_dim;
-    uint32_t window, sinks;
+    int32_t window, sinks;         // 0: no window
     uint32_t rows_from, rows_to;   // the launch takes the requests with that many rows (new tokens * kv_mul)
     uint32_t least_units;          // units of a CTA's range, at least
     uint32_t vec;                  // q and out are on 16-byte boundaries
@@ -60,16 +60,14 @@ struct TileShape { uint32_t heads, groups, tokens; };
 struct KeySpan { uint32_t sink_tiles, first, units, end; };   // end: positions before it are seen by some row
 template <uint32_t KT>
 __device__ __forceinline__ KeySpan key_span(const PagedAttn &a, const PagedRequest &q, uint32_t tokens, uint32_t j) {
-    const long long lo = (long long)q.p0 + (long long)j * tokens, hi = (long long)q.p0 + min((j + 1) * tokens, q.n);   // positions of the tile's tokens: lo .. hi - 1
+    const int32_t lo = q.p0 + (int32_t)(j * tokens), hi = q.p0 + (int32_t)min((j + 1) * tokens, q.n);   // positions of the tile's tokens: lo .. hi - 1
     KeySpan s = {0, 0, 1, hi > 0 ? (uint32_t)hi : 0u};
     const uint32_t tiles = (s.end + KT - 1) / KT;
-    if (a.window) {
-        const long long from = lo - (long long)a.window + 1;
-        if (from > 0) {
-            s.first = (uint32_t)from / KT;
-            s.sink_tiles = (uint32_t)((min((long long)a.sinks, from) + KT - 1) / KT);
-            if (s.sink_tiles >= s.first) s.first = s.sink_tiles = 0;
-        }
+    if (a.window && lo >= a.window) {
+        const int32_t from = lo - a.window + 1;
+        s.first = (uint32_t)from / KT;
+        s.sink_tiles = ((uint32_t)min(a.sinks, from) + KT - 1) / KT;
+        if (s.sink_tiles >= s.first) s.first = s.sink_tiles = 0;
     }
     const uint32_t n = s.sink_tiles + tiles - s.first;
     if (n > 1) s.units = n;
@@ -101,27 +99,39 @@ __device__ __forceinline__ unsigned long long request_units(const PagedAttn &a, 
 }
 
 // ---- a CTA's range ----
+// Ranges of equal length, the last one shorter.  (Written without divisions where it can be: this is the code that a launch begins with, and code that runs once costs 12 clocks an instruction.)
 struct PagedRange {
-    unsigned long long total, offset;   // units of the launch; the range's first unit, counted inside its request
+    unsigned long long total, length, offset;   // units of the launch, of a range; the range's first unit, counted inside its request
     uint32_t ranges, request;
-    __device__ __forceinline__ unsigned long long first_unit(uint32_t c) const { return (unsigned long long)c * total / ranges; }
-    __device__ __forceinline__ uint32_t range_of(unsigned long long unit) const { return (uint32_t)(((unit + 1) * ranges - 1) / total); }
+    __device__ __forceinline__ unsigned long long first_unit(uint32_t c) const { return min(c * length, total); }
+    __device__ __forceinline__ uint32_t range_of(unsigned long long unit) const { return (uint32_t)(unit / length); }
 };
-struct PagedRangeShared { unsigned long long sum[33], offset; uint32_t owner, request; };
+struct PagedRangeShared { unsigned long long sum[32], offset; uint32_t owner, request; };
 
-// Called by a whole CTA of THREADS threads (every thread a stretch of the requests); ends with a barrier.  total == 0: nothing to do in this launch.
+// Called by a whole CTA of THREADS threads; ends with a barrier.  total == 0: nothing to do in this launch.
 template <uint32_t KT, uint32_t THREADS>
 __device__ __forceinline__ PagedRange paged_range(const PagedAttn &a, const TileShape &shape, PagedRangeShared &sh) {
     constexpr uint32_t WARPS = THREADS / 32;
     static_assert(WARPS <= 32, "one sum per warp");
-    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per = (a.n_requests + THREADS - 1) / THREADS, head_groups = a.kv_heads * shape.groups;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, head_groups = a.kv_heads * shape.groups;
+    // Few requests: a warp each, whose lanes share the request's tiles.  Otherwise every thread has a stretch of them.
+    const bool by_warp = a.n_requests <= WARPS;
+    const uint32_t per = by_warp ? 1 : (a.n_requests + THREADS - 1) / THREADS;
     auto units_of = [&](uint32_t r) {
         PagedRequest q = {0, 0, 0};
         if (r < a.n_requests) q = paged_request(a, r);
         return request_units<KT>(a, q, shape.tokens) * head_groups;
     };
     unsigned long long mine = 0;
-    for (uint32_t b = 0; b < per; b++) mine += units_of(tid * per + b);
+    if (by_warp) {
+        if (warp < a.n_requests) {
+            const PagedRequest q = paged_request(a, warp);
+            const uint32_t tiles = (q.n + shape.tokens - 1) / shape.tokens;
+            for (uint32_t j = lane; j < tiles; j += 32) mine += key_span<KT>(a, q, shape.tokens, j).units;
+            mine *= head_groups;
+        }
+    } else
+        for (uint32_t b = 0; b < per; b++) mine += units_of(tid * per + b);
     unsigned long long upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -130,20 +140,34 @@ __device__ __forceinline__ PagedRange paged_range(const PagedAttn &a, const Tile
     }
     if (lane == 31) sh.sum[warp] = upto;
     __syncthreads();
-    unsigned long long ahead = 0, total = 0;
-    for (uint32_t w = 0; w < WARPS; w++) {
-        if (w < warp) ahead += sh.sum[w];
-        total += sh.sum[w];
+    // every warp: the sums of all warps
+    unsigned long long sums = lane < WARPS ? sh.sum[lane] : 0ull;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long t = __shfl_up_sync(0xffffffffu, sums, o);
+        if (lane >= (uint32_t)o) sums += t;
     }
-    PagedRange g = {total, 0, 0, 0};
-    if (total == 0) return g;
-    const unsigned long long most = (total + a.least_units - 1) / a.least_units;
-    g.ranges = most < gridDim.x ? (uint32_t)most : gridDim.x;
-    const unsigned long long first = g.first_unit(blockIdx.x), before = ahead + upto - mine;
-    if (blockIdx.x < g.ranges && first >= before && first < before + mine) {
-        sh.owner = tid;
-        sh.offset = first - before;
-        sh.request = tid;
+    PagedRange g = {__shfl_sync(0xffffffffu, sums, 31), 1, 0, 0, 0};
+    if (g.total == 0) return g;
+    g.length = (g.total + gridDim.x - 1) / gridDim.x;
+    if (g.length < a.least_units) g.length = a.least_units;
+    g.ranges = (uint32_t)((g.total + g.length - 1) / g.length);
+    const unsigned long long first = g.first_unit(blockIdx.x);
+    unsigned long long before = __shfl_sync(0xffffffffu, sums, warp ? warp - 1 : 0);
+    if (warp == 0) before = 0;
+    if (by_warp) {
+        const unsigned long long all = __shfl_sync(0xffffffffu, upto, 31);
+        if (lane == 0 && first >= before && first < before + all) {
+            sh.offset = first - before;
+            sh.request = warp;
+        }
+    } else {
+        before += upto - mine;
+        if (first >= before && first < before + mine) {
+            sh.owner = tid;
+            sh.offset = first - before;
+            sh.request = tid;
+        }
     }
     __syncthreads();
     if (per > 1) {   // which of the owner's requests
@@ -255,8 +279,8 @@ struct PagedWalk {
 // The place of CTA c's partial of the tile that starts at unit `tile_unit`
 __device__ __forceinline__ uint32_t paged_place(const PagedRange &g, unsigned long long tile_unit, uint32_t c) { return 2 * c + (g.first_unit(c) < tile_unit ? 1u : 0u); }
 
-__device__ __forceinline__ bool paged_sees(const PagedAttn &a, long long p, long long j) {
-    return j >= 0 && j <= p && (a.window == 0 || p - j < (long long)a.window || j < (long long)a.sinks);
+__device__ __forceinline__ bool paged_sees(const PagedAttn &a, int32_t p, uint32_t j) {   // (j: a position, below 2^31)
+    return (int32_t)j <= p && (a.window == 0 || p - (int32_t)j < a.window || (int32_t)j < a.sinks);
 }
 
 __device__ __forceinline__ float paged_ex2(float x) {
@@ -276,7 +300,7 @@ __device__ __forceinline__ int paged_exponent(float most) {
 // the row's largest score (rounded up, in units of log2) known - unless its sum of weights is none either: then it sees a key, or is a query, that is none, and all of the row is rightly
 // so.  Called by a whole warp.
 template <typename T>
-static __device__ __noinline__ void paged_repair(const PagedAttn &a, uint32_t KT, uint32_t request, uint32_t kv_head, const KeySpan span, long long p, float most, const float *q, float *out, uint32_t hs) {
+static __device__ __noinline__ void paged_repair(const PagedAttn &a, uint32_t KT, uint32_t request, uint32_t kv_head, const KeySpan span, int32_t p, float most, const float *q, float *out, uint32_t hs) {
     const uint32_t lane = threadIdx.x & 31, E = hs / 32;
     const float scale = 1.4426950408889634f / sqrtf((float)hs);
     float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};

@@ -164,6 +164,9 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
         __syncwarp();
     };
     auto unpark = [&]() { w = *const_cast<const PagedWalk<PC_KT> *>(&kept); };
+    // row r of a tile is token r / kv_mul of it (r < 256, kv_mul <= 64: exact)
+    const uint32_t inverse = (65535 + a.kv_mul) / a.kv_mul;
+    auto token_of = [&](uint32_t r) { return r * inverse >> 16; };
     auto rows_of = [&]() { return min(shape.tokens, w.q.n - w.tile * shape.tokens) * a.kv_mul; };
 
     if (warp < PC_W_MMA) {
@@ -183,27 +186,26 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
         uint32_t ps = 0;   // parity of the scores; that of the products before them is the other one
         do {
             if (half == 1 && rows_of() <= 128) continue;
-            const uint32_t r = 128 * half + row, tt = r / a.kv_mul;
-            const int32_t p = w.q.p0 + (int32_t)(w.tile * shape.tokens + tt);
+            const int32_t p = w.q.p0 + (int32_t)(w.tile * shape.tokens + token_of(128 * half + row));
             if (side == 0 && (warp & 3) == 0) {   // (read behind the exchanges)
                 park();
                 if (lane == 0) {
-                    S.lo[half] = w.q.p0 + (int32_t)(w.tile * shape.tokens + 128 * half / a.kv_mul);
+                    S.lo[half] = w.q.p0 + (int32_t)(w.tile * shape.tokens + token_of(128 * half));
                     S.hi[half] = w.q.p0 + (int32_t)min((w.tile + 1) * shape.tokens, w.q.n) - 1;
                 }
             }
             // q: a warp takes rows as they lie in memory (a thread with a row of its own would touch 32 lines with every load), 16 of the half's
-            constexpr uint32_t LANES = HS / 4, AT_ONCE = 32 / LANES, LOADS = 4;   // lanes of a row, rows of a load, loads in flight
+            constexpr uint32_t LANES = HS / 4, AT_ONCE = 32 / LANES, LOADS = 8;   // lanes of a row, rows of a load, loads in flight
             const uint32_t column = 4 * (lane % LANES);
 #pragma unroll 1
             for (uint32_t i = 0; i < 16; i += LOADS * AT_ONCE) {
                 float4 v[LOADS];
 #pragma unroll
                 for (uint32_t k = 0; k < LOADS; k++) {
-                    const uint32_t rr = 16 * (warp & 7) + i + k * AT_ONCE + lane / LANES, at = 128 * half + rr, token = at / a.kv_mul;
+                    const uint32_t rr = 16 * (warp & 7) + i + k * AT_ONCE + lane / LANES, at = 128 * half + rr, token = token_of(at);
                     v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (token < shape.tokens && w.tile * shape.tokens + token < w.q.n) {
-                        const float *q = a.q + (uint64_t)(w.q.start + w.tile * shape.tokens + token) * a.q_stride + (uint64_t)(w.group * a.kv_mul + at % a.kv_mul) * HS + column;
+                        const float *q = a.q + (uint64_t)(w.q.start + w.tile * shape.tokens + token) * a.q_stride + (uint64_t)(w.group * a.kv_mul + at - token * a.kv_mul) * HS + column;
                         if (a.vec) v[k] = *reinterpret_cast<const float4 *>(q);
                         else v[k] = make_float4(q[0], q[1], q[2], q[3]);
                     }
@@ -261,14 +263,20 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                 if (i) fold();   // of the tile before: its products are done before this one's scores
                 const uint32_t unit = now.at + i, sink_tiles = now.span.sink_tiles;
                 const int32_t base = (int32_t)((unit < sink_tiles ? unit : now.span.first + unit - sink_tiles) * PC_KT + 64 * side);
-                const bool masked = base + 63 > *const_cast<volatile int32_t *>(&S.lo[half]) || (a.window && (int64_t)base + a.window <= *const_cast<volatile int32_t *>(&S.hi[half]));
+                const bool masked = base + 63 > *const_cast<volatile int32_t *>(&S.lo[half]) || (a.window && *const_cast<volatile int32_t *>(&S.hi[half]) - base >= a.window);
                 if (!ok || !wait(bs, ps, 12)) break;
                 ps ^= 1;
                 pg_fence_after();
-                // which of its 64 columns the row sees: up to `last`, and of those from `from` on or ahead of `sinks`
-                const int32_t last = p - base;
-                const int32_t from = a.window ? (int32_t)max((int64_t)p - a.window + 1 - base, (int64_t)-1) : -1, sinks = (int32_t)min((int64_t)a.sinks - base, (int64_t)64);
-                auto sees = [&](int32_t c) { return c <= last && (c >= from || c < sinks); };
+                uint64_t seen = ~0ull;   // which of its 64 columns the row sees: up to its own position, and of those the window's and the sinks
+                if (masked) {
+                    const int32_t last = p - base;
+                    if (a.window) {
+                        const int32_t from = last - a.window + 1, sinks = a.sinks - base;
+                        seen = (from <= 0 ? ~0ull : (from > 63 ? 0ull : ~0ull << from)) | (sinks <= 0 ? 0ull : (sinks > 63 ? ~0ull : ~(~0ull << sinks)));
+                    }
+                    seen &= last < 0 ? 0ull : (last > 62 ? ~0ull : ~(~0ull << (last + 1)));
+                }
+                auto sees = [&](int c) { return ((c < 32 ? (uint32_t)seen : (uint32_t)(seen >> 32)) & (1u << (c & 31))) != 0; };
                 // A load from tensor memory takes 200 clocks and more whatever its size (while products run), so it is of as many columns as there are registers for; those that are looked at
                 // last for the maximum are the first to become weights.
                 constexpr int ST = HS == 128 ? 16 : 32, NC = 64 / ST;   // (HS 128, in pieces of 32: 474 us instead of 464; HS 64, of 16: 165 instead of 155)
@@ -381,11 +389,11 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                 const uint32_t mine = __ballot_sync(0xffffffffu, odd && isfinite(l));
                 if (lane == 0) S.odd[half][side][warp & 3] = mine;
                 pc_sync_half(half);
-#pragma unroll 1
+#pragma unroll 4
                 for (uint32_t i = 0; i < 16; i++) {
-                    const uint32_t rr = 16 * (warp & 7) + i, at = 128 * half + rr, token = at / a.kv_mul;
+                    const uint32_t rr = 16 * (warp & 7) + i, at = 128 * half + rr, token = token_of(at);
                     if (token >= shape.tokens || w.tile * shape.tokens + token >= w.q.n) break;   // (so are the rows behind it)
-                    float *out = a.out + (uint64_t)(w.q.start + w.tile * shape.tokens + token) * a.out_stride + (uint64_t)(w.group * a.kv_mul + at % a.kv_mul) * HS;
+                    float *out = a.out + (uint64_t)(w.q.start + w.tile * shape.tokens + token) * a.out_stride + (uint64_t)(w.group * a.kv_mul + at - token * a.kv_mul) * HS;
 #pragma unroll
                     for (uint32_t c = lane; c < HS; c += 32) out[c] = rows[rr * HS + (c ^ (rr & 31))];
                 }
@@ -395,9 +403,9 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                     pc_sync_half(half);   // (the rows are stored)
                     for (uint32_t who = (mine | S.odd[half][side ^ 1][warp & 3]) & (side ? 0xFFFF0000u : 0xFFFFu); who; who &= who - 1) {   // (the two warps of the rows share them)
                         const int b = __ffs(who) - 1;
-                        const uint32_t at = 128 * half + 32 * (warp & 3) + b, token = at / a.kv_mul;
+                        const uint32_t at = 128 * half + 32 * (warp & 3) + b, token = token_of(at);
                         if (token >= shape.tokens || w.tile * shape.tokens + token >= w.q.n) break;
-                        const uint64_t q_row = w.q.start + w.tile * shape.tokens + token, from = (uint64_t)(w.group * a.kv_mul + at % a.kv_mul) * HS;
+                        const uint64_t q_row = w.q.start + w.tile * shape.tokens + token, from = (uint64_t)(w.group * a.kv_mul + at - token * a.kv_mul) * HS;
                         paged_repair<__half>(a, PC_KT, w.request, w.group, w.span, __shfl_sync(0xffffffffu, p, b), __shfl_sync(0xffffffffu, m, b), a.q + q_row * a.q_stride + from,
                                              a.out + q_row * a.out_stride + from, HS);
                     }

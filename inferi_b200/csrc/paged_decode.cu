@@ -172,12 +172,12 @@ __global__ void __launch_bounds__(PD_THREADS, pd_ctas_per_sm(sizeof(T))) paged_d
                 x[i][0] = d[0] + d[2];
                 x[i][1] = d[1] + d[3];
             }
-            if ((int64_t)j0 + NP - 1 > p_lo || (a.window && (int64_t)j0 + a.window <= p_hi)) {   // not every row sees all of these positions
+            if ((int32_t)j0 + NP - 1 > p_lo || (a.window && p_hi - (int32_t)j0 >= a.window)) {   // not every row sees all of these positions
 #pragma unroll
                 for (int i = 0; i < NP / 8; i++)
 #pragma unroll
                     for (int e = 0; e < 2; e++)
-                        if (!paged_sees(a, p, (long long)j0 + 8 * i + 2 * c + e)) x[i][e] = -INFINITY;
+                        if (!paged_sees(a, p, j0 + 8 * i + 2 * c + e)) x[i][e] = -INFINITY;
                 if (j0 + NP > end) {   // what nobody sees may be anything
 #pragma unroll
                     for (int i = 0; i < NP / 4; i++)
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(PD_THREADS, pd_ctas_per_sm(sizeof(T))) paged_d
                     const uint32_t r = 2 * warp + h, ft = r / shape.heads, fg = r % shape.heads;
                     const uint64_t fr = w.q.start + t0 + ft;
                     __syncwarp();
-                    paged_repair<T>(a, PD_KT, w.request, kv_head, w.span, (long long)p_lo + ft, __shfl_sync(0xffffffffu, mx, 16 * h), a.q + fr * a.q_stride + (uint64_t)(head0 + fg) * HS,
+                    paged_repair<T>(a, PD_KT, w.request, kv_head, w.span, p_lo + (int32_t)ft, __shfl_sync(0xffffffffu, mx, 16 * h), a.q + fr * a.q_stride + (uint64_t)(head0 + fg) * HS,
                                     a.out + fr * a.out_stride + (uint64_t)(head0 + fg) * HS, HS);
                 }
         }
