@@ -24,6 +24,10 @@ struct Entry {
     decltype(&ib_attention) attention;
     decltype(&ib_argmax) argmax;
     decltype(&ib_sample) sample;
+    decltype(&ib_page_plan) page_plan;
+    decltype(&ib_paged_append) paged_append;
+    decltype(&ib_paged_attention) paged_attention;
+    decltype(&ib_sample_batch) sample_batch;
 } lib;
 constexpr Py_ssize_t ENTRIES = sizeof(Entry) / sizeof(void *);
 
@@ -53,10 +57,10 @@ uint32_t u32(PyObject *o) {
     return static_cast<uint32_t>(v);
 }
 
-// The call on the current device's current stream, without the interpreter's lock (a launch waits where the stream's queue is full)
+// The call on the current device's current stream (`device`: on that one's), without the interpreter's lock (a launch waits where the stream's queue is full)
 template <class F>
-long on_stream(F &&f) {
-    void *s = c10::cuda::getCurrentCUDAStream().stream();
+long on_stream(F &&f, int64_t device = -1) {
+    void *s = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream();
     long rc;
     Py_BEGIN_ALLOW_THREADS rc = f(s);
     Py_END_ALLOW_THREADS return rc;
@@ -175,6 +179,145 @@ long sample(PyObject *const *a) {   // ctx, logits, vocabulary, temperature, top
     return on_stream([&](void *s) { return lib.sample(ctx, s, px, n, temperature, topp, coin, po); });
 }
 
+// ---- a batch of requests over a paged cache: tensors on the context's device, 32-bit integers, rows with a stride ----
+struct OnDevice {
+    int64_t device;
+    bool ok = true;
+    const at::Tensor *any(PyObject *o) {
+        const at::Tensor *t = THPVariable_CheckExact(o) ? &THPVariable_Unpack(o) : nullptr;
+        if (!t || !t->is_cuda() || t->device().index() != device) { ok = false; return nullptr; }
+        return t;
+    }
+    int32_t *ints(PyObject *o, int64_t numel = -1) {
+        const at::Tensor *t = any(o);
+        if (!t || t->scalar_type() != at::kInt || !t->is_contiguous() || (numel >= 0 && t->numel() != numel)) { ok = false; return nullptr; }
+        return static_cast<int32_t *>(t->data_ptr());
+    }
+    float *floats(PyObject *o, int64_t numel) {
+        const at::Tensor *t = any(o);
+        if (!t || t->scalar_type() != at::kFloat || !t->is_contiguous() || t->numel() != numel) { ok = false; return nullptr; }
+        return at_f32(t);
+    }
+    float *rows(PyObject *o, uint64_t &stride, int64_t n = -1, int64_t dim = -1) {
+        const at::Tensor *t = any(o);
+        if (!t || t->scalar_type() != at::kFloat || t->dim() != 2 || (t->size(1) > 1 && t->stride(1) != 1) || (n >= 0 && t->size(0) != n) || (dim >= 0 && t->size(1) != dim)) {
+            ok = false;
+            return nullptr;
+        }
+        stride = static_cast<uint64_t>(t->size(0) > 1 ? t->stride(0) : t->size(1));
+        return at_f32(t);
+    }
+    ib_paged_cache cache(PyObject *ko, PyObject *vo) {
+        ib_paged_cache c = {};
+        const at::Tensor *k = any(ko), *v = any(vo);
+        if (!ok) return c;
+        const bool f16 = k->scalar_type() == at::kHalf;
+        if (k->scalar_type() != v->scalar_type() || (!f16 && k->scalar_type() != at::kFloat) || k->dim() != 3 || k->sizes() != v->sizes() || k->strides() != v->strides() || k->stride(2) != 1 ||
+            k->stride(1) != k->size(2) || k->size(0) > 0xFFFFFFFFll || k->size(1) > 0xFFFFFFFFll || k->size(2) > 0xFFFFFFFFll) {
+            ok = false;
+            return c;
+        }
+        c.k_dev = k->data_ptr();
+        c.v_dev = v->data_ptr();
+        c.page_stride = static_cast<uint64_t>(k->size(0) > 1 ? k->stride(0) : k->size(1) * k->size(2));
+        c.n_pages = static_cast<uint32_t>(k->size(0));
+        c.page_size = static_cast<uint32_t>(k->size(1));
+        c.kv_dim = static_cast<uint32_t>(k->size(2));
+        c.kv_dtype = f16 ? IB_KV_F16 : IB_KV_F32;
+        return c;
+    }
+};
+constexpr int64_t LARGEST = 0xFFFFFFFFll;
+
+long page_plan(PyObject *const *a) {   // ctx, device, page size, cached, new, table, free pages, n_free, kv_len, row_start, positions, slots, n_free_out, status
+    ib_ctx *ctx = handle<ib_ctx>(a[0]);
+    OnDevice d{PyLong_AsLongLong(a[1])};
+    const at::Tensor *cached = d.any(a[3]), *table = d.any(a[5]), *free = d.any(a[6]), *slots = d.any(a[11]);
+    if (!ctx || !d.ok || table->dim() != 2) return NOT_TAKEN;
+    const int64_t n = cached->numel();
+    if (table->size(0) != n || n > LARGEST || table->size(1) > LARGEST || slots->numel() > LARGEST || free->numel() > LARGEST) return NOT_TAKEN;
+    ib_page_plan_args p = {static_cast<uint32_t>(n), static_cast<uint32_t>(table->size(1)), static_cast<uint32_t>(slots->numel()), static_cast<uint32_t>(free->numel()), u32(a[2]),
+                           d.ints(a[3]), d.ints(a[4], n), d.ints(a[7], 1), d.ints(a[5]), d.ints(a[6]), d.ints(a[8], n), d.ints(a[9], n + 1), d.ints(a[10], slots->numel()), d.ints(a[11]), d.ints(a[12], 1),
+                           d.ints(a[13], n)};
+    if (!d.ok || PyErr_Occurred()) return NOT_TAKEN;
+    return on_stream([&](void *s) { return lib.page_plan(ctx, s, &p); }, d.device);
+}
+
+long paged_append(PyObject *const *a) {   // ctx, device, variant, head size, base, q, k, v, positions, slots, q_out, key cache, value cache
+    ib_ctx *ctx = handle<ib_ctx>(a[0]);
+    OnDevice d{PyLong_AsLongLong(a[1])};
+    const ib_paged_cache c = d.cache(a[11], a[12]);
+    const at::Tensor *q = d.any(a[5]);
+    if (!ctx || !d.ok || q->dim() != 2) return NOT_TAKEN;
+    const int64_t n = q->size(0), dim = q->size(1);
+    if (n > LARGEST || dim > LARGEST) return NOT_TAKEN;
+    ib_paged_append_args p = {};
+    p.q_dev = d.rows(a[5], p.q_stride);
+    p.k_dev = d.rows(a[6], p.k_stride, n, c.kv_dim);
+    p.v_dev = d.rows(a[7], p.v_stride, n, c.kv_dim);
+    p.q_out_dev = d.rows(a[10], p.q_out_stride, n, dim);
+    p.positions = d.ints(a[8], n);
+    p.slots = d.ints(a[9], n);
+    p.n = static_cast<uint32_t>(n);
+    p.q_dim = static_cast<uint32_t>(dim);
+    p.head_size = u32(a[3]);
+    const long variant = PyLong_AsLong(a[2]);
+    p.variant = static_cast<int32_t>(variant);
+    p.base_freq = f32(a[4]);
+    if (!d.ok || variant < 0 || variant > 0x7FFFFFFF || PyErr_Occurred()) return NOT_TAKEN;
+    return on_stream([&](void *s) { return lib.paged_append(ctx, s, &p, &c); }, d.device);
+}
+
+long paged_attention(PyObject *const *a) {   // ctx, device, heads, kv_mul, head size, window, sinks, longest_new, q, key cache, value cache, table, row_start, kv_len, out
+    ib_ctx *ctx = handle<ib_ctx>(a[0]);
+    OnDevice d{PyLong_AsLongLong(a[1])};
+    const ib_paged_cache c = d.cache(a[9], a[10]);
+    const at::Tensor *q = d.any(a[8]), *table = d.any(a[11]), *kv_len = d.any(a[13]);
+    if (!ctx || !d.ok || q->dim() != 2 || table->dim() != 2) return NOT_TAKEN;
+    const int64_t n = kv_len->numel(), tokens = q->size(0);
+    ib_paged_attn_args p = {};
+    p.n_heads = u32(a[2]);
+    p.kv_mul = u32(a[3]);
+    p.head_size = u32(a[4]);
+    p.window = u32(a[5]);
+    p.sinks = u32(a[6]);
+    p.longest_new = u32(a[7]);
+    const int64_t dim = static_cast<int64_t>(static_cast<uint64_t>(p.n_heads) * p.head_size);
+    if (dim < 0 || table->size(0) != n || n > LARGEST || tokens > LARGEST || table->size(1) > LARGEST) return NOT_TAKEN;
+    p.q_dev = d.rows(a[8], p.q_stride, tokens, dim);
+    p.out_dev = d.rows(a[14], p.out_stride, tokens, dim);
+    p.block_table = d.ints(a[11]);
+    p.row_start = d.ints(a[12], n + 1);
+    p.kv_len = d.ints(a[13]);
+    p.n_requests = static_cast<uint32_t>(n);
+    p.n_tokens = static_cast<uint32_t>(tokens);
+    p.max_pages = static_cast<uint32_t>(table->size(1));
+    if (!d.ok || PyErr_Occurred()) return NOT_TAKEN;
+    return on_stream([&](void *s) { return lib.paged_attention(ctx, s, &p, &c); }, d.device);
+}
+
+long sample_batch(PyObject *const *a) {   // ctx, device, vocabulary, logits, temperature, top_k, top_p, min_p, coin, token, prob (top_k .. min_p, prob: or None)
+    ib_ctx *ctx = handle<ib_ctx>(a[0]);
+    OnDevice d{PyLong_AsLongLong(a[1])};
+    const at::Tensor *x = d.any(a[3]);
+    const uint32_t vocab = u32(a[2]);
+    if (!ctx || !d.ok || x->dim() != 2 || x->size(0) > LARGEST) return NOT_TAKEN;
+    const int64_t n = x->size(0);
+    ib_sample_batch_args p = {};
+    p.logits_dev = d.rows(a[3], p.stride, n, vocab);
+    p.rows = static_cast<uint32_t>(n);
+    p.vocab = vocab;
+    p.temperature = d.floats(a[4], n);
+    if (a[5] != Py_None) p.top_k = d.ints(a[5], n);
+    if (a[6] != Py_None) p.top_p = d.floats(a[6], n);
+    if (a[7] != Py_None) p.min_p = d.floats(a[7], n);
+    p.coin = d.floats(a[8], n);
+    p.token = d.ints(a[9], n);
+    if (a[10] != Py_None) p.prob = d.floats(a[10], n);
+    if (!d.ok || PyErr_Occurred()) return NOT_TAKEN;
+    return on_stream([&](void *s) { return lib.sample_batch(ctx, s, &p); }, d.device);
+}
+
 // The library's entry points, in the order of `Entry`, from whoever loaded it
 PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (n != ENTRIES) {
@@ -205,6 +348,10 @@ PyMethodDef methods[] = {
     method<attention, 6>("attention"),
     method<argmax, 3>("argmax"),
     method<sample, 7>("sample"),
+    method<page_plan, 14>("page_plan"),
+    method<paged_append, 13>("paged_append"),
+    method<paged_attention, 15>("paged_attention"),
+    method<sample_batch, 11>("sample_batch"),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -42,7 +42,7 @@ def _f32_dev(t: torch.Tensor, name: str) -> int:
 # with -1 where it has not launched anything: for arguments that it does not know (tensor subclasses), and for those that are refused.  The Python
 # way then does the call or raises the error, and does all of them where there is no binding, or one of another torch.
 class _NoBinding:
-    gemv = gemm = rms_norm = rope = silu = add = attention = argmax = sample = staticmethod(lambda *a: -1)
+    gemv = gemm = rms_norm = rope = silu = add = attention = argmax = sample = page_plan = paged_append = paged_attention = sample_batch = staticmethod(lambda *a: -1)
     bind = staticmethod(lambda *a: None)
 
 
@@ -55,7 +55,8 @@ def _load_binding():
 
 
 _fast = _load_binding()
-_BOUND = ("ib_gemv_quant", "ib_gemm_quant", "ib_rms_norm", "ib_rope", "ib_silu_mul", "ib_add_assign", "ib_attention", "ib_argmax", "ib_sample")
+_BOUND = ("ib_gemv_quant", "ib_gemm_quant", "ib_rms_norm", "ib_rope", "ib_silu_mul", "ib_add_assign", "ib_attention", "ib_argmax", "ib_sample", "ib_page_plan",
+          "ib_paged_append", "ib_paged_attention", "ib_sample_batch")
 
 
 # The Python ways take their tensors' addresses first: with a CUDA tensor among them CUDA is initialised, and the stream can be
@@ -370,6 +371,13 @@ class Sampler:
 PLAN_OK, PLAN_NO_PAGES, PLAN_TABLE_FULL, PLAN_NO_ROOM, PLAN_INVALID = range(5)   # what PagePlan says of a request
 
 
+def _stream_of(backend: Backend) -> int:
+    """The current stream of the context's device, which need not be the current one."""
+    if not torch.cuda.is_initialized():
+        return torch.cuda.current_stream(backend.device).cuda_stream
+    return _raw_stream(backend.device)
+
+
 def _on_device(backend: Backend, *named) -> None:
     for name, t in named:
         if not isinstance(t, _tensor) or not t.is_cuda or t.device.index != backend.device:
@@ -416,6 +424,11 @@ class PagePlan:
                row_start: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, n_free_out: torch.Tensor, status: torch.Tensor) -> None:
         """int32 CUDA tensors: lengths and status [n], block_table [n, max_pages], free_pages [pages of the cache], row_start [n + 1], positions and slots [room for
         tokens], n_free and n_free_out [1].  kv_len may be cached_len and n_free_out n_free."""
+        rc = _fast.page_plan(self.backend._address, self.backend.device, page_size, cached_len, new_len, block_table, free_pages, n_free, kv_len, row_start, positions, slots, n_free_out, status)
+        if rc == 0:
+            return
+        if rc > 0:
+            check(rc)
         b, n = self.backend, cached_len.numel()
         _on_device(b, ("cached_len", cached_len), ("new_len", new_len), ("block_table", block_table), ("free_pages", free_pages), ("n_free", n_free), ("kv_len", kv_len), ("row_start", row_start),
                    ("positions", positions), ("slots", slots), ("n_free_out", n_free_out), ("status", status))
@@ -424,7 +437,7 @@ class PagePlan:
         a = PagePlanArgs(n, block_table.shape[1], _u32(slots.numel(), "slots"), _u32(free_pages.numel(), "free_pages"), _u32(page_size, "page_size"), _i32_dev(cached_len, "cached_len"), _i32_dev(new_len, "new_len", n), _i32_dev(n_free, "n_free", 1),
                          _i32_dev(block_table, "block_table"), _i32_dev(free_pages, "free_pages"), _i32_dev(kv_len, "kv_len", n), _i32_dev(row_start, "row_start", n + 1),
                          _i32_dev(positions, "positions", slots.numel()), _i32_dev(slots, "slots"), _i32_dev(n_free_out, "n_free_out", 1), _i32_dev(status, "status", n))
-        check(b.lib.ib_page_plan(b.handle, _stream_ptr(), C.byref(a)))
+        check(b.lib.ib_page_plan(b.handle, _stream_of(b), C.byref(a)))
 
 
 @dataclass
@@ -446,13 +459,18 @@ class PagedAppend:
                key_cache: torch.Tensor, value_cache: torch.Tensor) -> None:
         """q, q_out: [n, q_dim], k, v: [n, kv_dim] float32 with contiguous rows (q_out may be q); caches [pages, page_size, kv_dim] float16 or float32; positions and
         slots [n] int32.  Rows with slots outside the cache are left out."""
+        rc = _fast.paged_append(self.backend._address, self.backend.device, variant, config.head_size, config.base_freq, q, k, v, positions, slots, q_out, key_cache, value_cache)
+        if rc == 0:
+            return
+        if rc > 0:
+            check(rc)
         b = self.backend
         _on_device(b, ("q", q), ("k", k), ("v", v), ("positions", positions), ("slots", slots), ("q_out", q_out), ("key_cache", key_cache), ("value_cache", value_cache))
         c = _paged_cache(key_cache, value_cache)
         (pq, sq), (n, q_dim) = _f32_rows(q, "q"), q.shape
         (pk, sk), (pv, sv), (po, so) = _f32_rows(k, "k", n, c.kv_dim), _f32_rows(v, "v", n, c.kv_dim), _f32_rows(q_out, "q_out", n, q_dim)
         a = PagedAppendArgs(pq, pk, pv, po, sq, sk, sv, so, _i32_dev(positions, "positions", n), _i32_dev(slots, "slots", n), _u32(n, "rows"), _u32(q_dim, "q_dim"), _u32(config.head_size, "head_size"), variant, config.base_freq)
-        check(b.lib.ib_paged_append(b.handle, _stream_ptr(), C.byref(a), C.byref(c)))
+        check(b.lib.ib_paged_append(b.handle, _stream_of(b), C.byref(a), C.byref(c)))
 
 
 @dataclass
@@ -479,6 +497,12 @@ class PagedAttention:
                out: torch.Tensor) -> None:
         """q, out: [rows, n_heads * head_size] float32 with contiguous rows; caches [pages, page_size, kv_dim] float16 or float32; block_table [n, max_pages], row_start
         [n + 1], kv_len [n] int32.  Rows behind row_start[n] stay as they are."""
+        rc = _fast.paged_attention(self.backend._address, self.backend.device, config.n_heads, config.kv_mul, config.head_size, config.window, config.sinks, config.longest_new, q, key_cache,
+                                   value_cache, block_table, row_start, kv_len, out)
+        if rc == 0:
+            return
+        if rc > 0:
+            check(rc)
         b, n = self.backend, kv_len.numel()
         _on_device(b, ("q", q), ("key_cache", key_cache), ("value_cache", value_cache), ("block_table", block_table), ("row_start", row_start), ("kv_len", kv_len), ("out", out))
         c = _paged_cache(key_cache, value_cache)
@@ -489,7 +513,7 @@ class PagedAttention:
         counts = [_u32(getattr(config, f), f) for f in ("n_heads", "kv_mul", "head_size", "window", "sinks", "longest_new")]
         a = PagedAttnArgs(pq, po, sq, so, _i32_dev(block_table, "block_table"), _i32_dev(row_start, "row_start", n + 1), _i32_dev(kv_len, "kv_len"), n, _u32(q.shape[0], "rows"),
                           block_table.shape[1], *counts)
-        check(b.lib.ib_paged_attention(b.handle, _stream_ptr(), C.byref(a), C.byref(c)))
+        check(b.lib.ib_paged_attention(b.handle, _stream_of(b), C.byref(a), C.byref(c)))
 
 
 class BatchSampler:
@@ -504,6 +528,11 @@ class BatchSampler:
         if None) and, if given, prob [n] float32 are written; returns token."""
         b, n = self.backend, logits.shape[0]
         token = token if token is not None else torch.empty(n, dtype=torch.int32, device=logits.device)
+        rc = _fast.sample_batch(self.backend._address, self.backend.device, self.vocab_size, logits, temperature, top_k, top_p, min_p, coin, token, prob)
+        if rc == 0:
+            return token
+        if rc > 0:
+            check(rc)
         given = [(name, t) for name, t in (("logits", logits), ("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p), ("coin", coin), ("token", token), ("prob", prob))
                  if t is not None]
         _on_device(b, *given)
@@ -518,5 +547,5 @@ class BatchSampler:
 
         a = SampleBatchArgs(x, stride, _u32(n, "rows"), self.vocab_size, f32(temperature, "temperature"), _i32_dev(top_k, "top_k", n) if top_k is not None else None, f32(top_p, "top_p"),
                             f32(min_p, "min_p"), f32(coin, "coin"), _i32_dev(token, "token", n), f32(prob, "prob"))
-        check(b.lib.ib_sample_batch(b.handle, _stream_ptr(), C.byref(a)))
+        check(b.lib.ib_sample_batch(b.handle, _stream_of(b), C.byref(a)))
         return token
