@@ -7,14 +7,18 @@
 //
 // Which token it is hangs on sums of up to half a million weights next to a border, and on a flat distribution the border is 1e-5 of the sum away.  So weights are whole numbers, in units
 // of 2^-44 of the largest, good to 3e-10 of themselves: (x - max) log2(e) / T is one product of doubles, added to 1.5 * 2^20 so that its whole and fractional parts
-// are words of the result; 2^fraction is a table of 256 and three steps of a series in 32-bit fixed point.  Sums of whole numbers do not depend on their order.
+// are words of the result; 2^fraction is a table of 256 and three steps of a series in 32-bit fixed point.  Sums of whole numbers do not depend on their order.  Weights below the histogram
+// (below) only matter as a sum, mostly: there ex2.approx of a product with a two-word constant will do, whose errors of 1e-6 are each its own and vanish in the sum of thousands (1e-9 of
+// the total); where a border turns out to lie among them, the sums are formed anew from whole numbers (BS_EXACT).
 //
-// A row is a thread-block cluster of up to 8 CTAs, each with a slice of the row in shared memory: one read of the row from HBM, and what follows passes over shared memory.
+// A row is a thread-block cluster of up to 8 CTAs, each with a slice of the row in shared memory: one read of the row from HBM, and what follows passes over shared memory.  A warp goes over its
+// stretch of the slice once, adds up the small weights and lists the places of the others, which it takes together then (a few per cent of a language model's logits: with some of them
+// among the 32 lanes of every step, all of it ran at the price of the large ones).
 // Nothing is sorted but a list of at most 1024 elements: every border asks for the element at which a running count or sum in sorted order crosses a bound, and a histogram
-// (count and weight over 1024 equal stretches of x, those of the largest 11 factors of two) says which bin that is; its elements - or, where they fit, all up to
+// (count and weight over 1024 equal stretches of x, those of the largest 16 factors of two) says which bin that is; its elements - or, where they fit, all up to
 // there, so that one list answers every question - are listed and sorted.  Bins too full for the list (ties) or below the histogram: the same by digits of x's order, to the last
-// tie in index order.  The first CTA of the cluster leads: it looks at the merged histogram and says what all do next (Step).
-// What bounds it: a batch of many rows, the 25 instructions a token; few rows, the cluster's barriers.
+// tie in index order.  The first CTA of the cluster leads: it looks at the merged histogram and says what all do next (BsStep).  Its threads carry the same state and search sums by
+// bisection, each for itself, without barriers.
 #include "op_launch.cuh"
 
 #include <cooperative_groups.h>
@@ -29,9 +33,12 @@ constexpr uint32_t BS_THREADS = 512, BS_WARPS = BS_THREADS / 32, BS_CLUSTER = 8;
 constexpr uint32_t BS_BINS = 1024, BS_LIST = 1024;
 constexpr uint32_t BS_MAX_VOCAB = 1u << 19;   // S < 2^63
 constexpr int BS_ONE = 44;                    // the largest weight is 2^44 units
-constexpr double BS_OCTAVES = 11.0;           // the histogram's reach below the largest weight, at most
-// Vocabularies up to this size are one CTA's work
+// The histogram's reach below the largest weight, at most, in factors of two.  A border below it is looked for in a second one, of the stretch behind the first.
+constexpr double BS_OCTAVES = 16.0, BS_OCTAVES_K = 11.0;
+constexpr uint32_t BS_WINDOWS = 4;                  // such stretches, at most
+// Vocabularies up to this size are one CTA's work, up to twice this size two CTAs' and so on
 constexpr uint32_t BS_ONE_CTA = 4096;
+constexpr uint32_t BS_HOT = 32;               // places that a thread keeps
 constexpr uint32_t BS_SMEM_LIMIT = 227 * 1024;
 
 struct BatchSampleParams {
@@ -44,17 +51,34 @@ struct BatchSampleParams {
     float *prob;
 };
 
-enum BsStep : uint32_t { BS_DONE, BS_HISTOGRAM, BS_DIGIT, BS_LIST_BINS, BS_LIST_DIGITS, BS_SEGMENT, BS_COUNT_TIES, BS_PICK_TIE };
+// 2^(i / 256) with 31 fractional bits
+struct BsTable { uint32_t t[256]; };
+constexpr BsTable bs_make_table() {
+    BsTable r = {};
+    double x = 2147483648.0;
+    for (int i = 0; i < 256; i++) {
+        r.t[i] = (uint32_t)(x + 0.5);
+        x *= 1.0027112750502025;   // 2^(1 / 256)
+    }
+    return r;
+}
+__device__ const BsTable bs_table = bs_make_table();
+
+enum BsStep : uint32_t { BS_DONE, BS_HISTOGRAM, BS_EXACT, BS_DIGIT, BS_LIST_BINS, BS_LIST_DIGITS, BS_SEGMENT, BS_COUNT_TIES, BS_PICK_TIE };
 
 struct BsShared {
     uint32_t table[256];                                // 2^(i / 256), 31 fractional bits
     uint32_t cnt[BS_BINS];                              // this CTA's histogram: elements ...
-    uint2 mass[BS_BINS];                                // ... and their weight, as two words
+    union {
+        uint2 mass[BS_BINS];                            // ... and their weight, as two words; in the first CTA, when a list is there,
+        unsigned long long run[BS_LIST];                // the running weight through each of its elements
+    };
     unsigned long long tot_mass[BS_BINS];               // first CTA: the cluster's histogram, then the sums ahead of each bin
     uint32_t tot_cnt[BS_BINS];
-    unsigned long long list[BS_LIST], run[BS_LIST];     // first CTA: listed elements, (~order of x, index); running weight through each
+    unsigned long long list[BS_LIST];                   // listed elements, (~order of x, index)
     unsigned long long seg[BS_CLUSTER * BS_WARPS];      // first CTA: weight or count of every warp's stretch of the row
     unsigned long long red[2][BS_WARPS];
+    uint16_t hot[BS_WARPS][BS_HOT][32];                 // places in the slice of the elements that may be in the histogram, by threads
     float lo[BS_CLUSTER];                               // of every CTA's slice: its smallest finite logit
     unsigned long long best[BS_CLUSTER];                // ... and its arg-max
     unsigned long long part_mass[BS_CLUSTER], part_min[BS_CLUSTER];   // first CTA: weight of each slice, of its elements with w >= min_p
@@ -63,9 +87,9 @@ struct BsShared {
     uint32_t step, a, b, prefix;
     unsigned long long arg;
     uint32_t listed;
-    // first CTA: the whole histogram's sums; scratch of its searches
+    // first CTA: the whole histogram's sums
     unsigned long long all_mass;
-    uint32_t all_cnt, at;
+    uint32_t all_cnt;
 };
 
 // the order of x as a number: larger x, larger number
@@ -75,7 +99,14 @@ __device__ __forceinline__ uint32_t bs_order(float x) {
 }
 __device__ __forceinline__ float bs_value(uint32_t order) { return __uint_as_float(order & 0x80000000u ? order & 0x7FFFFFFFu : ~order); }
 // what is no number is never drawn; an infinity is the largest number
-__device__ __forceinline__ float bs_clean(float x) { return x != x ? -INFINITY : fminf(x, FLT_MAX); }
+__device__ __forceinline__ float bs_clean(float x) { return x > -INFINITY ? fminf(x, FLT_MAX) : -INFINITY; }
+
+// Sum over a warp of numbers below 2^44: the halves in the reduction unit
+__device__ __forceinline__ unsigned long long bs_sum(unsigned long long w) {
+    return (unsigned long long)__reduce_add_sync(0xffffffffu, (uint32_t)w & 0x3FFFFFu) + ((unsigned long long)__reduce_add_sync(0xffffffffu, (uint32_t)(w >> 22)) << 22);
+}
+
+static_assert(BS_MAX_VOCAB / BS_CLUSTER <= 65536, "places are 16 bits");
 
 struct BsWeight {
     float hi;
@@ -118,17 +149,32 @@ __device__ __forceinline__ void bs_scan(unsigned long long &a, unsigned long lon
     __syncthreads();
 }
 
-// Ascending sort of list[0 .. cap), cap a power of two
+// Ascending sort of list[0 .. cap), cap a power of two: exchanges over fewer than 32 places are shuffles
 __device__ __forceinline__ void bs_sort(unsigned long long *list, uint32_t cap) {
-    for (uint32_t k = 2; k <= cap; k <<= 1)
-        for (uint32_t j = k >> 1; j > 0; j >>= 1) {
-            for (uint32_t t = threadIdx.x; t < cap / 2; t += BS_THREADS) {
+    const uint32_t tid = threadIdx.x;
+    auto in_warps = [&](uint32_t k, uint32_t from) {
+        for (uint32_t t = tid; t - (tid & 31) < cap; t += BS_THREADS) {
+            unsigned long long v = t < cap ? list[t] : ~0ull;
+            for (uint32_t j = from; j > 0; j >>= 1) {
+                const unsigned long long o = __shfl_xor_sync(0xffffffffu, v, j);
+                const bool keep_min = ((t & k) == 0) == ((t & j) == 0);
+                v = keep_min ? (v < o ? v : o) : (v < o ? o : v);
+            }
+            if (t < cap) list[t] = v;
+        }
+        __syncthreads();
+    };
+    for (uint32_t k = 2; k <= cap; k <<= 1) {
+        for (uint32_t j = k >> 1; j >= 32; j >>= 1) {
+            for (uint32_t t = tid; t < cap / 2; t += BS_THREADS) {
                 const uint32_t a = ((t & ~(j - 1)) << 1) | (t & (j - 1)), b = a | j;
                 const unsigned long long x = list[a], y = list[b];
                 if ((x > y) == ((a & k) == 0)) { list[a] = y; list[b] = x; }
             }
             __syncthreads();
         }
+        in_warps(k, k < 64 ? k >> 1 : 16);
+    }
 }
 
 __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __grid_constant__ BatchSampleParams p) {
@@ -141,7 +187,7 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
     const uint32_t i0 = min(p.n, rank * p.slice), len = min(p.n, i0 + p.slice) - i0;
     const float *from = p.logits + row * p.stride + i0;
     float *held = reinterpret_cast<float *>(smem + sizeof(BsShared));
-    if (tid < 256) S.table[tid] = (uint32_t)__double2uint_rn(exp2((double)tid * (1.0 / 256)) * 2147483648.0);
+    if (tid < 256) S.table[tid] = bs_table.t[tid];
     pdl_enter();
 
     const float T = p.temperature[row];
@@ -151,23 +197,39 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
     const bool by_k = k > 0 && (uint32_t)k < p.n, by_p = top_p > 0.f && top_p < 1.f, by_min = min_p > 0.f, filtered = by_k || by_p || by_min;
 
     // the slice, its largest logit (lowest index on ties) and its smallest finite one
-    unsigned long long best = 0ull;
-    float lo = INFINITY;
-    constexpr uint32_t AT_ONCE = 8;
-    for (uint32_t base = tid; base < len; base += AT_ONCE * BS_THREADS) {
+    float top = -INFINITY, lo = INFINITY;
+    uint32_t top_at = i0 + tid;   // (a thread's first element, if it has one)
+    constexpr uint32_t AT_ONCE = 16;
+    auto look = [&](uint32_t i, float y) {
+        const float x = bs_clean(y);
+        const bool more = x > top;
+        top = more ? x : top;
+        top_at = more ? i0 + i : top_at;
+        if (x > -INFINITY) lo = fminf(lo, x);
+    };
+    uint32_t done = 0;
+    for (; done + AT_ONCE * BS_THREADS <= len; done += AT_ONCE * BS_THREADS) {   // (without a check for every element)
+        const float *y = from + done + tid;
         float v[AT_ONCE];
 #pragma unroll
-        for (uint32_t e = 0; e < AT_ONCE; e++) v[e] = base + e * BS_THREADS < len ? __ldg(from + base + e * BS_THREADS) : 0.f;
+        for (uint32_t e = 0; e < AT_ONCE; e++) v[e] = __ldg(y + e * BS_THREADS);
 #pragma unroll
         for (uint32_t e = 0; e < AT_ONCE; e++) {
-            const uint32_t i = base + e * BS_THREADS;
-            if (i >= len) continue;
-            const float x = bs_clean(v[e]);
-            if (p.resident) held[i] = x;
-            best = max(best, (unsigned long long)bs_order(x) << 32 | (0xFFFFFFFFu - (i0 + i)));
-            if (x > -INFINITY) lo = fminf(lo, x);
+            if (p.resident) held[done + tid + e * BS_THREADS] = v[e];
+            look(done + tid + e * BS_THREADS, v[e]);
         }
     }
+    {
+        float v[AT_ONCE];
+#pragma unroll
+        for (uint32_t e = 0; e < AT_ONCE; e++) v[e] = done + tid + e * BS_THREADS < len ? __ldg(from + done + tid + e * BS_THREADS) : -INFINITY;
+#pragma unroll
+        for (uint32_t e = 0; e < AT_ONCE; e++) {
+            if (p.resident && done + tid + e * BS_THREADS < len) held[done + tid + e * BS_THREADS] = v[e];
+            look(done + tid + e * BS_THREADS, v[e]);
+        }
+    }
+    unsigned long long best = tid >= len ? 0ull : (unsigned long long)bs_order(top) << 32 | (0xFFFFFFFFu - top_at);
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
@@ -202,37 +264,41 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
         return;   // nobody reads another CTA's memory from here on
     }
     const BsWeight weight = {hi, 1.4426950408889634074 / (double)T};
-    auto logit = [&](uint32_t i) { return p.resident ? held[i] : bs_clean(__ldg(from + i)); };
+    const float *here = p.resident ? held : from;   // (as they came)
+    auto logit = [&](uint32_t i) { return bs_clean(here[i]); };
+    // `body` for `many` elements of a warp, number k at place(k) of the slice; the loads of eight steps are in flight together (a slice that is not held comes from L2)
+    auto sweep = [&](uint32_t many, auto place, auto body) {
+        constexpr uint32_t K = 8;
+        for (uint32_t k = lane; k - lane < many; k += 32 * K) {
+            uint32_t at[K];
+            float x[K];
+#pragma unroll
+            for (uint32_t e = 0; e < K; e++) {
+                at[e] = k + 32 * e < many ? place(k + 32 * e) : 0u;
+                x[e] = k + 32 * e < many ? logit(at[e]) : -INFINITY;
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < K; e++) body(at[e], x[e]);   // (-infinity behind the last one)
+        }
+    };
     // a warp's elements: a stretch of the slice
     const uint32_t stretch = ((len + BS_WARPS - 1) / BS_WARPS + 31) & ~31u, w0 = min(len, warp * stretch), w1 = min(len, w0 + stretch);
 
     // ---- what a step does ----
     // bins of x: equal stretches down from the largest logit
-    const float reach = (float)fmin(BS_OCTAVES / weight.c, (double)hi - (double)lo), per_bin = reach > 0.f && isfinite(reach) ? (float)BS_BINS * (1.f - 0x1p-20f) / reach : 0.f;
-    auto bin_of = [&](float x) {   // >= BS_BINS: below the histogram
+    // (a limit by rank mostly ends far above one by mass, and one by min_p says itself where)
+    const double octaves = fmin(by_k ? BS_OCTAVES_K : BS_OCTAVES, by_min && !(by_k && by_p) ? 0.01 - log2((double)fmaxf(min_p, 1e-30f)) : BS_OCTAVES);
+    const float reach = (float)fmin(fmax(octaves, 0.01) / weight.c, (double)hi - (double)lo), per_bin = reach > 0.f && isfinite(reach) ? (float)BS_BINS * (1.f - 0x1p-20f) / reach : 0.f;
+    uint32_t window = 0;           // of the row's stretches of that length
+    auto bin_of = [&](float x) {   // >= BS_BINS: not in this window
         const float d = (hi - x) * per_bin;
-        return d < (float)BS_BINS ? (uint32_t)d : BS_BINS;
+        const uint32_t u = (d < (float)(BS_BINS * BS_WINDOWS) ? (uint32_t)d : BS_BINS * BS_WINDOWS) - BS_BINS * window;
+        return u < BS_BINS ? u : BS_BINS;
     };
     auto add = [&](uint32_t bin, unsigned long long w) {
         atomicAdd(&S.cnt[bin], 1u);
         const uint32_t l = (uint32_t)w, old = atomicAdd(&S.mass[bin].x, l), h = (uint32_t)(w >> 32) + ((uint32_t)(old + l) < old ? 1u : 0u);
         if (h) atomicAdd(&S.mass[bin].y, h);
-    };
-    // a warp's 32 elements; where all of them fall into one bin (a row of equal logits), one addition
-    auto add_warp = [&](uint32_t bin, unsigned long long w, bool in) {
-        const uint32_t who = __ballot_sync(0xffffffffu, in);
-        if (!who) return;
-        const uint32_t one = __shfl_sync(0xffffffffu, bin, __ffs(who) - 1);
-        if (__popc(who) > 8 && __all_sync(0xffffffffu, !in || bin == one)) {
-            unsigned long long sum = in ? w : 0ull;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (lane == 0) {
-                atomicAdd(&S.cnt[one], (uint32_t)__popc(who));
-                const uint32_t l = (uint32_t)sum, old = atomicAdd(&S.mass[one].x, l), h = (uint32_t)(sum >> 32) + ((uint32_t)(old + l) < old ? 1u : 0u);
-                if (h) atomicAdd(&S.mass[one].y, h);
-            }
-        } else if (in) add(bin, w);
     };
     auto clear = [&]() {
         for (uint32_t b = tid; b < BS_BINS; b += BS_THREADS) {
@@ -248,12 +314,14 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
         for (uint32_t b = rank * share + tid; b < min(BS_BINS, (rank + 1) * share); b += BS_THREADS) {
             unsigned long long m = 0ull;
             uint32_t n = 0u;
-            for (uint32_t r = 0; r < C; r++) {
-                const BsShared &o = *cluster.map_shared_rank(&S, r);
-                const uint2 x = o.mass[b];
-                m += ((unsigned long long)x.y << 32) + x.x;
-                n += o.cnt[b];
-            }
+#pragma unroll
+            for (uint32_t r = 0; r < BS_CLUSTER; r++)
+                if (r < C) {
+                    const BsShared &o = *cluster.map_shared_rank(&S, r);
+                    const uint2 x = o.mass[b];
+                    m += ((unsigned long long)x.y << 32) + x.x;
+                    n += o.cnt[b];
+                }
             L.tot_mass[b] = m;
             L.tot_cnt[b] = n;
         }
@@ -274,21 +342,67 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
     // ---- the weights: sums of every stretch and slice, and for filtered rows the histogram ----
     if (filtered) clear();
     const unsigned long long least = by_min ? (min_p > 1.f ? (1ull << BS_ONE) + 1 : (unsigned long long)ceil((double)min_p * (double)(1ull << BS_ONE))) : 0ull;
+    // elements that are looked at one by one: those of the histogram (and a little more), and what may reach min_p (a factor of two more: rounding)
+    const float near = fmaxf(per_bin > 0.f ? reach * (1.f + 0x1p-18f) : INFINITY, by_min ? (float)((1.0 - log2((double)fmaxf(min_p, 1e-30f))) / weight.c) : 0.f);
+    const float c_hi = (float)weight.c, c_lo = (float)(weight.c - (double)c_hi);
+    uint32_t n_hot = 0;       // the thread's places
+    bool all_listed = true;   // the warp's lists hold all of its elements of the histogram
     {
         unsigned long long sum = 0ull, above = 0ull;
         uint32_t n = 0u, n_above = 0u;
-        for (uint32_t i = w0 + lane; i - lane < w1; i += 32) {
-            const bool in = i < w1;
-            const float x = in ? logit(i) : -INFINITY;
-            const unsigned long long w = weight(x, S.table);
-            sum += w;
-            if (w) n++;
-            if (by_min && w >= least) { above += w; n_above++; }
-            if (filtered) {
-                const uint32_t bin = bin_of(x);
-                add_warp(bin, w, w != 0ull && bin < BS_BINS);
+        float small = 0.f;
+        auto take = [&]() {
+            constexpr uint32_t K = 4;   // a chain of some hundred clocks each: several at once
+            for (uint32_t k = 0; __any_sync(0xffffffffu, k < n_hot); k += K) {
+                unsigned long long w[K];
+                uint32_t bin[K];
+#pragma unroll
+                for (uint32_t e = 0; e < K; e++) {
+                    const float x = k + e < n_hot ? logit(S.hot[warp][k + e][lane]) : -INFINITY;
+                    w[e] = weight(x, S.table);
+                    bin[e] = w[e] ? bin_of(x) : BS_BINS;
+                }
+#pragma unroll
+                for (uint32_t e = 0; e < K; e++) {
+                    sum += w[e];
+                    if (by_min && w[e] >= least) { above += w[e]; n_above++; }
+                    if (filtered && bin[e] < BS_BINS) add(bin[e], w[e]);
+                }
             }
+        };
+        constexpr uint32_t U = 8;
+        auto some = [&](uint32_t i, const float (&x)[U]) {   // elements i + 32 e.  (What is no number is not above -infinity; an infinity is looked at one by one.)
+            if (__any_sync(0xffffffffu, n_hot > BS_HOT - U)) {
+                take();
+                n_hot = 0;
+                all_listed = false;
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < U; e++) {
+                const float d = x[e] - hi;
+                const bool any = x[e] > -INFINITY, far = d < -near;
+                float w;
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(fmaf(d, c_hi, d * c_lo)));
+                n += any;
+                if (any && far) small += fmaxf(w, 0x1p-44f);
+                if (any && !far) S.hot[warp][n_hot++][lane] = (uint16_t)(i + 32 * e);
+            }
+        };
+        uint32_t i = w0;
+        for (; i + 32 * U <= w1; i += 32 * U) {   // (without a check for every element)
+            float x[U];
+#pragma unroll
+            for (uint32_t e = 0; e < U; e++) x[e] = here[i + lane + 32 * e];
+            some(i + lane, x);
         }
+        if (i < w1) {
+            float x[U];
+#pragma unroll
+            for (uint32_t e = 0; e < U; e++) x[e] = i + lane + 32 * e < w1 ? here[i + lane + 32 * e] : -INFINITY;
+            some(i + lane, x);
+        }
+        take();
+        sum += (unsigned long long)((double)small * (double)(1ull << BS_ONE));
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
             sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -310,21 +424,23 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
             L.part_cnt[rank] = (uint32_t)(c >> 32);
         }
     }
-    if (filtered) merge(); else barrier();
 
     // ---- the first CTA leads ----
     // Every one of its threads carries the same state; the questions: 0 the k-th element, 1 top_p's, 2 the coin's.
-    unsigned long long total = 0ull, kept = 0ull, n_kept = 0ull, S_k = 0ull, bound = 0ull, base = 0ull, n_base = 0ull;
+    unsigned long long total = 0ull, kept = 0ull, n_kept = 0ull, S_k = 0ull, bound = 0ull, base = 0ull, n_base = 0ull, n_min = 0ull, S_min = 0ull, there = 0ull;
     uint32_t question = 0, list_lo = 1, list_hi = 0, list_n = 0, shift = 32, prefix = 0;   // the list: bins list_lo .. list_hi
-    bool histogram = true;   // tot_* are those of the bins of x
+    bool histogram = true, exact = false;   // tot_* are those of the bins of x; the sums are those of whole numbers
     unsigned long long list_mass = 0ull, list_cnt = 0ull;   // ahead of the list
-    if (rank == 0) {
-        for (uint32_t s = 0; s < C * BS_WARPS; s++) total += S.seg[s];
+    unsigned long long win_mass = 0ull, win_cnt = 0ull;     // ahead of the window
+    auto add_up = [&]() {
+        total = 0ull;
+        for (uint32_t s = lane; s < C * BS_WARPS; s += 32) total += S.seg[s];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
         kept = S_k = total;
         n_kept = p.n;
-    }
-    const unsigned long long n_min = rank == 0 && by_min ? [&]() { unsigned long long c = 0; for (uint32_t r = 0; r < C; r++) c += S.part_min_cnt[r]; return c; }() : 0ull;
-    const unsigned long long S_min = rank == 0 && by_min ? [&]() { unsigned long long m = 0; for (uint32_t r = 0; r < C; r++) m += S.part_min[r]; return m; }() : 0ull;
+        question = 0;
+    };
     auto scaled = [](float f, unsigned long long m) { return f > 0.f ? min((unsigned long long)((double)f * (double)m), m - 1) : 0ull; };   // f < 1
     auto say = [&](uint32_t step, uint32_t a, uint32_t b, uint32_t pre, unsigned long long arg) {
         if (tid == 0) { S.step = step; S.a = a; S.b = b; S.prefix = pre; S.arg = arg; }
@@ -333,13 +449,15 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
     auto ask = [&]() {
         for (;; question++) {
             if (question == 0 && by_k) {
-                unsigned long long there = 0;
-                for (uint32_t r = 0; r < C; r++) there += S.part_cnt[r];
-                if ((unsigned long long)k >= there) continue;   // all that have a weight
+                if ((unsigned long long)k >= there || (by_min && !by_p && n_min <= (unsigned long long)k)) continue;   // all that have a weight; min_p leaves no more
                 bound = (unsigned long long)k - 1;
                 return;
             }
-            if (question == 1 && by_p) { bound = scaled(top_p, S_k); return; }
+            if (question == 1 && by_p) {
+                bound = scaled(top_p, S_k);
+                if (by_min && n_min && bound >= S_min) continue;   // min_p leaves less
+                return;
+            }
             if (question == 2) {
                 if (by_min && n_min < n_kept) { n_kept = max(n_min, 1ull); kept = n_min ? S_min : 1ull << BS_ONE; }
                 bound = scaled(coin, kept);
@@ -362,39 +480,64 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
         return false;
     };
     auto by_count = [&]() { return question == 0; };
-    // the bin of the crossing in tot_* -> S.at (BS_BINS: none); ahead: weight or count ahead of the histogram
+    auto sum_upto = [&](uint32_t b) -> unsigned long long {
+        if (by_count()) return b + 1 < BS_BINS ? S.tot_cnt[b + 1] : S.all_cnt;
+        return b + 1 < BS_BINS ? S.tot_mass[b + 1] : S.all_mass;
+    };
+    // the bin of the crossing in tot_* (BS_BINS: none); ahead: weight or count ahead of the histogram
     auto find = [&](unsigned long long ahead) {
-        if (tid == 0) S.at = BS_BINS;
-        __syncthreads();
-        for (uint32_t b = tid; b < BS_BINS; b += BS_THREADS) {
-            const unsigned long long upto = b + 1 < BS_BINS ? (by_count() ? S.tot_cnt[b + 1] : S.tot_mass[b + 1]) : (by_count() ? S.all_cnt : S.all_mass);
-            const unsigned long long before = by_count() ? S.tot_cnt[b] : S.tot_mass[b];
-            if (bound >= ahead + before && bound < ahead + upto) S.at = b;
+        uint32_t lo = 0, hi = BS_BINS;   // the first bin whose sum exceeds the bound
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) >> 1;
+            if (bound < ahead + sum_upto(mid)) hi = mid; else lo = mid + 1;
         }
-        __syncthreads();
-        const uint32_t b = S.at;
-        __syncthreads();
-        return b;
+        return lo;
     };
     auto cnt_upto = [&](uint32_t b) { return b + 1 < BS_BINS ? S.tot_cnt[b + 1] : S.all_cnt; };
     // the crossing inside the sorted list, whose sums start behind list_mass, list_cnt
     auto from_list = [&]() {
-        if (tid == 0) S.at = list_n - 1;
-        __syncthreads();
-        if (by_count()) { if (tid == 0) S.at = (uint32_t)(bound - list_cnt); }
+        uint32_t lo = 0, hi = list_n - 1;
+        if (by_count()) lo = (uint32_t)(bound - list_cnt);
         else
-            for (uint32_t i = tid; i < list_n; i += BS_THREADS) {
-                const unsigned long long upto = list_mass + S.run[i], before = list_mass + (i ? S.run[i - 1] : 0ull);
-                if (bound >= before && bound < upto) S.at = i;
+            while (lo < hi) {
+                const uint32_t mid = (lo + hi) >> 1;
+                if (bound < list_mass + S.run[mid]) hi = mid; else lo = mid + 1;
             }
-        __syncthreads();
-        const uint32_t i = S.at;
-        __syncthreads();
-        return answered(S.list[i], list_mass + S.run[i], list_cnt + i + 1);
+        return answered(S.list[lo], list_mass + S.run[lo], list_cnt + lo + 1);
     };
     // Goes on until the cluster is needed; says what for.
+    uint32_t last = BS_HISTOGRAM;   // what the cluster has just done
     auto lead = [&]() {
-        for (;;) {
+        if (last == BS_DIGIT) {
+            const uint32_t bin = find(by_count() ? n_base : base), at = bin < BS_BINS ? bin : 0;   // (there is one: the elements' sums are the same)
+            const uint32_t n = cnt_upto(at) - S.tot_cnt[at], to = shift > 10 ? shift - 10 : 0;
+            base += S.tot_mass[at];
+            n_base += S.tot_cnt[at];
+            prefix = (shift == 32 ? 0u : prefix << (shift - to)) | at;
+            shift = to;
+            if (n <= BS_LIST) {
+                list_mass = base;
+                list_cnt = n_base;
+                say(BS_LIST_DIGITS, shift, 0, prefix, 0);
+            } else if (shift == 0) say(BS_COUNT_TIES, 0, 0, prefix, 0);
+            else say(BS_DIGIT, shift, shift > 10 ? shift - 10 : 0, prefix, 0);
+            return;
+        }
+        bool done = false;
+        if (last == BS_LIST_DIGITS) done = from_list();
+        if (last == BS_COUNT_TIES) {
+            const unsigned long long w = weight(bs_value(~prefix), S.table), th = by_count() ? bound - n_base : (bound - base) / w;   // number th of the equal ones
+            if (question == 2) {
+                unsigned long long left = th;
+                uint32_t s = 0;
+                while (s + 1 < C * BS_WARPS && left >= S.seg[s]) left -= S.seg[s++];
+                if (tid == 0 && p.prob) p.prob[row] = (float)((double)w / (double)kept);
+                say(BS_PICK_TIE, s, 0, prefix, left);
+                return;
+            }
+            answered(0ull, base + (th + 1) * w, n_base + th + 1);   // (which one it is does not matter to the sums)
+        }
+        while (!done) {
             ask();
             if (!filtered) {   // index order: the stretch of the crossing
                 unsigned long long ahead = 0ull;
@@ -403,34 +546,49 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
                 say(BS_SEGMENT, s, 0, 0, bound - ahead);
                 return;
             }
-            if (!histogram) { say(BS_HISTOGRAM, 0, 0, 0, 0); return; }
-            const uint32_t b = find(0ull);
+            const unsigned long long ahead = by_count() ? win_cnt : win_mass;
+            if (!histogram || bound < ahead) {
+                win_mass = win_cnt = 0ull;
+                list_lo = 1;
+                list_hi = 0;
+                say(BS_HISTOGRAM, 0, 0, 0, 0);
+                return;
+            }
+            const uint32_t b = find(ahead);
+            if (b == BS_BINS && window + 1 < BS_WINDOWS && (hi - lo) * per_bin >= (float)(BS_BINS * (window + 1))) {   // behind this window
+                win_mass += S.all_mass;
+                win_cnt += S.all_cnt;
+                list_lo = 1;
+                list_hi = 0;
+                say(BS_HISTOGRAM, window + 1, 0, 0, 0);
+                return;
+            }
             if (b < BS_BINS) {
                 if (b >= list_lo && b <= list_hi) {
-                    if (from_list()) { say(BS_DONE, 0, 0, 0, 0); return; }
+                    done = from_list();
                     continue;
                 }
                 const uint32_t first = cnt_upto(b) <= BS_LIST ? 0 : b;
                 if (cnt_upto(b) - S.tot_cnt[first] <= BS_LIST) {
                     list_lo = first;
                     list_hi = b;
-                    list_mass = S.tot_mass[first];
-                    list_cnt = S.tot_cnt[first];
-                    if (tid == 0) S.listed = 0;
+                    list_mass = win_mass + S.tot_mass[first];
+                    list_cnt = win_cnt + S.tot_cnt[first];
                     say(BS_LIST_BINS, first, b, 0, 0);
                     return;
                 }
             }
+            if (!exact) { say(BS_EXACT, 0, 0, 0, 0); return; }   // below the histogram, or a bin too full for the list
             // by digits of x's order
             shift = 32;
             prefix = 0;
             base = n_base = 0ull;
-            histogram = false;
             list_lo = 1;
             list_hi = 0;
             say(BS_DIGIT, 32, 22, 0, 0);
             return;
         }
+        say(BS_DONE, 0, 0, 0, 0);
     };
     auto sorted = [&]() {   // the first CTA's list has arrived
         list_n = min(S.listed, BS_LIST);
@@ -450,52 +608,53 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
         __syncthreads();
     };
 
-    if (rank == 0) lead();
-    for (;;) {
+    // (Every part of this stands here once: code that runs once costs 12 clocks an instruction, and a row comes through here a few times only.)
+    bool merging = filtered;
+#pragma unroll 1
+    for (bool first = true;; first = false) {
+        if (merging) merge();
+        else if (first || last == BS_EXACT || last == BS_COUNT_TIES) barrier();   // the stretches' sums are there
+        if (rank == 0) {
+            if (first || last == BS_EXACT) {
+                add_up();
+                exact = !first;
+            }
+            if (first)
+                for (uint32_t r = 0; r < C; r++) {
+                    n_min += S.part_min_cnt[r];
+                    S_min += S.part_min[r];
+                    there += S.part_cnt[r];
+                }
+            if (last == BS_LIST_BINS || last == BS_LIST_DIGITS) sorted();
+            lead();
+        }
         barrier();
         const uint32_t step = L.step, a = L.a, b = L.b, pre = L.prefix;
         const unsigned long long arg = L.arg;
+        last = step;
+        merging = step == BS_HISTOGRAM || step == BS_DIGIT;
         if (step == BS_DONE) break;
-        if (step == BS_HISTOGRAM) {
+        if (merging) {
+            // the histogram by stretches of x; or, of the elements whose order's bits from a on are `pre`, by their bits from b to a
             clear();
-            for (uint32_t i = w0 + lane; i - lane < w1; i += 32) {
-                const float x = i < w1 ? logit(i) : -INFINITY;
-                const uint32_t bin = bin_of(x);
-                add_warp(bin, weight(x, S.table), x > -INFINITY && bin < BS_BINS);
-            }
-            merge();
-            histogram = true;
-            if (rank == 0) lead();
-        } else if (step == BS_DIGIT) {   // elements whose order's bits from a on are `pre`: by their bits from b to a
-            clear();
-            for (uint32_t i = w0 + lane; i - lane < w1; i += 32) {
-                const float x = i < w1 ? logit(i) : -INFINITY;
+            histogram = step == BS_HISTOGRAM;
+            if (histogram) window = a;
+            sweep(w1 - w0, [&](uint32_t k) { return w0 + k; }, [&](uint32_t, float x) {
                 const uint32_t order = ~bs_order(x);   // (ascending: the largest x first)
-                add_warp((order >> b) & ((1u << (a - b)) - 1u), weight(x, S.table), x > -INFINITY && (a == 32 || order >> a == pre));
-            }
-            merge();
-            if (rank == 0) {
-                const unsigned long long ahead = by_count() ? n_base : base;
-                const uint32_t bin = find(ahead);   // (there is one: the elements' sums are the same)
-                const uint32_t at = bin < BS_BINS ? bin : 0;
-                const uint32_t n = cnt_upto(at) - S.tot_cnt[at];
-                base += S.tot_mass[at];
-                n_base += S.tot_cnt[at];
-                prefix = (shift == 32 ? 0u : prefix << (a - b)) | at;
-                shift = b;
-                if (n <= BS_LIST) {
-                    list_mass = base;
-                    list_cnt = n_base;
-                    if (tid == 0) S.listed = 0;
-                    __syncthreads();
-                    say(BS_LIST_DIGITS, shift, 0, prefix, 0);
-                } else if (shift == 0) say(BS_COUNT_TIES, 0, 0, prefix, 0);
-                else say(BS_DIGIT, shift, shift > 10 ? shift - 10 : 0, prefix, 0);
-                __syncthreads();
-            }
+                const uint32_t bin = histogram ? bin_of(x) : (order >> b) & ((1u << (a - b)) - 1u);
+                if (x > -INFINITY && (histogram ? bin < BS_BINS : a == 32 || order >> a == pre)) add(bin, weight(x, S.table));
+            });
+        } else if (step == BS_EXACT) {   // the stretches' sums from whole numbers; then all questions again
+            unsigned long long sum = 0ull;
+            sweep(w1 - w0, [&](uint32_t k) { return w0 + k; }, [&](uint32_t, float x) { sum += weight(x, S.table); });
+#pragma unroll
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane == 0) L.seg[rank * BS_WARPS + warp] = sum;
         } else if (step == BS_LIST_BINS || step == BS_LIST_DIGITS) {
-            for (uint32_t i = w0 + lane; i < w1; i += 32) {
-                const float x = logit(i);
+            // into this CTA's own list, a place for every warp's elements together; the first CTA fetches them from all
+            if (tid == 0) S.listed = 0;
+            __syncthreads();
+            auto list = [&](uint32_t i, float x) {
                 const uint32_t order = ~bs_order(x);
                 bool in = x > -INFINITY;
                 if (step == BS_LIST_BINS) {
@@ -503,46 +662,77 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
                     in = in && bin >= a && bin <= b;
                 } else in = in && (a == 32 || order >> a == pre);
                 if (in) {
-                    const uint32_t at = atomicAdd(&L.listed, 1u);
-                    if (at < BS_LIST) L.list[at] = (unsigned long long)order << 32 | (i0 + i);
+                    const uint32_t at = atomicAdd(&S.listed, 1u);
+                    if (at < BS_LIST) S.list[at] = (unsigned long long)order << 32 | (i0 + i);
                 }
-            }
+            };
+            if (step == BS_LIST_BINS && all_listed && window == 0)
+                for (uint32_t k = 0; k < n_hot; k++) list(S.hot[warp][k][lane], logit(S.hot[warp][k][lane]));
+            else sweep(w1 - w0, [&](uint32_t k) { return w0 + k; }, list);
             barrier();
-            if (rank == 0) {
-                sorted();
-                if (step == BS_LIST_BINS) lead();   // (finds its bin in the list now)
-                else if (from_list()) say(BS_DONE, 0, 0, 0, 0);
-                else lead();
+            if (rank == 0 && C > 1) {
+                uint32_t own = min(S.listed, BS_LIST);
+                for (uint32_t r = 1; r < C; r++) {
+                    const BsShared &o = *cluster.map_shared_rank(&S, r);
+                    const uint32_t n = min(o.listed, BS_LIST - own);
+                    for (uint32_t i = tid; i < n; i += BS_THREADS) S.list[own + i] = o.list[i];
+                    own += n;
+                }
+                __syncthreads();
+                if (tid == 0) S.listed = own;
                 __syncthreads();
             }
         } else if (step == BS_SEGMENT) {   // index order: the element of warp a's stretch at which the running weight exceeds arg
-            if (rank == a / BS_WARPS && warp == a % BS_WARPS) {
-                unsigned long long left = arg;
-                uint32_t last = 0xFFFFFFFFu;
-                unsigned long long last_w = 0ull;
-                for (uint32_t i = w0 + lane; i - lane < w1; i += 32) {
-                    const unsigned long long w = i < w1 ? weight(logit(i), S.table) : 0ull;
-                    unsigned long long run = w;
+            // The CTA's warps share that stretch; the one whose part the crossing is in goes through it element by element.
+            if (rank == a / BS_WARPS) {
+                const uint32_t o = a % BS_WARPS, s0 = min(len, o * stretch), s1 = min(len, s0 + stretch), part = ((s1 - s0 + BS_WARPS - 1) / BS_WARPS + 31) & ~31u;
+                const uint32_t p0 = min(s1, s0 + warp * part), p1 = min(s1, p0 + part);
+                unsigned long long sum = 0ull;
+                sweep(p1 - p0, [&](uint32_t k) { return p0 + k; }, [&](uint32_t, float x) { sum += weight(x, S.table); });
 #pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const unsigned long long t = __shfl_up_sync(0xffffffffu, run, o);
-                        if ((int)lane >= o) run += t;
-                    }
-                    const uint32_t hit = __ballot_sync(0xffffffffu, left < run);
-                    const uint32_t some = __ballot_sync(0xffffffffu, w != 0ull);
-                    if (hit || some) {
-                        const int l = hit ? __ffs(hit) - 1 : 31 - __clz(some);
-                        last = i0 + i - lane + l;
-                        last_w = __shfl_sync(0xffffffffu, w, l);
-                    }
-                    if (hit) break;
-                    left -= __shfl_sync(0xffffffffu, run, 31);
+                for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                if (lane == 0) S.red[0][warp] = sum;
+                __syncthreads();
+                uint32_t mine = BS_WARPS;   // the part of the crossing; (rounding of the small weights: perhaps none, then the last with a weight)
+                unsigned long long left = arg, ahead = 0ull;
+                for (uint32_t k = 0; k < BS_WARPS; k++) {
+                    const unsigned long long m = S.red[0][k];
+                    if (m && (mine == BS_WARPS || arg >= ahead)) { mine = k; left = arg - ahead; }
+                    ahead += m;
                 }
-                if (lane == 0) {
-                    p.token[row] = (int32_t)(last == 0xFFFFFFFFu ? 0u : last);
+                if (warp == mine || (mine == BS_WARPS && warp == 0)) {
+                    uint32_t at = i0 + s0;
+                    unsigned long long at_w = 0ull;
+                    bool found = false;
+                    sweep(p1 - p0, [&](uint32_t k) { return p0 + k; }, [&](uint32_t i, float x) {
+                        if (found) return;
+                        const unsigned long long w = weight(x, S.table), all = bs_sum(w);
+                        found = left < all;
+                        const uint32_t some = __ballot_sync(0xffffffffu, w != 0ull);
+                        if (found || some) {
+                            int l = 31 - __clz(some);
+                            if (found) {
+                                unsigned long long run = w;
+#pragma unroll
+                                for (int d = 1; d < 32; d <<= 1) {
+                                    const unsigned long long t = __shfl_up_sync(0xffffffffu, run, d);
+                                    if ((int)lane >= d) run += t;
+                                }
+                                l = __ffs(__ballot_sync(0xffffffffu, left < run)) - 1;
+                            }
+                            at = i0 + __shfl_sync(0xffffffffu, i, l);
+                            at_w = __shfl_sync(0xffffffffu, w, l);
+                        }
+                        left -= all;
+                    });
                     unsigned long long all = 0ull;
-                    for (uint32_t s = 0; s < C * BS_WARPS; s++) all += L.seg[s];
-                    if (p.prob) p.prob[row] = (float)((double)last_w / (double)all);
+                    for (uint32_t s = lane; s < C * BS_WARPS; s += 32) all += L.seg[s];
+#pragma unroll
+                    for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
+                    if (lane == 0) {
+                        p.token[row] = (int32_t)at;
+                        if (p.prob) p.prob[row] = (float)((double)at_w / (double)all);
+                    }
                 }
             }
             break;
@@ -551,21 +741,6 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
             for (uint32_t i = w0 + lane; i < w1; i += 32) n += ~bs_order(logit(i)) == pre;
             n = __reduce_add_sync(0xffffffffu, n);
             if (lane == 0) L.seg[rank * BS_WARPS + warp] = n;
-            barrier();
-            if (rank == 0) {
-                const unsigned long long w = weight(bs_value(~pre), S.table), th = by_count() ? bound - n_base : (bound - base) / w;   // number th of them
-                if (question == 2) {
-                    unsigned long long left = th;
-                    uint32_t s = 0;
-                    while (s + 1 < C * BS_WARPS && left >= S.seg[s]) left -= S.seg[s++];
-                    if (tid == 0 && p.prob) p.prob[row] = (float)((double)w / (double)kept);
-                    say(BS_PICK_TIE, s, 0, pre, left);
-                } else {   // (which one it is does not matter to the sums)
-                    answered(0ull, base + (th + 1) * w, n_base + th + 1);
-                    lead();
-                }
-                __syncthreads();
-            }
         } else {   // BS_PICK_TIE: number arg of warp a's stretch
             if (rank == a / BS_WARPS && warp == a % BS_WARPS) {
                 uint32_t left = (uint32_t)arg;
@@ -601,9 +776,13 @@ extern "C" int32_t ib_sample_batch(ib_ctx *ctx, void *stream, const ib_sample_ba
     p.logits = a.logits_dev; p.stride = a.stride; p.n = a.vocab;
     p.temperature = a.temperature; p.top_p = a.top_p; p.min_p = a.min_p; p.top_k = a.top_k; p.coin = a.coin;
     p.token = a.token; p.prob = a.prob;
-    const uint32_t ctas = a.vocab <= BS_ONE_CTA ? 1u : BS_CLUSTER;
+    // CTAs of a row: up to 8, while all rows' have a place at once (two on an SM); a slice has 65536 tokens at most
+    uint32_t ctas = BS_CLUSTER;
+    while (ctas > 1 && (a.vocab <= BS_ONE_CTA * ctas / 2 || ((uint64_t)a.rows * ctas > 2 * (uint64_t)ctx->sm_count && a.vocab <= 65536 * ctas / 2))) ctas /= 2;
     p.slice = (a.vocab + ctas - 1) / ctas;
-    p.resident = sizeof(BsShared) + p.slice * sizeof(float) <= BS_SMEM_LIMIT;
+    // held in shared memory where that costs no CTA its place
+    const size_t with = sizeof(BsShared) + p.slice * sizeof(float);
+    p.resident = with <= BS_SMEM_LIMIT && ((uint64_t)a.rows * ctas <= (uint64_t)ctx->sm_count || 2 * (with + 1024) <= BS_SMEM_LIMIT + 1024);
     static bool attr_set[16] = {false};
     const bool beyond = ctx->device >= 16;
     if (beyond || !attr_set[ctx->device]) {
