@@ -32,7 +32,7 @@ __device__ __forceinline__ void pd_mma_tf32(float (&d)[4], const uint32_t (&a)[4
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x = hi + lo: two f16 each of a pair; two tf32 (the MMA drops the remainder's bits beyond its 11)
+// x = hi + lo: two f16 each of a pair; two tf32
 __device__ __forceinline__ void pd_split(float x, float y, uint32_t &hi, uint32_t &lo) {
     const __half2 h = __floats2half2_rn(x, y);
     const float2 f = __half22float2(h);
@@ -42,7 +42,7 @@ __device__ __forceinline__ void pd_split(float x, float y, uint32_t &hi, uint32_
 }
 __device__ __forceinline__ void pd_split_tf32(float x, uint32_t &hi, uint32_t &lo) {
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-    lo = __float_as_uint(x - __uint_as_float(hi));
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));   // (the MMA would drop its lower bits, always towards zero)
 }
 __device__ __forceinline__ uint4 pd_load(const void *p) { return __ldcg(reinterpret_cast<const uint4 *>(p)); }
 __device__ __forceinline__ uint32_t pd_word(const uint4 &v, int i) { return i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w)); }
@@ -151,26 +151,32 @@ __global__ void __launch_bounds__(PD_THREADS, pd_ctas_per_sm(sizeof(T))) paged_d
             float x[NP / 8][2];
 #pragma unroll
             for (int i = 0; i < NP / 8; i++) {
-                float d[4] = {0.f, 0.f, 0.f, 0.f};
+                if constexpr (F16) {
+                    float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int s = 0; s < KP; s++) {
-                    if constexpr (F16) {
+                    for (int s = 0; s < KP; s++) {
                         pd_mma(d, qa[2 * s], kr[i][s].x, kr[i][s].y);
                         pd_mma(d, qa[2 * s + 1], kr[i][s].z, kr[i][s].w);
-                    } else {
+                    }
+                    x[i][0] = d[0] + d[2];
+                    x[i][1] = d[1] + d[3];
+                } else {
+                    // K's remainders have sums of their own, and its upper parts four: short chains drop less
+                    float d[5][4] = {};
+#pragma unroll
+                    for (int s = 0; s < KP; s++)
 #pragma unroll
                         for (int e = 0; e < 4; e += 2) {
                             const uint32_t qq[4] = {qa[4 * s + e][0], qa[4 * s + e][1], qa[4 * s + e + 1][0], qa[4 * s + e + 1][1]};
                             uint32_t h0, l0, h1, l1;
                             pd_split_tf32(__uint_as_float(pd_word(kr[i][s], e)), h0, l0);
                             pd_split_tf32(__uint_as_float(pd_word(kr[i][s], e + 1)), h1, l1);
-                            pd_mma_tf32(d, qq, h0, h1);
-                            pd_mma_tf32(d, qq, l0, l1);
+                            pd_mma_tf32(d[s & 3], qq, h0, h1);
+                            pd_mma_tf32(d[4], qq, l0, l1);
                         }
-                    }
+                    x[i][0] = ((d[0][0] + d[1][0]) + (d[2][0] + d[3][0])) + (((d[0][2] + d[1][2]) + (d[2][2] + d[3][2])) + (d[4][0] + d[4][2]));
+                    x[i][1] = ((d[0][1] + d[1][1]) + (d[2][1] + d[3][1])) + (((d[0][3] + d[1][3]) + (d[2][3] + d[3][3])) + (d[4][1] + d[4][3]));
                 }
-                x[i][0] = d[0] + d[2];
-                x[i][1] = d[1] + d[3];
             }
             if ((int32_t)j0 + NP - 1 > p_lo || (a.window && p_hi - (int32_t)j0 >= a.window)) {   // not every row sees all of these positions
 #pragma unroll
@@ -217,8 +223,8 @@ __global__ void __launch_bounds__(PD_THREADS, pd_ctas_per_sm(sizeof(T))) paged_d
                         uint32_t h0, l0, h1, l1;
                         pd_split_tf32(__uint_as_float(pd_word(vr[0][s], t)), h0, l0);
                         pd_split_tf32(__uint_as_float(pd_word(vr[1][s], t)), h1, l1);
+                        pd_mma_tf32(d, pa, l0, l1);   // (the remainders first: what the second addition drops is all)
                         pd_mma_tf32(d, pa, h0, h1);
-                        pd_mma_tf32(d, pa, l0, l1);
                     }
                     acc[2 * VN * s + t] = fmaf(acc[2 * VN * s + t], alpha, d[0] + d[2]);
                     acc[2 * VN * s + VN + t] = fmaf(acc[2 * VN * s + VN + t], alpha, d[1] + d[3]);
