@@ -98,15 +98,27 @@ __device__ __forceinline__ unsigned long long request_units(const PagedAttn &a, 
     return sum;
 }
 
+// Quotients whose operands mostly fit 32 bits
+__device__ __forceinline__ unsigned long long paged_div(unsigned long long a, unsigned long long b) {
+    return ((a | b) >> 32) == 0 ? (unsigned long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+// One arrival of a CTA whose threads have met at a barrier, and will again: what they wrote before is there for whoever counts it, and what the others wrote for this one
+__device__ __forceinline__ uint32_t paged_arrive(uint32_t *counter) {
+    uint32_t before;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+    return before;
+}
+
 // ---- a CTA's range ----
 // Ranges of equal length, the last one shorter.  (Written without divisions where it can be: this is the code that a launch begins with, and code that runs once costs 12 clocks an instruction.)
 struct PagedRange {
     unsigned long long total, length, offset;   // units of the launch, of a range; the range's first unit, counted inside its request
+    unsigned long long per_group;               // units of a head group of that request, where they are known (0: not)
     uint32_t ranges, request;
     __device__ __forceinline__ unsigned long long first_unit(uint32_t c) const { return min(c * length, total); }
-    __device__ __forceinline__ uint32_t range_of(unsigned long long unit) const { return (uint32_t)(unit / length); }
+    __device__ __forceinline__ uint32_t range_of(unsigned long long unit) const { return (uint32_t)paged_div(unit, length); }
 };
-struct PagedRangeShared { unsigned long long sum[32], offset; uint32_t owner, request; };
+struct PagedRangeShared { unsigned long long sum[32], offset, per_group; uint32_t owner, request; };
 
 // Called by a whole CTA of THREADS threads; ends with a barrier.  total == 0: nothing to do in this launch.
 template <uint32_t KT, uint32_t THREADS>
@@ -122,13 +134,13 @@ __device__ __forceinline__ PagedRange paged_range(const PagedAttn &a, const Tile
         if (r < a.n_requests) q = paged_request(a, r);
         return request_units<KT>(a, q, shape.tokens) * head_groups;
     };
-    unsigned long long mine = 0;
+    unsigned long long mine = 0, group_units = 0;
     if (by_warp) {
         if (warp < a.n_requests) {
             const PagedRequest q = paged_request(a, warp);
             const uint32_t tiles = (q.n + shape.tokens - 1) / shape.tokens;
-            for (uint32_t j = lane; j < tiles; j += 32) mine += key_span<KT>(a, q, shape.tokens, j).units;
-            mine *= head_groups;
+            for (uint32_t j = lane; j < tiles; j += 32) group_units += key_span<KT>(a, q, shape.tokens, j).units;
+            mine = group_units * head_groups;
         }
     } else
         for (uint32_t b = 0; b < per; b++) mine += units_of(tid * per + b);
@@ -147,19 +159,22 @@ __device__ __forceinline__ PagedRange paged_range(const PagedAttn &a, const Tile
         const unsigned long long t = __shfl_up_sync(0xffffffffu, sums, o);
         if (lane >= (uint32_t)o) sums += t;
     }
-    PagedRange g = {__shfl_sync(0xffffffffu, sums, 31), 1, 0, 0, 0};
+    PagedRange g = {__shfl_sync(0xffffffffu, sums, 31), 1, 0, 0, 0, 0};
     if (g.total == 0) return g;
-    g.length = (g.total + gridDim.x - 1) / gridDim.x;
+    g.length = paged_div(g.total + gridDim.x - 1, gridDim.x);
     if (g.length < a.least_units) g.length = a.least_units;
-    g.ranges = (uint32_t)((g.total + g.length - 1) / g.length);
+    g.ranges = (uint32_t)paged_div(g.total + g.length - 1, g.length);
     const unsigned long long first = g.first_unit(blockIdx.x);
     unsigned long long before = __shfl_sync(0xffffffffu, sums, warp ? warp - 1 : 0);
     if (warp == 0) before = 0;
     if (by_warp) {
         const unsigned long long all = __shfl_sync(0xffffffffu, upto, 31);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) group_units += __shfl_xor_sync(0xffffffffu, group_units, o);
         if (lane == 0 && first >= before && first < before + all) {
             sh.offset = first - before;
             sh.request = warp;
+            sh.per_group = group_units;
         }
     } else {
         before += upto - mine;
@@ -196,6 +211,7 @@ __device__ __forceinline__ PagedRange paged_range(const PagedAttn &a, const Tile
     }
     g.request = sh.request;
     g.offset = sh.offset;
+    if (by_warp) g.per_group = sh.per_group;
     return g;
 }
 
@@ -222,10 +238,13 @@ struct PagedWalk {
         unit = g.first_unit(blockIdx.x);
         end = g.first_unit(blockIdx.x + 1);
         load(a, s, g.request);
-        PagedRequest one = q;
-        if (lane) one.n = 0;   // (the others help)
-        per_group = __shfl_sync(0xffffffffu, request_units<KT>(a, one, s.tokens), 0);
-        group = (uint32_t)(g.offset / per_group);
+        per_group = g.per_group;
+        if (per_group == 0) {
+            PagedRequest one = q;
+            if (lane) one.n = 0;   // (the others help)
+            per_group = __shfl_sync(0xffffffffu, request_units<KT>(a, one, s.tokens), 0);
+        }
+        group = (uint32_t)paged_div(g.offset, per_group);
         unsigned long long left = g.offset - group * per_group;
         for (uint32_t j = 0;; j += 32) {   // the query tile
             const uint32_t u = j + lane < tiles ? key_span<KT>(a, q, s.tokens, j + lane).units : 0u;

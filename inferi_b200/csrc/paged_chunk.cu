@@ -350,12 +350,10 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                     __stcg(part + 128 * HS + row, m);
                     __stcg(part + 128 * (HS + 1) + row, l);
                 }
-                __threadfence();
                 pc_sync_half(half);
                 if (row == 0 && side == 0) {
-                    const uint32_t is_last = atomicAdd(a.counters + 2 * c0 + half, 1u) == c1 - c0;
+                    const uint32_t is_last = paged_arrive(a.counters + 2 * c0 + half) == c1 - c0;
                     if (is_last) a.counters[2 * c0 + half] = 0u;   // for the next launch
-                    __threadfence();
                     S.last[half] = is_last;
                 }
                 pc_sync_half(half);

@@ -266,31 +266,47 @@ __global__ void __launch_bounds__(PD_THREADS, pd_ctas_per_sm(sizeof(T))) paged_d
 #pragma unroll
             for (int i = 0; i < D; i += 4) __stcg(reinterpret_cast<float4 *>(part + 2 * PD_ROWS + row * HS + d0 + i), make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]));
             if ((tid & 15) == 0) __stcg(reinterpret_cast<float2 *>(part) + row, make_float2(mx, sum));
-            __threadfence();
             __syncthreads();
             if (tid == 0) {
-                const uint32_t last = atomicAdd(a.counters + c0, 1u) == c1 - c0;
+                const uint32_t last = paged_arrive(a.counters + c0) == c1 - c0;
                 if (last) a.counters[c0] = 0u;   // for the next launch
-                __threadfence();
                 sm_last = last;
             }
             __syncthreads();
             finish = sm_last != 0;
             if (finish) {
+                // the pieces in their order, some at a time: their loads are in flight together
+                constexpr uint32_t AT_ONCE = HS == 128 ? 4 : 8;
                 mx = -INFINITY;
                 sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < D; i++) y[i] = 0.f;
-                for (uint32_t k = c0; k <= c1; k++) mx = fmaxf(mx, __ldcg(reinterpret_cast<const float2 *>(a.scratch + (size_t)paged_place(range, w.tile_unit(), k) * pd_partial_floats(HS)) + row).x);
-                for (uint32_t k = c0; k <= c1; k++) {
-                    const float *from = a.scratch + (size_t)paged_place(range, w.tile_unit(), k) * pd_partial_floats(HS);
-                    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(from) + row);
-                    const float wt = mx == -INFINITY ? 0.f : paged_ex2(ml.x - mx);
-                    sum += wt * ml.y;
+                for (uint32_t k0 = c0; k0 <= c1; k0 += AT_ONCE) {
+                    float2 ml[AT_ONCE];
+                    float4 v[AT_ONCE][D / 4];
+                    float top = mx;
 #pragma unroll
-                    for (int i = 0; i < D; i += 4) {
-                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(from + 2 * PD_ROWS + row * HS + d0 + i));
-                        y[i] += wt * v.x; y[i + 1] += wt * v.y; y[i + 2] += wt * v.z; y[i + 3] += wt * v.w;
+                    for (uint32_t k = 0; k < AT_ONCE; k++) {
+                        const float *from = a.scratch + (size_t)paged_place(range, w.tile_unit(), min(k0 + k, c1)) * pd_partial_floats(HS);
+                        ml[k] = __ldcg(reinterpret_cast<const float2 *>(from) + row);
+#pragma unroll
+                        for (int i = 0; i < D / 4; i++) v[k][i] = __ldcg(reinterpret_cast<const float4 *>(from + 2 * PD_ROWS + row * HS + d0) + i);
+                    }
+#pragma unroll
+                    for (uint32_t k = 0; k < AT_ONCE; k++) top = fmaxf(top, ml[k].x);
+                    const float keep = mx == -INFINITY ? 0.f : paged_ex2(mx - top);
+                    mx = top;
+                    sum *= keep;
+#pragma unroll
+                    for (int i = 0; i < D; i++) y[i] *= keep;
+#pragma unroll
+                    for (uint32_t k = 0; k < AT_ONCE; k++) {
+                        const float wt = k0 + k > c1 || ml[k].x == -INFINITY ? 0.f : paged_ex2(ml[k].x - mx);
+                        sum += wt * ml[k].y;
+#pragma unroll
+                        for (int i = 0; i < D / 4; i++) {
+                            y[4 * i] += wt * v[k][i].x; y[4 * i + 1] += wt * v[k][i].y; y[4 * i + 2] += wt * v[k][i].z; y[4 * i + 3] += wt * v[k][i].w;
+                        }
                     }
                 }
             }
