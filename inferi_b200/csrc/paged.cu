@@ -12,16 +12,19 @@ namespace cg = cooperative_groups;
 // ---- ib_page_plan ----
 // Four sums over the requests, each taken ahead of a request: of the pages that ended requests return, of the new tokens (who has room among the rows), of the
 // pages that those need (who gets pages), and of the tokens of the requests that remain.  Everything written follows from these sums and the inputs, element by
-// element, so the launch is one cluster: every CTA forms the sums of all requests for itself in shared memory (a scan of 1024 requests is 0.5 us, an exchange
-// between CTAs not less), they meet once - all inputs have been read, which is what lets kv_len be cached_len - and share out what is written.  What a
-// token's page is never comes from the table entries or stack entries that this launch writes: a page from the stack's old part is read from there, a returned one from
-// the ended request's row of the table.
-// Latency bounds it: a chain of some scans, then binary searches in shared memory.
-constexpr uint32_t PLAN_MAX_REQUESTS = 8192, PLAN_THREADS = 1024, PLAN_CLUSTER = 8;
+// element, so the launch is one cluster: every CTA forms the sums of all requests for itself in shared memory (a scan is 0.5 us, an exchange between CTAs not
+// less), and they share out what is written.  They meet twice: once all lengths have been read, which is what lets kv_len be cached_len, and once the table's new
+// entries are written, from which a token's page is read as those of before are.  A page from the stack's old part is read from there, a returned one from
+// the ended request's row of the table; no entry that this launch puts on the stack is read.
+// Latency bounds it: a chain of some scans, then binary searches in shared memory and reads of the table.
+// 16 decoding requests take 4.8 us; 2000 with 40,000 tokens in chunks of prompts, 104,400 rows, 15.4 us: the sums 5, pages 4, tokens 5.
+// How many threads (decoding requests, us; 128 threads / 1024 / a cluster of 8): 16: 5.1 / 5.6 / 6.7; 100: 9.4 / 6.2 / 6.8; 250: 17.5 / 7.4 / 6.9; 2000: - / 28 / 12.6.
+constexpr uint32_t PLAN_MAX_REQUESTS = 8192, PLAN_THREADS = 1024, PLAN_FEW = 128, PLAN_CLUSTER = 8;
 
 struct PlanRequest { int32_t cached, tokens_end; uint32_t need_before, back_before; };   // sums ahead of it (tokens: including it)
 
 // Sums over the block ahead of each thread, of two values at once; *a_all, *b_all get the totals.  Ends with a barrier.
+template <uint32_t THREADS>
 __device__ __forceinline__ void plan_scan(unsigned long long &a, unsigned long long &b, unsigned long long *a_all, unsigned long long *b_all, unsigned long long (&red)[2][32]) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const unsigned long long a0 = a, b0 = b;
@@ -32,7 +35,7 @@ __device__ __forceinline__ void plan_scan(unsigned long long &a, unsigned long l
     }
     if (lane == 31) { red[0][warp] = a; red[1][warp] = b; }
     __syncthreads();
-    unsigned long long x = red[0][lane], y = red[1][lane];   // PLAN_THREADS == 1024: 32 warps
+    unsigned long long x = lane < THREADS / 32 ? red[0][lane] : 0ull, y = lane < THREADS / 32 ? red[1][lane] : 0ull;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const unsigned long long u = __shfl_up_sync(0xffffffffu, x, o), w = __shfl_up_sync(0xffffffffu, y, o);
@@ -46,7 +49,9 @@ __device__ __forceinline__ void plan_scan(unsigned long long &a, unsigned long l
     __syncthreads();
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const ib_page_plan_args p, uint32_t page_log2) {
+// THREADS: a few requests are a small CTA's work, whose barriers are cheaper
+template <uint32_t THREADS>
+__global__ void __launch_bounds__(THREADS) page_plan_kernel(const ib_page_plan_args p, uint32_t page_log2) {
     extern __shared__ __align__(16) PlanRequest R[];   // [n_requests]
     __shared__ unsigned long long red[2][32];
     cg::cluster_group cluster = cg::this_cluster();
@@ -57,7 +62,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const ib_page_p
     struct Lens { long long have, want, need; int32_t status; bool ended, bad; };
     auto lens_of = [&](uint32_t i) {   // of a request, as far as its own lengths go
         Lens l = {0, 0, 0, IB_PLAN_OK, false, false};
-        const int32_t cached = p.cached_len[i], add = p.new_len[i];
+        const int32_t cached = R[i].cached, add = R[i].tokens_end;   // (as loaded)
         l.ended = add < 0;
         l.bad = cached < 0 || pages_of(cached) > width;
         if (l.bad) { l.status = IB_PLAN_INVALID; return l; }
@@ -68,55 +73,64 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const ib_page_p
         if (l.have + l.need > width) { l.status = IB_PLAN_TABLE_FULL; l.want = l.need = 0; }
         return l;
     };
-    // Sums ahead of a request: returned pages; new tokens.  Then, where there is room for the tokens, needed pages; then tokens again, of those that got pages.
-    unsigned long long backs = 0, wants = 0, needs = 0, ends = 0, takens = 0;
-    for (uint32_t base = 0; base < n; base += PLAN_THREADS) {
-        const uint32_t i = base + tid;
-        Lens l = {0, 0, 0, IB_PLAN_OK, false, false};
-        if (i < n) l = lens_of(i);
-        unsigned long long back = l.ended ? l.have : 0, want = l.want, all_back, all_want;
-        plan_scan(back, want, &all_back, &all_want, red);
-        if (i < n) {
-            R[i].cached = l.want > 0 && wants + want + l.want > p.max_tokens ? 1 : 0;   // no room (kept here till the last pass)
-            R[i].back_before = (uint32_t)min(backs + back, 0xFFFFFFFFull);
-        }
-        backs += all_back;
-        wants += all_want;
+    // A thread's requests follow one another, so that a scan over the threads is one over all of them.
+    const uint32_t each = (n + THREADS - 1) / THREADS, mine = min(tid * each, n), mine_end = min(mine + each, n);
+#pragma unroll 2
+    for (uint32_t i = mine; i < mine_end; i++) {
+        R[i].cached = p.cached_len[i];
+        R[i].tokens_end = p.new_len[i];
     }
-    const unsigned long long size = min((unsigned long long)n_free + backs, (unsigned long long)p.n_pages), returned = size - n_free;   // (more than n_pages: pages returned twice)
-    for (uint32_t base = 0; base < n; base += PLAN_THREADS) {
-        const uint32_t i = base + tid;
-        Lens l = {0, 0, 0, IB_PLAN_OK, false, false};
-        bool room = true;
-        if (i < n) {
-            l = lens_of(i);
-            room = R[i].cached == 0;
-        }
-        unsigned long long need = room ? l.need : 0, none = 0, all, all_none, all_taken;
-        const unsigned long long mine = need;
-        plan_scan(need, none, &all, &all_none, red);
-        need += needs;
-        const bool pages = mine == 0 || need + mine <= size, in = room && pages;
-        needs += all;
-        unsigned long long tokens = in ? l.want : 0, taken = in ? mine : 0;
-        const unsigned long long my_tokens = tokens;
-        plan_scan(tokens, taken, &all, &all_taken, red);
-        if (i < n) {
-            PlanRequest r;
-            r.cached = l.bad || l.ended ? 0 : p.cached_len[i];
-            r.tokens_end = (int32_t)(ends + tokens + my_tokens);
-            r.need_before = (uint32_t)min(need, size);   // (those that get pages are ahead of all that do not: the sum ahead of one is the sum of what is taken)
-            r.back_before = R[i].back_before;
-            R[i] = r;
-            if (cluster.block_rank() == 0) p.status[i] = !room ? IB_PLAN_NO_ROOM : (!pages ? IB_PLAN_NO_PAGES : l.status);
-        }
-        ends += all;
-        takens += all_taken;
+    // Sums ahead of a request: returned pages; new tokens.  Then, where there is room for the tokens, needed pages; then, if anyone is refused, tokens again, of those that got pages.
+    unsigned long long back = 0, want = 0, need = 0, none = 0, returns, wants, needs, all_none;
+    for (uint32_t i = mine; i < mine_end; i++) {
+        const Lens l = lens_of(i);
+        back += l.ended ? l.have : 0;
+        want += l.want;
     }
-    const uint32_t n_tokens = (uint32_t)ends;
+    plan_scan<THREADS>(back, want, &returns, &wants, red);
+    const unsigned long long size = min((unsigned long long)n_free + returns, (unsigned long long)p.n_pages), returned = size - n_free;   // (more than n_pages: pages returned twice)
+    auto has_room = [&](const Lens &l, unsigned long long &ahead) {   // ahead: the tokens wanted ahead of it
+        ahead += l.want;
+        return l.want == 0 || ahead <= p.max_tokens;
+    };
+    unsigned long long ahead = want;
+    for (uint32_t i = mine; i < mine_end; i++) {
+        const Lens l = lens_of(i);
+        if (has_room(l, ahead)) need += l.need;
+    }
+    plan_scan<THREADS>(need, none, &needs, &all_none, red);
+    unsigned long long tokens = 0, taken = 0, got = need;
+    bool out = false;
+    ahead = want;
+    for (uint32_t i = mine; i < mine_end; i++) {
+        const Lens l = lens_of(i);
+        const bool room = has_room(l, ahead);
+        if (room) got += l.need;
+        if (room && (l.need == 0 || got <= size)) { tokens += l.want; taken += l.need; }
+        else out = true;
+    }
+    unsigned long long n_all = wants, takens = needs;
+    if (__syncthreads_or(out)) plan_scan<THREADS>(tokens, taken, &n_all, &takens, red);
+    else tokens = want;
+    ahead = want;
+    for (uint32_t i = mine; i < mine_end; i++) {
+        const Lens l = lens_of(i);
+        const bool room = has_room(l, ahead), pages = l.need == 0 || need + l.need <= size;
+        PlanRequest r;
+        if (room && pages) tokens += l.want;
+        r.cached = l.bad || l.ended ? 0 : R[i].cached;
+        r.tokens_end = (int32_t)tokens;
+        r.need_before = (uint32_t)min(need, size);   // (those that get pages are ahead of all that do not: the sum ahead of one is the sum of what is taken)
+        r.back_before = (uint32_t)min(back, 0xFFFFFFFFull);
+        if (room) need += l.need;
+        back += l.ended ? l.have : 0;
+        R[i] = r;
+        if (cluster.block_rank() == 0) p.status[i] = !room ? IB_PLAN_NO_ROOM : (!pages ? IB_PLAN_NO_PAGES : l.status);
+    }
+    const uint32_t n_tokens = (uint32_t)n_all;
     __syncthreads();
     if (cluster.num_blocks() > 1) cluster.sync();   // everyone has read the lengths
-    const uint32_t worker = cluster.block_rank() * PLAN_THREADS + tid, workers = cluster.num_blocks() * PLAN_THREADS;
+    const uint32_t worker = cluster.block_rank() * THREADS + tid, workers = cluster.num_blocks() * THREADS;
 
     auto owner = [&](uint32_t PlanRequest::*sum, uint32_t x) {   // the last request with its sum ahead <= x (requests without pages share their successor's)
         uint32_t lo = 0, hi = n;
@@ -140,29 +154,44 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const ib_page_p
         p.row_start[i + 1] = R[i].tokens_end;
         if (i == 0) p.row_start[0] = 0;
     }
-    for (uint32_t i = worker >> 5; i < n; i += workers >> 5) {   // a warp per request: chunks of a prompt need many pages
-        const uint32_t add = (uint32_t)R[i].tokens_end - tokens_before(i), have = (uint32_t)pages_of(R[i].cached);
-        const uint32_t need = add ? (uint32_t)pages_of((long long)R[i].cached + add) - have : 0u;
-        for (uint32_t j = tid & 31; j < need; j += 32) p.block_table[(size_t)i * width + have + j] = stack((uint32_t)size - 1 - R[i].need_before - j);
+    for (uint32_t g = worker; g < (uint32_t)takens; g += workers) {   // a thread per page: chunks of a prompt need many
+        const uint32_t i = owner(&PlanRequest::need_before, g);
+        p.block_table[(size_t)i * width + (uint32_t)pages_of(R[i].cached) + (g - R[i].need_before)] = stack((uint32_t)size - 1 - g);
     }
     if (worker == 0) *p.n_free_out = (int32_t)(size - takens);
     for (uint32_t r = worker; r < (uint32_t)returned; r += workers) p.free_pages[n_free + r] = returned_page(r);
-    for (uint32_t t = worker; t < p.max_tokens; t += workers) {
-        int32_t pos = 0, slot = -1;
-        if (t < n_tokens) {
-            uint32_t lo = 0, hi = n - 1;   // the first request whose tokens end behind t
+    __syncthreads();
+    if (cluster.num_blocks() > 1) cluster.sync();   // the table is whole
+    // Tokens, four to a thread: one search, and their table entries are requested together
+    const bool whole = (((uintptr_t)p.positions | (uintptr_t)p.slots) & 15) == 0;
+    for (uint32_t t0 = 4 * worker; t0 < p.max_tokens; t0 += 4 * workers) {
+        int32_t pos[4] = {0, 0, 0, 0}, slot[4] = {-1, -1, -1, -1}, page[4];
+        if (t0 < n_tokens) {
+            uint32_t lo = 0, hi = n - 1;   // the first request whose tokens end behind t0
             while (lo < hi) {
                 const uint32_t mid = (lo + hi) >> 1;
-                if ((uint32_t)R[mid].tokens_end > t) hi = mid; else lo = mid + 1;
+                if ((uint32_t)R[mid].tokens_end > t0) hi = mid; else lo = mid + 1;
             }
-            const uint32_t have = (uint32_t)pages_of(R[lo].cached);
-            pos = R[lo].cached + (int32_t)(t - tokens_before(lo));
-            const uint32_t at = (uint32_t)pos >> page_log2;
-            const int32_t page = at < have ? p.block_table[(size_t)lo * width + at] : stack((uint32_t)size - 1 - R[lo].need_before - (at - have));
-            if (page >= 0 && (uint32_t)page < p.n_pages) slot = (int32_t)(((uint32_t)page << page_log2) + ((uint32_t)pos & (P - 1)));
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) {
+                page[e] = -1;
+                if (t0 + e >= n_tokens) continue;
+                while (lo + 1 < n && (uint32_t)R[lo].tokens_end <= t0 + e) lo++;
+                pos[e] = R[lo].cached + (int32_t)(t0 + e - tokens_before(lo));
+                page[e] = p.block_table[(size_t)lo * width + ((uint32_t)pos[e] >> page_log2)];
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++)
+                if (page[e] >= 0 && (uint32_t)page[e] < p.n_pages) slot[e] = (int32_t)(((uint32_t)page[e] << page_log2) + ((uint32_t)pos[e] & (P - 1)));
         }
-        p.positions[t] = pos;
-        p.slots[t] = slot;
+        if (whole && t0 + 4 <= p.max_tokens) {
+            *reinterpret_cast<int4 *>(p.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+            *reinterpret_cast<int4 *>(p.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+        } else
+            for (uint32_t e = 0; e < 4 && t0 + e < p.max_tokens; e++) {
+                p.positions[t0 + e] = pos[e];
+                p.slots[t0 + e] = slot[e];
+            }
     }
 }
 
@@ -321,24 +350,25 @@ int32_t ib_page_plan(ib_ctx *ctx, void *stream, const ib_page_plan_args *args) {
     static bool attr_set[16] = {false};
     const bool beyond = ctx->device >= 16;
     if (beyond || !attr_set[ctx->device]) {
-        IB_CHECK_CUDA(cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(PLAN_MAX_REQUESTS * sizeof(PlanRequest))));
+        IB_CHECK_CUDA(cudaFuncSetAttribute(page_plan_kernel<PLAN_THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(PLAN_MAX_REQUESTS * sizeof(PlanRequest))));
         if (!beyond) attr_set[ctx->device] = true;
     }
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
-    const uint32_t ctas = a.n_requests <= 256 && a.max_tokens <= 2 * PLAN_THREADS ? 1 : PLAN_CLUSTER;
+    const bool few = a.n_requests <= PLAN_FEW / 4 && a.max_tokens <= 8 * PLAN_FEW;
+    const uint32_t ctas = few || (a.n_requests <= PLAN_FEW && a.max_tokens <= 4 * PLAN_THREADS) ? 1 : PLAN_CLUSTER;
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = ctas;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(PLAN_THREADS);
+    cfg.blockDim = dim3(few ? PLAN_FEW : PLAN_THREADS);
     cfg.dynamicSmemBytes = a.n_requests * sizeof(PlanRequest);
     cfg.stream = (cudaStream_t)stream;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    IB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, page_plan_kernel, a, log2_of(a.page_size)));
+    IB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, few ? page_plan_kernel<PLAN_FEW> : page_plan_kernel<PLAN_THREADS>, a, log2_of(a.page_size)));
     ctx->launches++;
     return IB_OK;
 }
