@@ -34,17 +34,19 @@ constexpr uint32_t BS_BINS = 1024, BS_LIST = 1024;
 constexpr uint32_t BS_MAX_VOCAB = 1u << 19;   // S < 2^63
 constexpr int BS_ONE = 44;                    // the largest weight is 2^44 units
 // The histogram's reach below the largest weight, at most, in factors of two.  A border below it is looked for in a second one, of the stretch behind the first.
-constexpr double BS_OCTAVES = 16.0, BS_OCTAVES_K = 11.0;
+constexpr double BS_OCTAVES = 16.0, BS_OCTAVES_K = 11.0, BS_OCTAVES_SUM = 8.0;
 constexpr uint32_t BS_WINDOWS = 4;                  // such stretches, at most
 // Vocabularies up to this size are one CTA's work, up to twice this size two CTAs' and so on
 constexpr uint32_t BS_ONE_CTA = 4096;
-constexpr uint32_t BS_HOT = 32;               // places that a thread keeps
+constexpr uint32_t BS_QUEUE = 16, BS_STEP = 8;  // a thread's elements that wait to be taken; those that come together
+constexpr uint32_t BS_KEPT = 768;             // the histogram's elements whose places a warp keeps
+constexpr uint32_t BS_SAMPLE = 4096, BS_SAMPLED = 20000;   // logits that say how far the histogram should reach, for slices above that size
 constexpr uint32_t BS_SMEM_LIMIT = 227 * 1024;
 
 struct BatchSampleParams {
     const float *logits;
     uint64_t stride;
-    uint32_t n, slice, resident;   // tokens of a row, of a CTA; whether a slice is held in shared memory
+    uint32_t n, slice, resident, sampled;   // tokens of a row, of a CTA; whether a slice is held in shared memory; whether some logits say how far the histogram goes
     const float *temperature, *top_p, *min_p, *coin;
     const int32_t *top_k;
     int32_t *token;
@@ -73,12 +75,20 @@ struct BsShared {
         uint2 mass[BS_BINS];                            // ... and their weight, as two words; in the first CTA, when a list is there,
         unsigned long long run[BS_LIST];                // the running weight through each of its elements
     };
-    unsigned long long tot_mass[BS_BINS];               // first CTA: the cluster's histogram, then the sums ahead of each bin
-    uint32_t tot_cnt[BS_BINS];
-    unsigned long long list[BS_LIST];                   // listed elements, (~order of x, index)
+    union {
+        struct {
+            unsigned long long tot_mass[BS_BINS];       // first CTA: the cluster's histogram, then the sums ahead of each bin
+            uint32_t tot_cnt[BS_BINS];
+            unsigned long long list[BS_LIST];           // listed elements, (~order of x, index)
+        };
+        struct {                                        // before there is any of these, by threads: elements that wait to be taken, and their places in the warp's stretch
+            float wait_x[BS_WARPS][BS_QUEUE][32];
+            uint16_t wait_at[BS_WARPS][BS_QUEUE][32];
+        };
+    };
+    uint16_t kept[BS_WARPS][BS_KEPT];                   // places in its stretch of a warp's elements that are in the histogram
     unsigned long long seg[BS_CLUSTER * BS_WARPS];      // first CTA: weight or count of every warp's stretch of the row
     unsigned long long red[2][BS_WARPS];
-    uint16_t hot[BS_WARPS][BS_HOT][32];                 // places in the slice of the elements that may be in the histogram, by threads
     float lo[BS_CLUSTER];                               // of every CTA's slice: its smallest finite logit
     unsigned long long best[BS_CLUSTER];                // ... and its arg-max
     unsigned long long part_mass[BS_CLUSTER], part_min[BS_CLUSTER];   // first CTA: weight of each slice, of its elements with w >= min_p
@@ -98,15 +108,15 @@ __device__ __forceinline__ uint32_t bs_order(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float bs_value(uint32_t order) { return __uint_as_float(order & 0x80000000u ? order & 0x7FFFFFFFu : ~order); }
-// what is no number is never drawn; an infinity is the largest number
-__device__ __forceinline__ float bs_clean(float x) { return x > -INFINITY ? fminf(x, FLT_MAX) : -INFINITY; }
+// what is no number is never drawn; an infinity is the largest number; the zeros are the same
+__device__ __forceinline__ float bs_clean(float x) { return x > -INFINITY ? fminf(x, FLT_MAX) + 0.f : -INFINITY; }
 
 // Sum over a warp of numbers below 2^44: the halves in the reduction unit
 __device__ __forceinline__ unsigned long long bs_sum(unsigned long long w) {
     return (unsigned long long)__reduce_add_sync(0xffffffffu, (uint32_t)w & 0x3FFFFFu) + ((unsigned long long)__reduce_add_sync(0xffffffffu, (uint32_t)(w >> 22)) << 22);
 }
 
-static_assert(BS_MAX_VOCAB / BS_CLUSTER <= 65536, "places are 16 bits");
+static_assert(BS_MAX_VOCAB / BS_WARPS <= 65536, "places are 16 bits");
 
 struct BsWeight {
     float hi;
@@ -273,12 +283,11 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
             uint32_t at[K];
             float x[K];
 #pragma unroll
-            for (uint32_t e = 0; e < K; e++) {
-                at[e] = k + 32 * e < many ? place(k + 32 * e) : 0u;
-                x[e] = k + 32 * e < many ? logit(at[e]) : -INFINITY;
-            }
+            for (uint32_t e = 0; e < K; e++) at[e] = place(min(k + 32 * e, many - 1));
 #pragma unroll
-            for (uint32_t e = 0; e < K; e++) body(at[e], x[e]);   // (-infinity behind the last one)
+            for (uint32_t e = 0; e < K; e++) x[e] = here[at[e]];   // (without a condition: a branch each would wait for each)
+#pragma unroll
+            for (uint32_t e = 0; e < K; e++) body(at[e], k + 32 * e < many ? bs_clean(x[e]) : -INFINITY);
         }
     };
     // a warp's elements: a stretch of the slice
@@ -286,9 +295,53 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
 
     // ---- what a step does ----
     // bins of x: equal stretches down from the largest logit
-    // (a limit by rank mostly ends far above one by mass, and one by min_p says itself where)
-    const double octaves = fmin(by_k ? BS_OCTAVES_K : BS_OCTAVES, by_min && !(by_k && by_p) ? 0.01 - log2((double)fmaxf(min_p, 1e-30f)) : BS_OCTAVES);
-    const float reach = (float)fmin(fmax(octaves, 0.01) / weight.c, (double)hi - (double)lo), per_bin = reach > 0.f && isfinite(reach) ? (float)BS_BINS * (1.f - 0x1p-20f) / reach : 0.f;
+    // As far as the borders, if that can be told: min_p says so itself; where rank k or the mass top_p lies is seen from some of the row's logits, by half octaves.
+    // (Every CTA of the row takes the same ones.  A border behind the reach costs another histogram, no more.)
+    double octaves = filtered ? (by_k ? BS_OCTAVES_K : BS_OCTAVES) : BS_OCTAVES_SUM;
+    if (p.sampled && (by_k || by_p)) {
+        octaves = BS_OCTAVES;
+        constexpr uint32_t HALVES = 64, E = BS_SAMPLE / BS_THREADS;
+        const bool all = p.n <= BS_SAMPLE;
+        if (tid < HALVES) S.cnt[tid] = 0u;
+        float x[E];
+#pragma unroll
+        for (uint32_t e = 0; e < E; e++) {
+            const uint32_t j = e * BS_THREADS + tid, at = all ? j : (uint32_t)((uint64_t)(j >> 3) * p.n / (BS_SAMPLE / 8)) + (j & 7);   // (eight neighbours are a sector of memory)
+            x[e] = at < p.n ? bs_clean(__ldg(p.logits + row * p.stride + at)) : -INFINITY;
+        }
+        __syncthreads();
+        const float scale = 2.f * (float)weight.c;
+#pragma unroll
+        for (uint32_t e = 0; e < E; e++) {
+            const float h = (hi - x[e]) * scale;
+            if (h < (float)HALVES) atomicAdd(&S.cnt[(uint32_t)h], 1u);
+        }
+        __syncthreads();
+        const float share = all ? 1.f : (float)p.n / (float)BS_SAMPLE;   // a sampled one stands for so many
+        const float n0 = (float)S.cnt[2 * lane] * share, n1 = (float)S.cnt[2 * lane + 1] * share, octave = exp2f(-(float)lane);
+        // By rank: where there are a quarter more, and six sampled ones.  By mass: where what is behind is less than 1 - top_p of the whole.  Many sampled ones are behind, few perhaps
+        // in front, so the whole is taken as low as their scatter allows: 1.5 times the root of the sum of squares less.
+        const float m0 = n0 * 0.84f * octave, m1 = n1 * 0.59f * octave;
+        float sum = by_k ? n0 + n1 : m0 + m1, whole = m0 + m1, scatter = all ? 0.f : (m0 * 0.84f + m1 * 0.59f) * octave * share;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const float t = by_k ? __shfl_up_sync(0xffffffffu, sum, o) : __shfl_down_sync(0xffffffffu, sum, o);
+            if (by_k ? (int)lane >= o : (int)lane + o < 32) sum += t;
+            whole += __shfl_xor_sync(0xffffffffu, whole, o);
+            scatter += __shfl_xor_sync(0xffffffffu, scatter, o);
+        }
+        const float far = (1.f - top_p) * fmaxf(1.f, whole - 1.5f * sqrtf(scatter));
+        const uint32_t in0 = __ballot_sync(0xffffffffu, by_k ? sum - n1 >= (float)k * 1.25f + 6.f * share : sum - m0 <= far);
+        const uint32_t in1 = __ballot_sync(0xffffffffu, by_k ? sum >= (float)k * 1.25f + 6.f * share : sum - m0 - m1 <= far);
+        const uint32_t l0 = in0 ? __ffs(in0) - 1 : 32, l1 = in1 ? __ffs(in1) - 1 : 32;
+        octaves = fmin(octaves, fmin((double)l0 + 0.5, (double)l1 + 1.0) + 0.5);
+        __syncthreads();   // (the counters are cleared for the histogram)
+    }
+    if (by_min && !(by_k && by_p)) octaves = fmin(octaves, 0.01 - log2((double)fmaxf(min_p, 1e-30f)));
+    auto reach_of = [&](double octaves) { return (float)fmin(fmax(octaves, 0.01) / weight.c, (double)hi - (double)lo); };
+    auto bins_of = [&](float reach) { return reach > 0.f && isfinite(reach) ? (float)BS_BINS * (1.f - 0x1p-20f) / reach : 0.f; };
+    const float reach = reach_of(octaves);
+    float per_bin = bins_of(reach);
     uint32_t window = 0;           // of the row's stretches of that length
     auto bin_of = [&](float x) {   // >= BS_BINS: not in this window
         const float d = (hi - x) * per_bin;
@@ -345,20 +398,40 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
     // elements that are looked at one by one: those of the histogram (and a little more), and what may reach min_p (a factor of two more: rounding)
     const float near = fmaxf(per_bin > 0.f ? reach * (1.f + 0x1p-18f) : INFINITY, by_min ? (float)((1.0 - log2((double)fmaxf(min_p, 1e-30f))) / weight.c) : 0.f);
     const float c_hi = (float)weight.c, c_lo = (float)(weight.c - (double)c_hi);
-    uint32_t n_hot = 0;       // the thread's places
-    bool all_listed = true;   // the warp's lists hold all of its elements of the histogram
+    uint32_t n_places = 0;      // the warp's kept places
+    bool all_kept = true;     // they are those of all of its elements of the histogram
     {
         unsigned long long sum = 0ull, above = 0ull;
-        uint32_t n = 0u, n_above = 0u;
+        uint32_t n = 0u, n_above = 0u, waiting = 0u;
         float small = 0.f;
         auto take = [&]() {
+            // one behind the other, from the front: a place that is written has been read
+            float *queue_x = &S.wait_x[warp][0][0];
+            uint16_t *queue_at = &S.wait_at[warp][0][0];
+            const uint32_t below = (1u << lane) - 1u;
+            uint32_t many = 0;
+            for (uint32_t k = 0;; k++) {
+                const uint32_t here = __ballot_sync(0xffffffffu, k < waiting);
+                if (!here) break;
+                const float x = queue_x[32 * k + lane];
+                const uint16_t at = queue_at[32 * k + lane];
+                __syncwarp();
+                if (k < waiting) {
+                    const uint32_t to = many + __popc(here & below);
+                    queue_x[to] = x;
+                    queue_at[to] = at;
+                }
+                many += __popc(here);
+            }
+            waiting = 0;
+            __syncwarp();
             constexpr uint32_t K = 4;   // a chain of some hundred clocks each: several at once
-            for (uint32_t k = 0; __any_sync(0xffffffffu, k < n_hot); k += K) {
+            for (uint32_t i = lane; i - lane < many; i += 32 * K) {
                 unsigned long long w[K];
                 uint32_t bin[K];
 #pragma unroll
                 for (uint32_t e = 0; e < K; e++) {
-                    const float x = k + e < n_hot ? logit(S.hot[warp][k + e][lane]) : -INFINITY;
+                    const float x = i + 32 * e < many ? queue_x[i + 32 * e] : -INFINITY;
                     w[e] = weight(x, S.table);
                     bin[e] = w[e] ? bin_of(x) : BS_BINS;
                 }
@@ -366,17 +439,21 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
                 for (uint32_t e = 0; e < K; e++) {
                     sum += w[e];
                     if (by_min && w[e] >= least) { above += w[e]; n_above++; }
-                    if (filtered && bin[e] < BS_BINS) add(bin[e], w[e]);
+                    if (!filtered) continue;
+                    const bool in = bin[e] < BS_BINS;
+                    if (in) add(bin[e], w[e]);
+                    const uint32_t stay = __ballot_sync(0xffffffffu, in);
+                    all_kept = all_kept && n_places + __popc(stay) <= BS_KEPT;
+                    if (!all_kept) continue;
+                    if (in) S.kept[warp][n_places + __popc(stay & below)] = queue_at[i + 32 * e];
+                    n_places += __popc(stay);
                 }
             }
+            __syncwarp();
         };
-        constexpr uint32_t U = 8;
-        auto some = [&](uint32_t i, const float (&x)[U]) {   // elements i + 32 e.  (What is no number is not above -infinity; an infinity is looked at one by one.)
-            if (__any_sync(0xffffffffu, n_hot > BS_HOT - U)) {
-                take();
-                n_hot = 0;
-                all_listed = false;
-            }
+        constexpr uint32_t U = BS_STEP;
+        auto some = [&](uint32_t i, const float (&x)[U]) {   // elements i + 32 e of the stretch.  (What is no number is not above -infinity; an infinity is FLT_MAX.)
+            if (__any_sync(0xffffffffu, waiting > BS_QUEUE - U)) take();
 #pragma unroll
             for (uint32_t e = 0; e < U; e++) {
                 const float d = x[e] - hi;
@@ -385,21 +462,33 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
                 asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(fmaf(d, c_hi, d * c_lo)));
                 n += any;
                 if (any && far) small += fmaxf(w, 0x1p-44f);
-                if (any && !far) S.hot[warp][n_hot++][lane] = (uint16_t)(i + 32 * e);
+                if (any && !far) {
+                    S.wait_x[warp][waiting][lane] = fminf(x[e], FLT_MAX);
+                    S.wait_at[warp][waiting++][lane] = (uint16_t)(i + 32 * e);
+                }
             }
         };
-        uint32_t i = w0;
-        for (; i + 32 * U <= w1; i += 32 * U) {   // (without a check for every element)
-            float x[U];
+        // (without a check for every element; the next ones are requested before these are looked at)
+        const float *mine = here + w0 + lane;
+        const uint32_t many = w1 - w0, whole = many / (32 * U) * (32 * U);
+        float x[U];
+        if (whole) {
 #pragma unroll
-            for (uint32_t e = 0; e < U; e++) x[e] = here[i + lane + 32 * e];
-            some(i + lane, x);
+            for (uint32_t e = 0; e < U; e++) x[e] = mine[32 * e];
         }
-        if (i < w1) {
-            float x[U];
+        for (uint32_t i = 0; i < whole; i += 32 * U) {
+            float y[U];
+            const bool more = i + 32 * U < whole;
 #pragma unroll
-            for (uint32_t e = 0; e < U; e++) x[e] = i + lane + 32 * e < w1 ? here[i + lane + 32 * e] : -INFINITY;
+            for (uint32_t e = 0; e < U; e++) y[e] = more ? mine[i + 32 * (U + e)] : 0.f;
             some(i + lane, x);
+#pragma unroll
+            for (uint32_t e = 0; e < U; e++) x[e] = y[e];
+        }
+        if (whole < many) {
+#pragma unroll
+            for (uint32_t e = 0; e < U; e++) x[e] = whole + lane + 32 * e < many ? mine[whole + 32 * e] : -INFINITY;
+            some(whole + lane, x);
         }
         take();
         sum += (unsigned long long)((double)small * (double)(1ull << BS_ONE));
@@ -560,7 +649,10 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
                 win_cnt += S.all_cnt;
                 list_lo = 1;
                 list_hi = 0;
-                say(BS_HISTOGRAM, window + 1, 0, 0, 0);
+                if (octaves < BS_OCTAVES) {
+                    win_mass = win_cnt = 0ull;
+                    say(BS_HISTOGRAM, 0, 1, 0, 0);
+                } else say(BS_HISTOGRAM, window + 1, 0, 0, 0);
                 return;
             }
             if (b < BS_BINS) {
@@ -639,6 +731,11 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
             clear();
             histogram = step == BS_HISTOGRAM;
             if (histogram) window = a;
+            if (histogram && b) {   // as far as a histogram goes
+                per_bin = bins_of(reach_of(BS_OCTAVES));
+                octaves = BS_OCTAVES;
+                all_kept = false;
+            }
             sweep(w1 - w0, [&](uint32_t k) { return w0 + k; }, [&](uint32_t, float x) {
                 const uint32_t order = ~bs_order(x);   // (ascending: the largest x first)
                 const uint32_t bin = histogram ? bin_of(x) : (order >> b) & ((1u << (a - b)) - 1u);
@@ -654,20 +751,17 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
             // into this CTA's own list, a place for every warp's elements together; the first CTA fetches them from all
             if (tid == 0) S.listed = 0;
             __syncthreads();
+            const float from_bin = (float)(a + BS_BINS * window), to_bin = (float)(b + 1 + BS_BINS * window);
             auto list = [&](uint32_t i, float x) {
                 const uint32_t order = ~bs_order(x);
-                bool in = x > -INFINITY;
-                if (step == BS_LIST_BINS) {
-                    const uint32_t bin = bin_of(x);
-                    in = in && bin >= a && bin <= b;
-                } else in = in && (a == 32 || order >> a == pre);
-                if (in) {
+                const float d = (hi - x) * per_bin;   // (bins a to b, without forming the bin)
+                if (step == BS_LIST_BINS ? d >= from_bin && d < to_bin : x > -INFINITY && (a == 32 || order >> a == pre)) {
                     const uint32_t at = atomicAdd(&S.listed, 1u);
                     if (at < BS_LIST) S.list[at] = (unsigned long long)order << 32 | (i0 + i);
                 }
             };
-            if (step == BS_LIST_BINS && all_listed && window == 0)
-                for (uint32_t k = 0; k < n_hot; k++) list(S.hot[warp][k][lane], logit(S.hot[warp][k][lane]));
+            const bool by_place = step == BS_LIST_BINS && all_kept && window == 0;
+            if (by_place) sweep(n_places, [&](uint32_t k) { return w0 + S.kept[warp][k]; }, list);
             else sweep(w1 - w0, [&](uint32_t k) { return w0 + k; }, list);
             barrier();
             if (rank == 0 && C > 1) {
@@ -780,8 +874,9 @@ extern "C" int32_t ib_sample_batch(ib_ctx *ctx, void *stream, const ib_sample_ba
     uint32_t ctas = BS_CLUSTER;
     while (ctas > 1 && (a.vocab <= BS_ONE_CTA * ctas / 2 || ((uint64_t)a.rows * ctas > 2 * (uint64_t)ctx->sm_count && a.vocab <= 65536 * ctas / 2))) ctas /= 2;
     p.slice = (a.vocab + ctas - 1) / ctas;
+    p.sampled = p.slice > BS_SAMPLED;
     // held in shared memory where that costs no CTA its place
-    const size_t with = sizeof(BsShared) + p.slice * sizeof(float);
+    const size_t without = sizeof(BsShared), with = without + p.slice * sizeof(float);
     p.resident = with <= BS_SMEM_LIMIT && ((uint64_t)a.rows * ctas <= (uint64_t)ctx->sm_count || 2 * (with + 1024) <= BS_SMEM_LIMIT + 1024);
     static bool attr_set[16] = {false};
     const bool beyond = ctx->device >= 16;
@@ -798,7 +893,7 @@ extern "C" int32_t ib_sample_batch(ib_ctx *ctx, void *stream, const ib_sample_ba
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3(a.rows * ctas);
     cfg.blockDim = dim3(BS_THREADS);
-    cfg.dynamicSmemBytes = sizeof(BsShared) + (p.resident ? p.slice * sizeof(float) : 0);
+    cfg.dynamicSmemBytes = p.resident ? with : without;
     cfg.stream = (cudaStream_t)stream;
     cfg.attrs = attr;
     cfg.numAttrs = 2;

@@ -216,3 +216,35 @@ def test_refusals(backend):
     refused("524289 tokens", vocab=524289, x=torch.zeros(3, 524289, device="cuda"))
     refused("0 tokens", vocab=0, x=torch.zeros(3, 0, device="cuda"))
     assert backend.lib.ib_sample_batch(backend.handle, None, None) == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [70, 5000, 150000])
+def test_zeros_of_either_sign_are_ties(backend, vocab):
+    """-0 and 0 are the same logit: the lower index first, whatever the sign."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    logits = -1.0 - torch.rand(8, vocab, generator=g, device="cuda")
+    at = torch.randperm(vocab, generator=g, device="cuda")[:60]
+    logits[:, at] = torch.where(torch.rand(8, 60, generator=g, device="cuda") < 0.5, -0.0, 0.0)
+    coin = [0.0, 0.1, 0.25, 0.5, 0.75, 0.9, 0.99, 0.3]
+    check(backend, logits, [0.1] * 8, [20] * 8, [0.9] * 8, None, coin)
+    check(backend, logits, [0.1] * 8, [0] * 8, [0.5] * 8, [0.2] * 8, coin)
+    tokens, _ = run(backend, logits, [0.0] * 8, None, None, None, coin)
+    assert tokens == [int(at.min())] * 8
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows, vocab", [(80, 128256), (160, 70000), (300, 33000)])
+def test_many_rows_whose_histogram_reaches_as_far_as_a_sample_says(backend, rows, vocab):
+    """Peaked and flat rows side by side: a few large logits that a sample misses, or finds; a border far behind them."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    logits = torch.randn(rows, vocab, generator=g, device="cuda") * torch.linspace(0.1, 4.0, rows, device="cuda")[:, None]
+    top = torch.randint(0, vocab, (rows, 3), generator=g, device="cuda")
+    logits.scatter_(1, top, torch.rand(rows, 3, generator=g, device="cuda") * 30)
+    logits[: rows // 8, :4096] -= 20.0
+    rng = np.random.default_rng(rows)
+    T = (0.4 + rng.random(rows)).astype(np.float32).tolist()
+    top_p = np.where(np.arange(rows) % 3 == 0, 0.9999, 0.5 + 0.49 * rng.random(rows)).astype(np.float32).tolist()
+    coin = rng.random(rows).astype(np.float32).tolist()
+    check(backend, logits, T, None, top_p, None, coin)
+    check(backend, logits, T, np.where(np.arange(rows) % 2, rng.integers(1, 5000, rows), 0).tolist(), top_p, [1e-6] * rows, coin)
