@@ -229,7 +229,7 @@ IB_API int32_t ib_paged_append(ib_ctx *ctx, void *stream, const ib_paged_append_
  * new ones, at position p = kv_len[r] - (number of new ones) + i, whose keys and values are in the cache already.  It sees the positions j <= p with
  * p - j < window or j < sinks (window 0: all of them): out = softmax(q K^T / sqrt(head_size)) V over these, and 0 where there are none.  Head h uses kv
  * head h / kv_mul.  head_size 64 or 128; kv_mul up to 64; kv_dim of the cache = n_heads / kv_mul * head_size.  Rows of q and out are *_stride floats apart; rows
- * behind row_start[n_requests] are neither read nor written.  Masked positions and rows of pages behind kv_len may hold anything, infinities and NaN too.
+ * behind row_start[n_requests] are neither read nor written, and out does not overlap q (out = q is refused).  Masked positions and rows of pages behind kv_len may hold anything, infinities and NaN too.
  * A page number outside the cache is never followed; what the rows of that request get then is not specified.
  * longest_new: the most new tokens that a request has, where the host knows it, else 0.  It chooses kernels, and any value gives right results. */
 typedef struct ib_paged_attn_args {

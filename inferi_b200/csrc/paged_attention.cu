@@ -6,7 +6,9 @@ namespace ib {
 int32_t check_paged_cache(const char *who, const ib_paged_cache *c);   // paged.cu
 uint32_t log2_of(uint32_t power);
 
-constexpr uint32_t PAGED_FEW_ROWS = 16;
+// Rows (new tokens * kv_mul) up to which a request is the decode kernel's.  At 32 requests over 4000 positions the two take the same at 20 rows (head size 64: 125 us and 131, 128: 186 and 181);
+// 16 rows 83 and 131, 117 and 181; 32 rows 155 and 132, 243 and 181.  One request alone is faster with the decode kernel (17 us and 28, 27 and 49 at 64 rows), until it is long: 249 us and 86 at 256 rows over 16,000 positions.
+constexpr uint32_t PAGED_FEW_ROWS = 24;
 
 // Scratch of a context, of one size whatever the arguments: made once and never moved, so a captured launch may be replayed at any time.  (Made while a stream is being
 // captured, it is cleared on a stream of its own: the capture does not get the clearing as a node.)
@@ -42,6 +44,7 @@ extern "C" int32_t ib_paged_attention(ib_ctx *ctx, void *stream, const ib_paged_
     if (rc) return rc;
     if (p.n_requests == 0 || p.n_tokens == 0) return IB_OK;
     IB_REQUIRE(p.q_dev && p.out_dev && p.block_table && p.row_start && p.kv_len, "ib_paged_attention: null pointer");
+    IB_REQUIRE((const float *)p.out_dev != p.q_dev, "ib_paged_attention: out is q");
     IB_REQUIRE(p.kv_mul >= 1 && p.kv_mul <= 64 && p.n_heads >= p.kv_mul && p.n_heads % p.kv_mul == 0, "ib_paged_attention: n_heads=%u is not a multiple of kv_mul=%u (1 to 64)", p.n_heads, p.kv_mul);
     if (p.head_size != 64 && p.head_size != 128) return set_error(IB_ERR_UNSUPPORTED, "ib_paged_attention: head_size=%u (supported: 64, 128)", p.head_size);
     IB_REQUIRE(p.n_heads <= (1u << 16), "ib_paged_attention: %u heads (up to 65536)", p.n_heads);

@@ -28,7 +28,7 @@ struct PagedAttn {
     uint32_t kv_heads, kv_mul, kv_dim;
     int32_t window, sinks;         // 0: no window
     uint32_t rows_from, rows_to;   // the launch takes the requests with that many rows (new tokens * kv_mul)
-    uint32_t least_units;          // units of a CTA's range, at least
+    float merge_cost;              // of a partial, in units' time
     uint32_t vec;                  // q and out are on 16-byte boundaries
     float *scratch;                // two partials per CTA
     uint32_t *counters;            // of arrivals, one per CTA and half of its tiles; zero between launches
@@ -120,8 +120,8 @@ struct PagedRange {
 };
 struct PagedRangeShared { unsigned long long sum[32], offset, per_group; uint32_t owner, request; };
 
-// Called by a whole CTA of THREADS threads; ends with a barrier.  total == 0: nothing to do in this launch.
-template <uint32_t KT, uint32_t THREADS>
+// Called by a whole CTA of THREADS threads; ends with a barrier.  MERGE_COST: partials cost something (a.merge_cost).  total == 0: nothing to do in this launch.
+template <uint32_t KT, uint32_t THREADS, bool MERGE_COST>
 __device__ __forceinline__ PagedRange paged_range(const PagedAttn &a, const TileShape &shape, PagedRangeShared &sh) {
     constexpr uint32_t WARPS = THREADS / 32;
     static_assert(WARPS <= 32, "one sum per warp");
@@ -135,11 +135,16 @@ __device__ __forceinline__ PagedRange paged_range(const PagedAttn &a, const Tile
         return request_units<KT>(a, q, shape.tokens) * head_groups;
     };
     unsigned long long mine = 0, group_units = 0;
+    uint32_t most = 0;   // units of a tile (by_warp)
     if (by_warp) {
         if (warp < a.n_requests) {
             const PagedRequest q = paged_request(a, warp);
             const uint32_t tiles = (q.n + shape.tokens - 1) / shape.tokens;
-            for (uint32_t j = lane; j < tiles; j += 32) group_units += key_span<KT>(a, q, shape.tokens, j).units;
+            for (uint32_t j = lane; j < tiles; j += 32) {
+                const uint32_t units = key_span<KT>(a, q, shape.tokens, j).units;
+                group_units += units;
+                if constexpr (MERGE_COST) most = max(most, units);
+            }
             mine = group_units * head_groups;
         }
     } else
@@ -150,10 +155,15 @@ __device__ __forceinline__ PagedRange paged_range(const PagedAttn &a, const Tile
         const unsigned long long t = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= (uint32_t)o) upto += t;
     }
-    if (lane == 31) sh.sum[warp] = upto;
+    if constexpr (MERGE_COST) most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 31) sh.sum[warp] = upto | (unsigned long long)min(most, 0xFFFFu) << 48;   // (units are far below 2^48: 2^25 rows over 2^31 positions make 2^47 at most)
     __syncthreads();
     // every warp: the sums of all warps
     unsigned long long sums = lane < WARPS ? sh.sum[lane] : 0ull;
+    if constexpr (MERGE_COST) {
+        most = __reduce_max_sync(0xffffffffu, (uint32_t)(sums >> 48));
+        sums &= (1ull << 48) - 1;
+    }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const unsigned long long t = __shfl_up_sync(0xffffffffu, sums, o);
@@ -162,7 +172,12 @@ __device__ __forceinline__ PagedRange paged_range(const PagedAttn &a, const Tile
     PagedRange g = {__shfl_sync(0xffffffffu, sums, 31), 1, 0, 0, 0, 0};
     if (g.total == 0) return g;
     g.length = paged_div(g.total + gridDim.x - 1, gridDim.x);
-    if (g.length < a.least_units) g.length = a.least_units;
+    // A tile of u units in ranges of L is done in the time of L units and of u / L partials, one after the other: L is the root of u times a partial's cost, at least.  (Where there are more
+    // requests than warps the tiles are more than the CTAs, mostly, and have one or two each.)
+    if (MERGE_COST && by_warp && a.merge_cost > 0.f) {
+        const uint32_t least = (uint32_t)sqrtf((float)most * a.merge_cost);
+        if (g.length < least) g.length = least;
+    }
     g.ranges = (uint32_t)paged_div(g.total + g.length - 1, g.length);
     const unsigned long long first = g.first_unit(blockIdx.x);
     unsigned long long before = __shfl_sync(0xffffffffu, sums, warp ? warp - 1 : 0);

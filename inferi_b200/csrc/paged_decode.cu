@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(PD_THREADS, pd_ctas_per_sm(sizeof(T))) paged_d
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = lane >> 2, c = lane & 3;
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const PagedRange range = paged_range<PD_KT, PD_THREADS>(a, shape, range_sh);
+    const PagedRange range = paged_range<PD_KT, PD_THREADS, false>(a, shape, range_sh);
     if (range.total == 0 || blockIdx.x >= range.ranges) return;
     PagedWalk<PD_KT> w;
     w.begin(a, shape, range);
@@ -355,7 +355,6 @@ int32_t launch_paged_decode(ib_ctx *ctx, cudaStream_t s, PagedAttn a, uint32_t h
     shape.heads = a.kv_mul < PD_ROWS ? a.kv_mul : PD_ROWS;
     shape.groups = (a.kv_mul + shape.heads - 1) / shape.heads;
     shape.tokens = PD_ROWS / shape.heads;
-    a.least_units = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((uint32_t)ctx->sm_count * (kv_dtype == IB_KV_F16 ? pd_ctas_per_sm(2) : pd_ctas_per_sm(4)));
     cfg.blockDim = dim3(PD_THREADS);

@@ -276,12 +276,16 @@ def test_both_ways_refuse_the_same(backend, monkeypatch):
     def sample(vocab=50, logits=(4, 50), T=4, k=None, token=None):
         return lambda: BatchSampler(b, vocab).sample(f(*logits), f(T), k, None, None, f(4), token)
 
+    def in_place():
+        q = f(3, 128)
+        PagedAttention(b).launch(PagedAttentionConfig(2, 2, 64), q, cache, cache, i(2, 2), i(3), i(2), q)
+
     refused = [plan(page=24), plan(page=8), plan(table=(3, 2)), plan(table=(8,)), plan(starts=4), plan(status=3), plan(slots=7), plan(free=0), plan(n=9000, table=(9000, 1), starts=9001, status=9000),
                append(variant=7), append(hs=48), append(hs=512, q=(3, 512)), append(q=(3, 100)), append(k=(3, 128)), append(slots=2), append(vc=half), append(kc=f(2, 16, 60), vc=f(2, 16, 60)),
                append(kc=f(2, 17, 64), vc=f(2, 17, 64)), append(kc=cache[0], vc=cache[0]),
                attention(hs=32, heads=4), attention(mul=1), attention(mul=3, heads=3, q=(3, 192), out=(3, 192), kc=half), attention(out=(2, 128)), attention(q=(3, 64)), attention(table=(3, 2)), attention(starts=2),
                attention(heads=0), attention(window=-1), attention(vc=cache[:, :, :32]), attention(heads=130, mul=130, q=(3, 130 * 64), out=(3, 130 * 64)),
-               sample(vocab=51), sample(vocab=600000, logits=(4, 600000)), sample(T=3), sample(k=f(4)), sample(token=f(4)), sample(token=i(5))]
+               in_place, sample(vocab=51), sample(vocab=600000, logits=(4, 600000)), sample(T=3), sample(k=f(4)), sample(token=f(4)), sample(token=i(5))]
 
     def answers():
         out = []
