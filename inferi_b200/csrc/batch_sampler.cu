@@ -20,6 +20,8 @@
 // there, so that one list answers every question - are listed and sorted.  Bins too full for the list (ties) or below the histogram: the same by digits of x's order, to the last
 // tie in index order.  The first CTA of the cluster leads: it looks at the merged histogram and says what all do next (BsStep).  Its threads carry the same state and search sums by
 // bisection, each for itself, without barriers.
+// What bounds it, at 128,256 logits: a chain of barriers, scans and short lists for few rows (one row with top-p 39 us; 33 rows of 32,003 45 us); for many the passes over logits that
+// have left the caches and the arithmetic of the elements in the histogram: 250 rows 190 us with settings of every row's own; arg-max 32, no filter 100, top-k 50 124, top-p 0.9 228.
 #include "op_launch.cuh"
 
 #include <cooperative_groups.h>
@@ -34,14 +36,16 @@ constexpr uint32_t BS_THREADS = 512, BS_WARPS = BS_THREADS / 32, BS_CLUSTER = 8;
 constexpr uint32_t BS_BINS = 1024, BS_LIST = 1024;
 constexpr uint32_t BS_MAX_VOCAB = 1u << 19;   // S < 2^63
 constexpr int BS_ONE = 44;                    // the largest weight is 2^44 units
-// The histogram's reach below the largest weight, at most, in factors of two.  A border below it is looked for in a second one, of the stretch behind the first.
+// The histogram's reach below the largest weight, in factors of two, where no sample says better; of the elements that are taken one by one without a filter.  A border below it is looked for
+// in a second one, of the stretch behind the first.  (Normal logits of deviation 3.  One row, top-k 50, reach 11 or 16: 29 and 36 us.  No filter, 8 or 16: one row 20 and 25, 250 rows 100 and 174.)
 constexpr double BS_OCTAVES = 16.0, BS_OCTAVES_K = 11.0, BS_OCTAVES_SUM = 8.0;
 constexpr uint32_t BS_WINDOWS = 4;                  // such stretches, at most
-// Vocabularies up to this size are one CTA's work, up to twice this size two CTAs' and so on
-constexpr uint32_t BS_ONE_CTA = 4096;
+// Vocabularies up to this size are one CTA's work, up to twice this size two CTAs' and so on: what a cluster's barriers cost is not less than what a small slice saves.  (Top-k 50, slices of 8192
+// or 4096 at most: one row of 8000 20 and 23 us, 33 rows of 32,003 25 and 35; 12,000 at most: the same, but top-p 0.9 of one row of 20,000 35 and 39.)
+constexpr uint32_t BS_ONE_CTA = 8192;
 constexpr uint32_t BS_QUEUE = 16, BS_STEP = 8;  // a thread's elements that wait to be taken; those that come together
 constexpr uint32_t BS_KEPT = 768;             // the histogram's elements whose places a warp keeps
-constexpr uint32_t BS_SAMPLE = 4096, BS_SAMPLED = 20000;   // logits that say how far the histogram should reach, for slices above that size
+constexpr uint32_t BS_SAMPLE = 4096, BS_SAMPLED = 20000;   // logits that say how far the histogram should reach, for slices above that size (250 rows, top-p 0.9: 236 us, without 306; one row in slices of 16,032: 44 and 45, top-k 50 30 and 29)
 constexpr uint32_t BS_SMEM_LIMIT = 227 * 1024;
 
 struct BatchSampleParams {
@@ -873,7 +877,8 @@ extern "C" int32_t ib_sample_batch(ib_ctx *ctx, void *stream, const ib_sample_ba
     p.logits = a.logits_dev; p.stride = a.stride; p.n = a.vocab;
     p.temperature = a.temperature; p.top_p = a.top_p; p.min_p = a.min_p; p.top_k = a.top_k; p.coin = a.coin;
     p.token = a.token; p.prob = a.prob;
-    // CTAs of a row: up to 8, while all rows' have a place at once (two on an SM); a slice has 65536 tokens at most
+    // CTAs of a row: up to 8, while all rows' have a place at once (two on an SM); a slice has 65536 tokens at most.  (250 rows of 128,256: one CTA each 279 us, two 190, four 195: with one, the
+    // rows that take longest are alone at the end.)
     uint32_t ctas = BS_CLUSTER;
     while (ctas > 1 && (a.vocab <= BS_ONE_CTA * ctas / 2 || ((uint64_t)a.rows * ctas > 2 * (uint64_t)ctx->sm_count && a.vocab <= 65536 * ctas / 2))) ctas /= 2;
     p.slice = (a.vocab + ctas - 1) / ctas;
