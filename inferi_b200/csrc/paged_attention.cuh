@@ -156,7 +156,7 @@ __device__ __forceinline__ PagedRange paged_range(const PagedAttn &a, const Tile
         if (lane >= (uint32_t)o) upto += t;
     }
     if constexpr (MERGE_COST) most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 31) sh.sum[warp] = upto | (unsigned long long)min(most, 0xFFFFu) << 48;   // (units are far below 2^48: 2^25 rows over 2^31 positions make 2^47 at most)
+    if (lane == 31) sh.sum[warp] = upto | (unsigned long long)min(most, 0xFFFFu) << 48;   // (2^48 units would take years)
     __syncthreads();
     // every warp: the sums of all warps
     unsigned long long sums = lane < WARPS ? sh.sum[lane] : 0ull;

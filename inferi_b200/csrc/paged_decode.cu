@@ -47,6 +47,12 @@ __device__ __forceinline__ void pd_split_tf32(float x, uint32_t &hi, uint32_t &l
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));   // (the MMA would drop its lower bits, always towards zero)
 }
+// The same for what the cache holds, without conversions (16 a clock and SM): the upper bits, as which the MMA takes x itself, and what is left of x, rounded by half a step of what the MMA drops.
+// A value that is no number is one in hi, whatever lo becomes.
+__device__ __forceinline__ void pd_cut_tf32(uint32_t x, uint32_t &hi, uint32_t &lo) {
+    hi = x & 0xFFFFE000u;
+    lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi)) + 0x1000u;
+}
 __device__ __forceinline__ uint4 pd_load(const void *p) { return __ldcg(reinterpret_cast<const uint4 *>(p)); }
 __device__ __forceinline__ uint32_t pd_word(const uint4 &v, int i) { return i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w)); }
 
@@ -172,8 +178,8 @@ __global__ void __launch_bounds__(PD_THREADS, pd_ctas_per_sm(sizeof(T))) paged_d
                         for (int e = 0; e < 4; e += 2) {
                             const uint32_t qq[4] = {qa[4 * s + e][0], qa[4 * s + e][1], qa[4 * s + e + 1][0], qa[4 * s + e + 1][1]};
                             uint32_t h0, l0, h1, l1;
-                            pd_split_tf32(__uint_as_float(pd_word(kr[i][s], e)), h0, l0);
-                            pd_split_tf32(__uint_as_float(pd_word(kr[i][s], e + 1)), h1, l1);
+                            pd_cut_tf32(pd_word(kr[i][s], e), h0, l0);
+                            pd_cut_tf32(pd_word(kr[i][s], e + 1), h1, l1);
                             pd_mma_tf32(d[s & 3], qq, h0, h1);
                             pd_mma_tf32(d[4], qq, l0, l1);
                         }
@@ -224,8 +230,8 @@ __global__ void __launch_bounds__(PD_THREADS, pd_ctas_per_sm(sizeof(T))) paged_d
                         pd_mma(d, pa, __byte_perm(pd_word(vr[0][s], t / 2), pd_word(vr[1][s], t / 2), sel), __byte_perm(pd_word(vr[2][s], t / 2), pd_word(vr[3][s], t / 2), sel));
                     } else {
                         uint32_t h0, l0, h1, l1;
-                        pd_split_tf32(__uint_as_float(pd_word(vr[0][s], t)), h0, l0);
-                        pd_split_tf32(__uint_as_float(pd_word(vr[1][s], t)), h1, l1);
+                        pd_cut_tf32(pd_word(vr[0][s], t), h0, l0);
+                        pd_cut_tf32(pd_word(vr[1][s], t), h1, l1);
                         pd_mma_tf32(d, pa, l0, l1);   // (the remainders first: what the second addition drops is all)
                         pd_mma_tf32(d, pa, h0, h1);
                     }
