@@ -15,8 +15,8 @@
 //   V   lane (n, c) has elements 64 i + 8 n .. + 7 of positions 2c, 2c + 1, 2c + 8, 2c + 9: MMA t of a piece makes the result's elements 64 i + 8 n + t, n = 0 .. 7,
 //       from pairs of positions that a byte permute puts together.  A lane's results are elements 64 i + 16 c .. + 15 of row n.
 // 64 requests over up to 8000 positions, 32 heads of 128, four to a kv head (1.57 GB): 248 us, 6.3 TB/s.  One over 500: 7.1 us, of which a launch is 2.5; the rest is the chain of lengths,
-// pages, K, softmax, V, arrival and merge.  24 requests with 5 tokens and 8 heads to a kv head over 3000 positions of a 32-bit cache (224 MB): 177 us: five tiles of 8 rows read every
-// row again, and splitting it into two tf32 is what issue slots go to.
+// pages, K, softmax, V, arrival and merge.  24 requests with 5 tokens and 8 heads to a kv head over 3000 positions of a 32-bit cache (224 MB): 133 us: up to five
+// tiles of 8 rows read and cut every row again, and a warp's step is a chain (data, K's products, softmax, V's products) that 12 warps on an SM do not hide.
 // (32-bit: pieces of 4 elements, MMAs of 8 columns: K elements 16 i + 4 c .. + 3, V elements 32 i + 4 n .. + 3 of positions 2c, 2c + 1; results 32 i + 8 c .. + 7.)
 #include "paged_attention.cuh"
 
@@ -57,10 +57,10 @@ __device__ __forceinline__ uint4 pd_load(const void *p) { return __ldcg(reinterp
 __device__ __forceinline__ uint32_t pd_word(const uint4 &v, int i) { return i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w)); }
 
 constexpr uint32_t pd_partial_floats(uint32_t hs) { return PD_ROWS * (hs + 2); }
-constexpr uint32_t pd_ctas_per_sm(uint32_t elem) { return elem == 2 ? 3u : 2u; }
+constexpr uint32_t PD_CTAS_PER_SM = 3;   // (32-bit, with two of 237 registers a thread: 140 us instead of 133, see above)
 
 template <typename T, int HS>
-__global__ void __launch_bounds__(PD_THREADS, pd_ctas_per_sm(sizeof(T))) paged_decode_kernel(const __grid_constant__ PagedAttn a, const TileShape shape) {
+__global__ void __launch_bounds__(PD_THREADS, PD_CTAS_PER_SM) paged_decode_kernel(const __grid_constant__ PagedAttn a, const TileShape shape) {
     constexpr bool F16 = sizeof(T) == 2;
     constexpr int NP = F16 ? 16 : 8;               // positions of a warp's step
     constexpr int KP = HS * sizeof(T) / 64;        // a lane's pieces of a position of K (the row's 16-byte pieces over four lanes)
@@ -170,8 +170,8 @@ __global__ void __launch_bounds__(PD_THREADS, pd_ctas_per_sm(sizeof(T))) paged_d
                     x[i][0] = d[0] + d[2];
                     x[i][1] = d[1] + d[3];
                 } else {
-                    // K's remainders have sums of their own, and its upper parts four: short chains drop less
-                    float d[5][4] = {};
+                    // K's remainders have sums of their own, four as its upper parts have: short chains drop less and take less time (one for the remainders: 157 us instead of 140)
+                    float d[8][4] = {};
 #pragma unroll
                     for (int s = 0; s < KP; s++)
 #pragma unroll
@@ -181,10 +181,10 @@ __global__ void __launch_bounds__(PD_THREADS, pd_ctas_per_sm(sizeof(T))) paged_d
                             pd_cut_tf32(pd_word(kr[i][s], e), h0, l0);
                             pd_cut_tf32(pd_word(kr[i][s], e + 1), h1, l1);
                             pd_mma_tf32(d[s & 3], qq, h0, h1);
-                            pd_mma_tf32(d[4], qq, l0, l1);
+                            pd_mma_tf32(d[4 + (s & 3)], qq, l0, l1);
                         }
-                    x[i][0] = ((d[0][0] + d[1][0]) + (d[2][0] + d[3][0])) + (((d[0][2] + d[1][2]) + (d[2][2] + d[3][2])) + (d[4][0] + d[4][2]));
-                    x[i][1] = ((d[0][1] + d[1][1]) + (d[2][1] + d[3][1])) + (((d[0][3] + d[1][3]) + (d[2][3] + d[3][3])) + (d[4][1] + d[4][3]));
+                    x[i][0] = ((d[0][0] + d[1][0]) + (d[2][0] + d[3][0])) + (((d[0][2] + d[1][2]) + (d[2][2] + d[3][2])) + (((d[4][0] + d[5][0]) + (d[6][0] + d[7][0])) + ((d[4][2] + d[5][2]) + (d[6][2] + d[7][2]))));
+                    x[i][1] = ((d[0][1] + d[1][1]) + (d[2][1] + d[3][1])) + (((d[0][3] + d[1][3]) + (d[2][3] + d[3][3])) + (((d[4][1] + d[5][1]) + (d[6][1] + d[7][1])) + ((d[4][3] + d[5][3]) + (d[6][3] + d[7][3]))));
                 }
             }
             if ((int32_t)j0 + NP - 1 > p_lo || (a.window && p_hi - (int32_t)j0 >= a.window)) {   // not every row sees all of these positions
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(PD_THREADS, pd_ctas_per_sm(sizeof(T))) paged_d
     } while (w.next(a, shape));
 }
 
-uint32_t paged_decode_ctas(const ib_ctx *ctx) { return (uint32_t)ctx->sm_count * 3; }
+uint32_t paged_decode_ctas(const ib_ctx *ctx) { return (uint32_t)ctx->sm_count * PD_CTAS_PER_SM; }
 size_t paged_decode_scratch_floats(const ib_ctx *ctx, uint32_t head_size) { return (size_t)paged_decode_ctas(ctx) * 2 * pd_partial_floats(head_size); }
 
 int32_t launch_paged_decode(ib_ctx *ctx, cudaStream_t s, PagedAttn a, uint32_t head_size, int kv_dtype) {
@@ -365,7 +365,7 @@ int32_t launch_paged_decode(ib_ctx *ctx, cudaStream_t s, PagedAttn a, uint32_t h
     shape.groups = (a.kv_mul + shape.heads - 1) / shape.heads;
     shape.tokens = PD_ROWS / shape.heads;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((uint32_t)ctx->sm_count * (kv_dtype == IB_KV_F16 ? pd_ctas_per_sm(2) : pd_ctas_per_sm(4)));
+    cfg.gridDim = dim3(paged_decode_ctas(ctx));
     cfg.blockDim = dim3(PD_THREADS);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];

@@ -248,3 +248,40 @@ def test_many_rows_whose_histogram_reaches_as_far_as_a_sample_says(backend, rows
     coin = rng.random(rows).astype(np.float32).tolist()
     check(backend, logits, T, None, top_p, None, coin)
     check(backend, logits, T, np.where(np.arange(rows) % 2, rng.integers(1, 5000, rows), 0).tolist(), top_p, [1e-6] * rows, coin)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows, vocab", [(200, 45000), (80, 128256)])
+def test_odd_rows_among_many(backend, rows, vocab):
+    """Rows of one value, of two, with one number only, with none, with infinities and NaN; temperatures from nothing to a million; limits at their ends - where a slice is large enough for
+    a sample to say how far the histogram goes."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    logits = torch.randn(rows, vocab, generator=g, device="cuda") * 2
+    logits[0] = 3.0
+    logits[1] = torch.where(torch.rand(vocab, generator=g, device="cuda") < 0.5, 1.0, -1.0)
+    logits[2] = -math.inf
+    logits[2, vocab - 3] = -5.0
+    logits[3] = math.nan
+    logits[4, ::3] = math.nan
+    logits[5, 100:107] = math.inf
+    logits[6] = torch.linspace(-1e30, 1e30, vocab, device="cuda")
+    logits[7] = logits[7].round()
+    logits[8, : vocab // 2] = -math.inf
+    logits[9] = 1000.0 + logits[9] * 1e-3
+    logits[10] = logits[10] * 1e-6
+    logits[11, ::31] = 9.0    # (whatever a sample finds, or misses)
+    logits[12, 5:13] = 30.0
+    rng = np.random.default_rng(vocab)
+    kinds = 20
+    T = np.tile(np.array([1.0, 0.7, 1e-6, 1e6, 1e-30, 30.0, 0.9, 1.0], dtype=np.float32), rows)[:rows]
+    T[:16] = 1.0
+    coin = rng.random(rows).astype(np.float32)
+    coin[::17], coin[5::17] = 0.0, np.float32(1 - 2**-24)
+    for top_k, top_p, min_p in ((None, [0.9] * rows, None), ([1, 2, 50, vocab - 1, vocab, 0, 3000, 40000][:8] * (rows // 8), None, None),
+                                (None, [1e-6, 1 - 2**-24, 0.5, 0.9999] * (rows // 4), [0.0, 1e-30, 0.5, 1.0] * (rows // 4)), ([200, 0] * (rows // 2), [0.8, 0.99] * (rows // 2), None)):
+        tokens, probs = run(backend, logits, T.tolist(), top_k, top_p, min_p, coin.tolist())
+        x = logits.cpu().numpy()
+        for r in list(range(kinds)) + list(range(kinds, rows, 7)):
+            want, p = choose(x[r], float(T[r]), top_k[r] if top_k else 0, top_p[r] if top_p else 1.0, min_p[r] if min_p else 0.0, coin[r])
+            assert tokens[r] == want, (r, tokens[r], want)
+            assert abs(probs[r] - p) <= p * (2**-24 + 2**-29) + vocab * 2**-44, (r, probs[r], p)
