@@ -772,15 +772,22 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
             else sweep(w1 - w0, [&](uint32_t k) { return w0 + k; }, list);
             barrier();
             if (rank == 0 && C > 1) {
-                uint32_t own = min(S.listed, BS_LIST);
-                for (uint32_t r = 1; r < C; r++) {
+                // all CTAs' counts at once, then two warps per CTA
+                static_assert(BS_WARPS / 2 >= BS_CLUSTER - 1, "two warps for every other CTA");
+                const uint32_t n = lane < C ? min(cluster.map_shared_rank(&S, lane)->listed, BS_LIST) : 0u;
+                uint32_t upto = n;
+#pragma unroll
+                for (int o = 1; o < (int)BS_CLUSTER; o <<= 1) {
+                    const uint32_t t = __shfl_up_sync(0xffffffffu, upto, o);
+                    if ((int)lane >= o) upto += t;
+                }
+                const uint32_t r = 1 + warp / 2, many = __shfl_sync(0xffffffffu, n, r), to = __shfl_sync(0xffffffffu, upto, r) - many, all = __shfl_sync(0xffffffffu, upto, C - 1);
+                if (r < C) {
                     const BsShared &o = *cluster.map_shared_rank(&S, r);
-                    const uint32_t n = min(o.listed, BS_LIST - own);
-                    for (uint32_t i = tid; i < n; i += BS_THREADS) S.list[own + i] = o.list[i];
-                    own += n;
+                    for (uint32_t i = lane + 32 * (warp & 1); i < many && to + i < BS_LIST; i += 64) S.list[to + i] = o.list[i];
                 }
                 __syncthreads();
-                if (tid == 0) S.listed = own;
+                if (tid == 0) S.listed = min(all, BS_LIST);
                 __syncthreads();
             }
         } else if (step == BS_SEGMENT) {   // index order: the element of warp a's stretch at which the running weight exceeds arg
