@@ -20,7 +20,7 @@
 // there, so that one list answers every question - are listed and sorted.  Bins too full for the list (ties) or below the histogram: the same by digits of x's order, to the last
 // tie in index order.  The first CTA of the cluster leads: it looks at the merged histogram and says what all do next (BsStep).  Its threads carry the same state and search sums by
 // bisection, each for itself, without barriers.
-// What bounds it, at 128,256 logits: a chain of barriers, scans and short lists for few rows (one row with top-p 39 us; 33 rows of 32,003 45 us); for many the passes over logits that
+// What bounds it, at 128,256 logits: a chain of barriers, scans and short lists for few rows (one row with top-p 38 us; 33 rows of 32,003 45 us); for many the passes over logits that
 // have left the caches and the arithmetic of the elements in the histogram: 250 rows 190 us with settings of every row's own; arg-max 32, no filter 100, top-k 50 124, top-p 0.9 228.
 #include "op_launch.cuh"
 

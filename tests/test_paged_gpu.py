@@ -302,3 +302,29 @@ def test_refusals(backend):
     a = ops.PagePlanArgs(9000, 1, 1, 1, 16, *[idx.data_ptr()] * 11)
     assert backend.lib.ib_page_plan(backend.handle, None, C.byref(a)) == 1 and b"9000 requests" in backend.lib.ib_last_error_string()
     assert backend.lib.ib_page_plan(backend.handle, None, None) == 1 and backend.lib.ib_paged_append(backend.handle, None, None, None) == 1
+
+
+@pytest.mark.parametrize("n", [32, 33, 128, 129, 8192])
+def test_plan_at_the_borders_of_its_launches(backend, n):
+    test_plan_against_one_request_after_the_other(backend, n, 16, 90, 7, True)
+
+
+@pytest.mark.parametrize("offset,room", [(0, 41), (1, 40), (2, 43), (3, 8)])
+def test_plan_writes_its_rows_and_no_others(backend, offset, room):
+    """Positions and slots that begin off the 16-byte boundaries, and end where four do not."""
+    n, P = 6, 16
+    cached, new, free = i32([0, 15, 16, 40, 3, 31]), i32([5, 2, -1, 9, 0, 11]), i32(np.arange(30))
+    table = i32(np.arange(100, 100 + 6 * 4).reshape(6, 4) % 30)
+    d = [i32([-7] * 60) for _ in range(2)]
+    positions, slots = (t[offset: offset + room] for t in d)
+    kv, starts, status, n_free = i32([0] * n), i32([0] * (n + 1)), i32([0] * n), i32([20])
+    PagePlan(backend).launch(P, cached, new, table, free, n_free, kv, starts, positions, slots, n_free, status)
+    for t in d:
+        assert (t[:offset] == -7).all() and (t[offset + room:] == -7).all()
+    total = int(starts[-1])
+    assert total == (27 if room > 8 else 7)
+    assert (positions[total:] == 0).all() and (slots[total:] == -1).all() and (slots[:total] >= 0).all()
+    want = [p for c, a, b in zip(cached.tolist(), starts.tolist(), starts.tolist()[1:]) for p in range(c, c + b - a)]
+    assert positions[:total].tolist() == want
+    assert [s % P for s in slots[:total].tolist()] == [p % P for p in want]
+    assert [s // P for s in slots[:total].tolist()] == [int(table[r, p // P]) for r, (c, a, b) in enumerate(zip(cached.tolist(), starts.tolist(), starts.tolist()[1:])) for p in range(c, c + b - a)]
