@@ -197,9 +197,12 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(const ib_page_plan_a
 
 // ---- ib_paged_append ----
 // A CTA per row.  It requests all of its data, computes the row's (cos, sin) pairs meanwhile, and rotates: every element is read and written once, and HBM bounds it: 8001 rows of 32 heads of 128
-// (360 MB) take 64 us, 5.6 TB/s; 64 rows of 64 take 2.6 us, a launch.
+// (360 MB) take 57.5 us, 6.3 TB/s; 64 rows of 64 take 2.6 us, a launch.
 // An item is eight elements as two vectors of four: four pairs of the rotation (ORIGINAL: (0, 1), (2, 3) of each; NEOX: element i of the first with i of the second).
-constexpr uint32_t APPEND_THREADS = 256, APPEND_ITEMS = 3;   // items of a thread that are in flight together
+constexpr uint32_t APPEND_ITEMS = 3;   // items of a thread that are in flight together
+// Threads of a CTA: 256 while the rows' CTAs have a place together, more or less; behind that 128, of which twice as many rows are under way.  (32 heads of 128, 128 or 256: one row 3.8 and 2.9 us, 500
+// 9.2 and 5.6, 2000 17.9 and 18.7, 8001 57.5 and 64.)
+constexpr uint32_t APPEND_FEW = 256, APPEND_MANY = 128, APPEND_ROWS_PER_SM = 12;
 constexpr uint32_t APPEND_MAX_HEAD = 256;
 
 struct AppendParams {
@@ -219,8 +222,8 @@ __device__ __forceinline__ void put1(float *p, float x) { *p = x; }
 __device__ __forceinline__ void put1(__half *p, float x) { *p = __float2half_rn(x); }
 
 // VEC: everything is on 16-byte boundaries and head_size is a multiple of 8; otherwise a pair at a time
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(const __grid_constant__ AppendParams p) {
+template <typename T, bool VEC, uint32_t THREADS>
+__global__ void __launch_bounds__(THREADS) paged_append_kernel(const __grid_constant__ AppendParams p) {
     __shared__ float2 cs[APPEND_MAX_HEAD / 2];
     const uint32_t tid = threadIdx.x, row = blockIdx.x, hs = p.a.head_size, half = hs / 2, q_dim = p.a.q_dim, kv_dim = p.kv_dim;
     const bool neox = p.a.variant == IB_ROPE_NEOX;
@@ -232,7 +235,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(const __gr
     float *q_out = p.a.q_out_dev + row * p.a.q_out_stride;
     T *kc = static_cast<T *>(p.k) + at, *vc = static_cast<T *>(p.v) + at;
     auto angles = [&]() {
-        for (uint32_t j = tid; j < half; j += APPEND_THREADS) {
+        for (uint32_t j = tid; j < half; j += THREADS) {
             const double t = (double)pos * p.turns[j];
             float s, c;
             sincospif((float)(2.0 * (t - rint(t))), &s, &c);
@@ -255,11 +258,11 @@ __global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(const __gr
             y = x + half;
         };
         bool first = true;
-        for (uint32_t base = tid; base < n_items || first; base += APPEND_THREADS * APPEND_ITEMS) {
+        for (uint32_t base = tid; base < n_items || first; base += THREADS * APPEND_ITEMS) {
             float4 f[APPEND_ITEMS][2];
 #pragma unroll
             for (uint32_t i = 0; i < APPEND_ITEMS; i++) {
-                const uint32_t e = base + i * APPEND_THREADS;
+                const uint32_t e = base + i * THREADS;
                 if (e >= n_items) continue;
                 const float *src = e < n_q ? q : (e < n_q + n_k ? k : v);
                 uint32_t x, y, j;
@@ -270,7 +273,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(const __gr
             if (first) { angles(); first = false; }
 #pragma unroll
             for (uint32_t i = 0; i < APPEND_ITEMS; i++) {
-                const uint32_t e = base + i * APPEND_THREADS;
+                const uint32_t e = base + i * THREADS;
                 if (e >= n_items) continue;
                 const bool rotated = e < n_q + n_k;
                 uint32_t x, y, j;
@@ -298,7 +301,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(const __gr
     } else {
         angles();
         const uint32_t n_q = q_dim / 2, n_k = kv_dim / 2;
-        for (uint32_t e = tid; e < n_q + n_k; e += APPEND_THREADS) {
+        for (uint32_t e = tid; e < n_q + n_k; e += THREADS) {
             const bool of_q = e < n_q;
             const uint32_t i = of_q ? e : e - n_q, j = i % half, x = neox ? (i / half) * hs + j : 2 * i, y = neox ? x + half : x + 1;
             const float *src = of_q ? q : k;
@@ -306,7 +309,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(const __gr
             if (of_q) { q_out[x] = r.x; q_out[y] = r.y; }
             else { put1(kc + x, r.x); put1(kc + y, r.y); }
         }
-        for (uint32_t e = tid; e < kv_dim; e += APPEND_THREADS) put1(vc + e, v[e]);
+        for (uint32_t e = tid; e < kv_dim; e += THREADS) put1(vc + e, v[e]);
     }
 }
 
@@ -408,9 +411,11 @@ int32_t ib_paged_append(ib_ctx *ctx, void *stream, const ib_paged_append_args *a
     for (uint32_t j = 0; j < a.head_size / 2; j++) p.turns[j] = turns[j];
     auto whole = [](const void *ptr, uint64_t stride) { return (uintptr_t)ptr % 16 == 0 && stride % 4 == 0; };
     const bool vec = a.head_size % 8 == 0 && whole(a.q_dev, a.q_stride) && whole(a.k_dev, a.k_stride) && whole(a.v_dev, a.v_stride) && whole(a.q_out_dev, a.q_out_stride);
-    void (*kernel)(AppendParams) = cache->kv_dtype == IB_KV_F16 ? (vec ? paged_append_kernel<__half, true> : paged_append_kernel<__half, false>)
-                                                                : (vec ? paged_append_kernel<float, true> : paged_append_kernel<float, false>);
-    return launch_op(ctx, (cudaStream_t)stream, kernel, a.n, APPEND_THREADS, p);
+    const bool f16 = cache->kv_dtype == IB_KV_F16, many = vec && a.n > APPEND_ROWS_PER_SM * (uint32_t)ctx->sm_count;
+    void (*kernel)(AppendParams) = many  ? (f16 ? paged_append_kernel<__half, true, APPEND_MANY> : paged_append_kernel<float, true, APPEND_MANY>)
+                                   : vec ? (f16 ? paged_append_kernel<__half, true, APPEND_FEW> : paged_append_kernel<float, true, APPEND_FEW>)
+                                         : (f16 ? paged_append_kernel<__half, false, APPEND_FEW> : paged_append_kernel<float, false, APPEND_FEW>);
+    return launch_op(ctx, (cudaStream_t)stream, kernel, a.n, many ? APPEND_MANY : APPEND_FEW, p);
 }
 
 }  // extern "C"

@@ -328,3 +328,10 @@ def test_plan_writes_its_rows_and_no_others(backend, offset, room):
     assert positions[:total].tolist() == want
     assert [s % P for s in slots[:total].tolist()] == [p % P for p in want]
     assert [s // P for s in slots[:total].tolist()] == [int(table[r, p // P]) for r, (c, a, b) in enumerate(zip(cached.tolist(), starts.tolist(), starts.tolist()[1:])) for p in range(c, c + b - a)]
+
+
+@pytest.mark.parametrize("variant", [ops.ROPE_ORIGINAL, ops.ROPE_NEOX])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("hs,heads,kv_heads,n", [(64, 4, 2, 1776), (64, 4, 2, 1777), (128, 3, 3, 2500), (8, 40, 2, 2000)])
+def test_append_of_more_rows_than_have_a_place_together(backend, variant, dtype, hs, heads, kv_heads, n):
+    check_append(backend, variant, hs, heads, kv_heads, n, 32, dtype, 2000)
