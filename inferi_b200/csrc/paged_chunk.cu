@@ -26,7 +26,8 @@
 // 1000 tokens after 15,000, 32 heads of 128, four to a kv head (254 GFLOP): 452 us, 0.56 PFLOP/s of results and 1.12 of products, two thirds of the measured 1.68; the SM clock is at 1.4 GHz then,
 // by the power limit.  7 chunks of 700 with a window of 1024 and 4 sinks, heads of 64: 130 us; there each CTA has a tile of 10 key tiles, and its start and end count.
 //
-// Every wait is bounded; a wait that gives up raises the context's error word, and the kernel returns after freeing its tensor memory.
+// Every wait for a copy or a product is bounded; a wait that gives up raises the context's error word, and the kernel returns after freeing its tensor memory.  Barriers are only waited at where all
+// who take part come: a half's warps leave as one, the remaining warps meet nobody until the end.
 #include "paged_attention.cuh"
 #include "tensor_core.cuh"
 
@@ -97,6 +98,13 @@ __device__ __forceinline__ void pc_load(uint32_t taddr, uint32_t (&r)[16]) {
 __device__ __forceinline__ void pc_sync_half(uint32_t half) {
     if (half) asm volatile("bar.sync 2, 256;" ::: "memory");
     else asm volatile("bar.sync 1, 256;" ::: "memory");
+}
+// The same barrier; whether all threads of the half hold `ok`
+__device__ __forceinline__ bool pc_agree_half(uint32_t half, bool ok) {
+    uint32_t all;
+    if (half) asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"((uint32_t)ok) : "memory");
+    else asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"((uint32_t)ok) : "memory");
+    return all != 0;
 }
 
 // Bounded wait without a function call: ptxas does not keep a caller's registers beyond the launch's number across one
@@ -249,7 +257,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
             float m = -INFINITY, l = 0.f, alpha = 1.f;
             const volatile PagedWalk<PC_KT> &now = kept;   // (registers are short: what is read once per key tile is read from there)
             auto fold = [&]() {   // acc = alpha acc + O
-                if (!wait(bo, ps ^ 1, 12)) return;
+                if (!ok || !wait(bo, ps ^ 1, 12)) return;
                 pg_fence_after();
 #pragma unroll
                 for (int c = 0; c < (int)D / 32; c++) {
@@ -262,12 +270,14 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                 __syncwarp();
                 if (lane == 0) pg_arrive(bf);
             };
-            for (uint32_t i = 0; i < now.count && ok; i++) {
+            // Each warp sees for itself that a wait gave up, and one that left by itself would keep the others at the half's next barrier for ever.  So it goes on without waiting, with whatever tensor
+            // memory holds, and the half leaves as one behind its last key tile.
+            for (uint32_t i = 0; i < now.count; i++) {
                 if (i) fold();   // of the tile before: its products are done before this one's scores
                 const uint32_t unit = now.at + i, sink_tiles = now.span.sink_tiles;
                 const int32_t base = (int32_t)((unit < sink_tiles ? unit : now.span.first + unit - sink_tiles) * PC_KT + 64 * side);
                 const bool masked = base + 63 > *const_cast<volatile int32_t *>(&S.lo[half]) || (a.window && *const_cast<volatile int32_t *>(&S.hi[half]) - base >= a.window);
-                if (!ok || !wait(bs, ps, 12)) break;
+                if (ok) wait(bs, ps, 12);
                 ps ^= 1;
                 pg_fence_after();
                 uint64_t seen = ~0ull;   // which of its 64 columns the row sees: up to its own position, and of those the window's and the sinks
@@ -337,9 +347,11 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                 if (lane == 0) pg_arrive(bp);
                 alpha = alpha1;
             }
-            if (ok) fold();
+            fold();
+            S.x[half][side][row] = l;
+            ok = pc_agree_half(half, ok);   // (also: the kept walk is there)
             if (!ok) break;
-            l += other(l);   // (also: the kept walk is there)
+            l += S.x[half][side ^ 1][row];
             unpark();
 
             // ---- the half's result, or its part of it ----

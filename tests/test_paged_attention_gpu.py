@@ -333,3 +333,24 @@ def test_refusals(backend):
     refused("float16 or both float32", vc=b.vc.float())
     refused("contiguous pages", kc=b.kc.transpose(0, 1), vc=b.vc.transpose(0, 1))
     assert backend.lib.ib_paged_attention(backend.handle, None, None, None) == 1
+
+
+def gives_up(backend, hs):
+    """A launch whose waits are given 1 us, and rows whose results take milliseconds: every row sees an infinite value, which does each of them again element by element, while the tensor cores'
+    warps wait for the next tile's queries.  More query tiles than CTAs, so that most CTAs have a part of one, a whole one or more, and a part of another."""
+    b = Batch([3000], [4100], 16, 4, hs, P=64)
+    b.put(0, 5, 1, float("inf"))
+    backend.set_wait_limit(1000)
+    b.run(backend)
+    backend.set_wait_limit(2_000_000_000)
+    return backend.lib.ib_stream_sync(backend.handle, torch.cuda.current_stream().cuda_stream)
+
+
+@pytest.mark.parametrize("hs", [64, 128])
+def test_a_wait_that_gives_up_ends_the_launch(hs):
+    """Some warps of a CTA give up, others do not: the launch ends, and the next synchronising call says so, once."""
+    own = Backend(0)
+    assert gives_up(own, hs) == 5 and b"gave up waiting" in own.lib.ib_last_error_string()
+    torch.cuda.synchronize()
+    assert own.lib.ib_stream_sync(own.handle, torch.cuda.current_stream().cuda_stream) == 0
+    own.close()
