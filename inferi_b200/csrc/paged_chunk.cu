@@ -127,6 +127,20 @@ __device__ __forceinline__ bool pc_wait(uint32_t bar, uint32_t parity, const Pag
 // moves every operand of every MMA over by itself (70 clocks an MMA instead of 20).
 __device__ __forceinline__ uint32_t pc_uniform(uint32_t x) { return __reduce_or_sync(0xffffffffu, x); }
 
+// A half that gave up arrives at the tiles that it would still have had a part of, from the one that it was at on (it gives up before it arrives there): the counters are zero again when the launch
+// ends, whoever gave up, and launches that follow, replayed ones too, find their last arrivals where they are.  Called by a warp.
+static __device__ __noinline__ void pc_arrive_at_rest(const PagedAttn &a, const TileShape &shape, const PcShared &S, uint32_t half) {
+    PagedRange range = {};
+    range.total = S.range.sum[0];
+    range.length = S.range.sum[1];
+    PagedWalk<PC_KT> w = S.walk[half];
+    do {
+        if (w.whole() || (half == 1 && min(shape.tokens, w.q.n - w.tile * shape.tokens) * a.kv_mul <= 128)) continue;
+        const uint32_t c0 = range.range_of(w.tile_unit()), c1 = range.range_of(w.tile_unit() + w.span.units - 1);
+        if ((threadIdx.x & 31) == 0 && paged_arrive(a.counters + 2 * c0 + half) == c1 - c0) a.counters[2 * c0 + half] = 0u;
+    } while (w.next(a, shape));
+}
+
 struct PcMaps { CUtensorMap k, v; };
 
 template <int HS>
@@ -142,6 +156,8 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
     const PagedRange range = paged_range<PC_KT, PC_THREADS, true>(a, shape, S.range);
     if (range.total == 0 || blockIdx.x >= range.ranges) return;
     if (warp == 0 && lane == 0) {
+        S.range.sum[0] = range.total;   // (nobody reads these any more, but who leaves early)
+        S.range.sum[1] = range.length;
         for (uint32_t i = 0; i < SLOTS; i++) {
             pg_bar_init(b_full + 8 * i, 1);
             pg_bar_init(b_empty + 8 * i, 2);   // both MMA warps
@@ -576,6 +592,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
       }
     }
     if (!ok) {   // a wait gave up: copies and products of this CTA may still be in flight; give them time to land before the CTA ends
+        if (warp == 0 || warp == 8) pc_arrive_at_rest(a, shape, S, warp >> 3);
         const unsigned long long t0 = pg_ns();
         while (pg_ns() - t0 < 100000ull) {}
     }

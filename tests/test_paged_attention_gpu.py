@@ -336,11 +336,11 @@ def test_refusals(backend):
 
 
 def gives_up(backend, hs):
-    """A launch whose waits are given 1 us, and rows whose results take milliseconds: every row sees an infinite value, which does each of them again element by element, while the tensor cores'
-    warps wait for the next tile's queries.  More query tiles than CTAs, so that most CTAs have a part of one, a whole one or more, and a part of another."""
+    """A launch whose waits are given 0.3 ms, thirty times what they take otherwise, and rows whose results take milliseconds: every row sees an infinite value, which does each of them again element by
+    element, while the tensor cores' warps wait for the next tile's queries.  More query tiles than CTAs, so that most CTAs have a part of one, a whole one or more, and a part of another."""
     b = Batch([3000], [4100], 16, 4, hs, P=64)
     b.put(0, 5, 1, float("inf"))
-    backend.set_wait_limit(1000)
+    backend.set_wait_limit(300_000)
     b.run(backend)
     backend.set_wait_limit(2_000_000_000)
     return backend.lib.ib_stream_sync(backend.handle, torch.cuda.current_stream().cuda_stream)
@@ -354,3 +354,21 @@ def test_a_wait_that_gives_up_ends_the_launch(hs):
     torch.cuda.synchronize()
     assert own.lib.ib_stream_sync(own.handle, torch.cuda.current_stream().cuda_stream) == 0
     own.close()
+
+
+@pytest.mark.parametrize("hs", [64, 128])
+def test_a_wait_that_gave_up_leaves_no_arrivals_for_later_launches(hs):
+    """CTAs that gave up had parts of tiles left, whose other parts had arrived: later launches find counters that are zero, and merge what is there."""
+    own, fresh = Backend(0), Backend(0)
+    b = Batch([2900], [4100], 16, 4, hs, P=64, seed=2)
+    want = b.run(fresh).clone()
+    for _ in range(2):
+        assert gives_up(own, hs) == 5
+        for _ in range(3):
+            b.out.fill_(float("nan"))
+            assert torch.equal(b.run(own), want)
+    assert own.lib.ib_stream_sync(own.handle, torch.cuda.current_stream().cuda_stream) == 0
+    exact, tol = b.exact(0)
+    assert (want.double() - exact).abs().max() <= tol
+    own.close()
+    fresh.close()
