@@ -7,10 +7,10 @@
 //
 // Which token it is hangs on sums of up to half a million weights next to a border, and on a flat distribution the border is 1e-5 of the sum away.  So weights are whole numbers, in units
 // of 2^-44 of the largest, good to 3e-10 of themselves: (x - max) log2(e) / T is one product of doubles, added to 1.5 * 2^20 so that its whole and fractional parts
-// are words of the result; 2^fraction is a table of 256 and three steps of a series in 32-bit fixed point.  Sums of whole numbers do not depend on their order.  Weights below the histogram
-// (below) only matter as a sum, mostly: there ex2.approx of a product with a two-word constant will do.  Its errors of 2e-7 are each its own and vanish in the sum of thousands, but for
-// their mean of -5.1e-8 (measured over 6e7 normal logits: -5.05e-8 to -5.3e-8, whatever the spread, the temperature and the border), which is put right: 2e-9 of such a sum remain.
-// Where a border turns out to lie among them, the sums are formed anew from whole numbers (BS_EXACT).
+// are words of the result; 2^fraction is a table of 256 and three steps of a series in 32-bit fixed point.  Sums of whole numbers do not depend on their order.  Of a row with filters, the weights
+// below the histogram (below) mostly matter as one sum only, and that only to top_p's bound: there ex2.approx in 32 bits will do, with a bound on what their sum is off by (BS_LOOSE).  Where the element
+// that top_p's border falls on is the same with that much more and less, it is the one that the exact sum gives; where it is not, or the whole is what the coin is held against, the sums are formed anew
+// from whole numbers (BS_EXACT).  Rows without a filter have nothing but exact sums.
 //
 // A row is a thread-block cluster of up to 8 CTAs, each with a slice of the row in shared memory: one read of the row from HBM, and what follows passes over shared memory.  A warp goes over its
 // stretch of the slice once, adds up the small weights and lists the places of the others, which it takes together then (a few per cent of a language model's logits: with some of them
@@ -20,8 +20,8 @@
 // there, so that one list answers every question - are listed and sorted.  Bins too full for the list (ties) or below the histogram: the same by digits of x's order, to the last
 // tie in index order.  The first CTA of the cluster leads: it looks at the merged histogram and says what all do next (BsStep).  Its threads carry the same state and search sums by
 // bisection, each for itself, without barriers.
-// What bounds it, at 128,256 logits: a chain of barriers, scans and short lists for few rows (one row with top-p 38 us; 33 rows of 32,003 45 us); for many the passes over logits that
-// have left the caches and the arithmetic of the elements in the histogram: 250 rows 190 us with settings of every row's own; arg-max 32, no filter 100, top-k 50 124, top-p 0.9 228.
+// What bounds it, at 128,256 logits: a chain of barriers, scans and short lists for few rows (one row with top-p 36 us, without a filter 13; 33 rows of 32,003 44 us); for many the passes over logits that
+// have left the caches and the arithmetic of the elements in the histogram: 250 rows 173 us with settings of every row's own (one that takes BS_EXACT late lengthens that: 192 to 229 by the numbers drawn); all of them without a filter 111, top-k up to 200 163, top-p 0.5 to 0.99 259.
 #include "op_launch.cuh"
 
 #include <cooperative_groups.h>
@@ -36,9 +36,14 @@ constexpr uint32_t BS_THREADS = 512, BS_WARPS = BS_THREADS / 32, BS_CLUSTER = 8;
 constexpr uint32_t BS_BINS = 1024, BS_LIST = 1024;
 constexpr uint32_t BS_MAX_VOCAB = 1u << 19;   // S < 2^63
 constexpr int BS_ONE = 44;                    // the largest weight is 2^44 units
-// The histogram's reach below the largest weight, in factors of two, where no sample says better; of the elements that are taken one by one without a filter.  A border below it is looked for
-// in a second one, of the stretch behind the first.  (Normal logits of deviation 3.  One row, top-k 50, reach 11 or 16: 29 and 36 us.  No filter, 8 or 16: one row 20 and 25, 250 rows 100 and 174.)
-constexpr double BS_OCTAVES = 16.0, BS_OCTAVES_K = 11.0, BS_OCTAVES_SUM = 8.0;
+// The histogram's reach below the largest weight, in factors of two, where no sample says better.  A border below it is looked for in a second one, of the stretch behind the first.  (Normal logits of
+// deviation 3.  One row, top-k 50, reach 11 or 16: 29 and 36 us.)
+constexpr double BS_OCTAVES = 16.0, BS_OCTAVES_K = 11.0;
+// What a sum of small weights may be off by.  A weight t octaves below the largest: by 2^-24 t octaves in its difference and as many in its product with log2(e) / T, which is t 2^-23 ln 2 of it, by
+// ex2.approx's 2^-22, and eight of them are added up in 32 bits, 7 * 2^-24.  That is 2.64e-6 of it at 24 octaves, 4.4e-6 at 44, where a weight is a unit; those behind 24 octaves are below 2^20 units each, so
+// it is 4.6 units of each of them, and on the other side there is half a unit for every whole number.
+constexpr double BS_LOOSE = 2.7e-6;
+constexpr uint32_t BS_LOOSE_EACH = 6;
 constexpr uint32_t BS_WINDOWS = 4;                  // such stretches, at most
 // Vocabularies up to this size are one CTA's work, up to twice this size two CTAs' and so on: what a cluster's barriers cost is not less than what a small slice saves.  (Top-k 50, slices of 8192
 // or 4096 at most: one row of 8000 20 and 23 us, 33 rows of 32,003 25 and 35; 12,000 at most: the same, but top-p 0.9 of one row of 20,000 35 and 39.)
@@ -71,7 +76,7 @@ constexpr BsTable bs_make_table() {
 }
 __device__ const BsTable bs_table = bs_make_table();
 
-enum BsStep : uint32_t { BS_DONE, BS_HISTOGRAM, BS_EXACT, BS_DIGIT, BS_LIST_BINS, BS_LIST_DIGITS, BS_SEGMENT, BS_COUNT_TIES, BS_PICK_TIE };
+enum BsStep : uint32_t { BS_DONE, BS_HISTOGRAM, BS_EXACT, BS_DIGIT, BS_LIST_BINS, BS_LIST_DIGITS, BS_COUNT_TIES, BS_PICK_TIE };
 
 struct BsShared {
     uint32_t table[256];                                // 2^(i / 256), 31 fractional bits
@@ -92,11 +97,12 @@ struct BsShared {
         };
     };
     uint16_t kept[BS_WARPS][BS_KEPT];                   // places in its stretch of a warp's elements that are in the histogram
-    unsigned long long seg[BS_CLUSTER * BS_WARPS];      // first CTA: weight or count of every warp's stretch of the row
+    unsigned long long seg[BS_CLUSTER * BS_WARPS];      // weight of every warp's stretch of the row; in the first CTA, or a count
     unsigned long long red[2][BS_WARPS];
     float lo[BS_CLUSTER];                               // of every CTA's slice: its smallest finite logit
     unsigned long long best[BS_CLUSTER];                // ... and its arg-max
-    unsigned long long part_mass[BS_CLUSTER], part_min[BS_CLUSTER];   // first CTA: weight of each slice, of its elements with w >= min_p
+    unsigned long long loose[BS_WARPS];                 // of every warp's small weights: their sum in 32 bits
+    unsigned long long part_loose[BS_CLUSTER], part_min[BS_CLUSTER];   // first CTA: of each slice, its small weights, and its elements with w >= min_p
     uint32_t part_cnt[BS_CLUSTER], part_min_cnt[BS_CLUSTER];
     // what the first CTA says
     uint32_t step, a, b, prefix;
@@ -136,7 +142,7 @@ struct BsWeight {
         // 2^(r / 2^40) - 1 = z + z^2 / 2 + z^3 / 6, z = ln 2 * r / 2^40, times 2^40
         const uint32_t q = __umulhi(r, __umulhi(r, __umulhi(r, 3638u) + 4030416u) + 2977044472u);
         const uint32_t w = t + (__umulhi(t, q) >> 8);   // 31 fractional bits
-        return max((((unsigned long long)w << (BS_ONE - 30)) >> down) + 1ull >> 1, 1ull);
+        return (((unsigned long long)w << (BS_ONE - 30)) >> down) + 1ull >> 1;   // (1 at least: down is 44 at most)
     }
 };
 
@@ -298,11 +304,83 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
     // a warp's elements: a stretch of the slice
     const uint32_t stretch = ((len + BS_WARPS - 1) / BS_WARPS + 31) & ~31u, w0 = min(len, warp * stretch), w1 = min(len, w0 + stretch);
 
+    auto scaled = [](float f, unsigned long long m) { return f > 0.f ? min((unsigned long long)((double)f * (double)m), m - 1) : 0ull; };   // f < 1
+    auto exact_sums = [&]() {   // of the warp's stretch, for every CTA
+        unsigned long long sum = 0ull;
+        sweep(w1 - w0, [&](uint32_t k) { return w0 + k; }, [&](uint32_t, float x) { sum += weight(x, S.table); });
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane < C) cluster.map_shared_rank(&S, lane)->seg[rank * BS_WARPS + warp] = sum;
+    };
+
+    // ---- a row without a filter: index order ----
+    if (!filtered) {
+        exact_sums();
+        barrier();
+        // every warp finds the stretch of the crossing, from four sums a lane
+        constexpr uint32_t E = BS_CLUSTER * BS_WARPS / 32;
+        unsigned long long seg[E], upto = 0ull;
+#pragma unroll
+        for (uint32_t e = 0; e < E; e++) {
+            seg[e] = E * lane + e < C * BS_WARPS ? S.seg[E * lane + e] : 0ull;
+            upto += seg[e];
+        }
+        unsigned long long ahead = upto;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long t = __shfl_up_sync(0xffffffffu, upto, o);
+            if ((int)lane >= o) upto += t;
+        }
+        ahead = upto - ahead;
+        const unsigned long long total = __shfl_sync(0xffffffffu, upto, 31), bound = scaled(coin, total);
+        uint32_t s = 0;
+        for (; s + 1 < E && bound >= ahead + seg[s]; s++) ahead += seg[s];
+        const int who = __ffs(__ballot_sync(0xffffffffu, bound < upto)) - 1;
+        s = __shfl_sync(0xffffffffu, E * lane + s, who);
+        ahead = __shfl_sync(0xffffffffu, ahead, who);
+        if (rank == s / BS_WARPS) {
+            // The CTA's warps share that stretch; the one whose part the crossing is in goes through it element by element.
+            const uint32_t o = s % BS_WARPS, s0 = min(len, o * stretch), s1 = min(len, s0 + stretch), part = ((s1 - s0 + BS_WARPS - 1) / BS_WARPS + 31) & ~31u;
+            const uint32_t p0 = min(s1, s0 + warp * part), p1 = min(s1, p0 + part);
+            unsigned long long sum = 0ull, left = bound - ahead;
+            sweep(p1 - p0, [&](uint32_t k) { return p0 + k; }, [&](uint32_t, float x) { sum += weight(x, S.table); });
+#pragma unroll
+            for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            if (lane == 0) S.red[0][warp] = sum;
+            __syncthreads();
+            uint32_t mine = 0;
+            while (mine + 1 < BS_WARPS && left >= S.red[0][mine]) left -= S.red[0][mine++];
+            if (warp == mine) {
+                bool found = false;
+                sweep(p1 - p0, [&](uint32_t k) { return p0 + k; }, [&](uint32_t i, float x) {
+                    if (found) return;
+                    const unsigned long long w = weight(x, S.table), all = bs_sum(w);
+                    found = left < all;
+                    if (!found) {
+                        left -= all;
+                        return;
+                    }
+                    unsigned long long run = w;
+#pragma unroll
+                    for (int d = 1; d < 32; d <<= 1) {
+                        const unsigned long long t = __shfl_up_sync(0xffffffffu, run, d);
+                        if ((int)lane >= d) run += t;
+                    }
+                    if ((int)lane == __ffs(__ballot_sync(0xffffffffu, left < run)) - 1) {
+                        p.token[row] = (int32_t)(i0 + i);
+                        if (p.prob) p.prob[row] = (float)((double)w / (double)total);
+                    }
+                });
+            }
+        }
+        return;   // nobody reads another CTA's memory from here on
+    }
+
     // ---- what a step does ----
     // bins of x: equal stretches down from the largest logit
     // As far as the borders, if that can be told: min_p says so itself; where rank k or the mass top_p lies is seen from some of the row's logits, by half octaves.
     // (Every CTA of the row takes the same ones.  A border behind the reach costs another histogram, no more.)
-    double octaves = filtered ? (by_k ? BS_OCTAVES_K : BS_OCTAVES) : BS_OCTAVES_SUM;
+    double octaves = by_k ? BS_OCTAVES_K : BS_OCTAVES;
     if (p.sampled && (by_k || by_p)) {
         octaves = BS_OCTAVES;
         constexpr uint32_t HALVES = 64, E = BS_SAMPLE / BS_THREADS;
@@ -397,15 +475,15 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
         }
     };
 
-    // ---- the weights: sums of every stretch and slice, and for filtered rows the histogram ----
-    if (filtered) clear();
+    // ---- the weights: sums of every stretch and slice, and the histogram ----
     const unsigned long long least = by_min ? (min_p > 1.f ? (1ull << BS_ONE) + 1 : (unsigned long long)ceil((double)min_p * (double)(1ull << BS_ONE))) : 0ull;
     // elements that are looked at one by one: those of the histogram (and a little more), and what may reach min_p (a factor of two more: rounding)
-    const float near = fmaxf(per_bin > 0.f ? reach * (1.f + 0x1p-18f) : INFINITY, by_min ? (float)((1.0 - log2((double)fmaxf(min_p, 1e-30f))) / weight.c) : 0.f);
+    const float near = fmaxf(per_bin > 0.f && weight.c < (double)FLT_MAX ? reach * (1.f + 0x1p-18f) : INFINITY, by_min ? (float)((1.0 - log2((double)fmaxf(min_p, 1e-30f))) / weight.c) : 0.f);
     const float c_hi = (float)weight.c, c_lo = (float)(weight.c - (double)c_hi);
     uint32_t n_places = 0;      // the warp's kept places
     bool all_kept = true;     // they are those of all of its elements of the histogram
     {
+        clear();
         unsigned long long sum = 0ull, above = 0ull;
         uint32_t n = 0u, n_above = 0u, waiting = 0u;
         double small = 0.0;
@@ -444,7 +522,6 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
                 for (uint32_t e = 0; e < K; e++) {
                     sum += w[e];
                     if (by_min && w[e] >= least) { above += w[e]; n_above++; }
-                    if (!filtered) continue;
                     const bool in = bin[e] < BS_BINS;
                     if (in) add(bin[e], w[e]);
                     const uint32_t stay = __ballot_sync(0xffffffffu, in);
@@ -498,23 +575,27 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
             some(whole + lane, x);
         }
         take();
-        sum += (unsigned long long)(small * ((double)(1ull << BS_ONE) * (1.0 + 5.1e-8)));
+        unsigned long long loose = (unsigned long long)(small * (double)(1ull << BS_ONE));   // (one of them is a unit at least)
+        sum += loose;
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
             sum += __shfl_xor_sync(0xffffffffu, sum, o);
             above += __shfl_xor_sync(0xffffffffu, above, o);
+            loose += __shfl_xor_sync(0xffffffffu, loose, o);
             n += __shfl_xor_sync(0xffffffffu, n, o);
             n_above += __shfl_xor_sync(0xffffffffu, n_above, o);
         }
         if (lane == 0) {
             L.seg[rank * BS_WARPS + warp] = sum;
+            S.loose[warp] = loose;
             S.red[0][warp] = above;
             S.red[1][warp] = (unsigned long long)n << 32 | n_above;
         }
         __syncthreads();
         if (tid == 0) {
-            unsigned long long a = 0ull, c = 0ull;
-            for (uint32_t w = 0; w < BS_WARPS; w++) { a += S.red[0][w]; c += S.red[1][w]; }
+            unsigned long long a = 0ull, c = 0ull, l = 0ull;
+            for (uint32_t w = 0; w < BS_WARPS; w++) { a += S.red[0][w]; c += S.red[1][w]; l += S.loose[w]; }
+            L.part_loose[rank] = l;
             L.part_min[rank] = a;
             L.part_min_cnt[rank] = (uint32_t)c;
             L.part_cnt[rank] = (uint32_t)(c >> 32);
@@ -522,22 +603,23 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
     }
 
     // ---- the first CTA leads ----
-    // Every one of its threads carries the same state; the questions: 0 the k-th element, 1 top_p's, 2 the coin's.
-    unsigned long long total = 0ull, kept = 0ull, n_kept = 0ull, S_k = 0ull, bound = 0ull, base = 0ull, n_base = 0ull, n_min = 0ull, S_min = 0ull, there = 0ull;
+    // Every one of its threads carries the same state; the questions: 0 the k-th element, 1 top_p's, 2 the coin's (3: one whose answer hangs on what
+    // the sums are off by).
+    unsigned long long kept = 0ull, n_kept = 0ull, bound = 0ull, base = 0ull, n_base = 0ull, n_min = 0ull, S_min = 0ull, there = 0ull, loose = 0ull;   // kept: what is left so far
     uint32_t question = 0, list_lo = 1, list_hi = 0, list_n = 0, shift = 32, prefix = 0;   // the list: bins list_lo .. list_hi
     bool histogram = true, exact = false;   // tot_* are those of the bins of x; the sums are those of whole numbers
     unsigned long long list_mass = 0ull, list_cnt = 0ull;   // ahead of the list
     unsigned long long win_mass = 0ull, win_cnt = 0ull;     // ahead of the window
     auto add_up = [&]() {
-        total = 0ull;
-        for (uint32_t s = lane; s < C * BS_WARPS; s += 32) total += S.seg[s];
+        kept = 0ull;
+        for (uint32_t s = lane; s < C * BS_WARPS; s += 32) kept += S.seg[s];
 #pragma unroll
-        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        kept = S_k = total;
+        for (int o = 16; o; o >>= 1) kept += __shfl_xor_sync(0xffffffffu, kept, o);
         n_kept = p.n;
         question = 0;
     };
-    auto scaled = [](float f, unsigned long long m) { return f > 0.f ? min((unsigned long long)((double)f * (double)m), m - 1) : 0ull; };   // f < 1
+    // what `kept` may be off by: while it is the sum of all, and that is not of whole numbers
+    auto slack = [&]() { return exact || n_kept != p.n ? 0ull : loose; };
     auto say = [&](uint32_t step, uint32_t a, uint32_t b, uint32_t pre, unsigned long long arg) {
         if (tid == 0) { S.step = step; S.a = a; S.b = b; S.prefix = pre; S.arg = arg; }
     };
@@ -550,22 +632,26 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
                 return;
             }
             if (question == 1 && by_p) {
-                bound = scaled(top_p, S_k);
+                const unsigned long long off = slack();
+                bound = scaled(top_p, kept - off);   // (the least that it can be)
                 if (by_min && n_min && bound >= S_min) continue;   // min_p leaves less
+                if (by_min && n_min && off && scaled(top_p, kept + off) >= S_min) question = 3;
                 return;
             }
             if (question == 2) {
                 if (by_min && n_min < n_kept) { n_kept = max(n_min, 1ull); kept = n_min ? S_min : 1ull << BS_ONE; }
                 bound = scaled(coin, kept);
+                if (slack()) question = 3;
                 return;
             }
         }
     };
     // What the answer - the element `key` with running weight and count through it - means; true: the row is done
     auto answered = [&](unsigned long long key, unsigned long long sum, unsigned long long cnt) {
-        if (question == 0) { S_k = kept = sum; n_kept = cnt; }
-        else if (question == 1) { kept = sum; n_kept = cnt; }
-        else {
+        if (question < 2) {
+            kept = sum;
+            n_kept = cnt;
+        } else {
             if (tid == 0) {
                 p.token[row] = (int32_t)(uint32_t)key;
                 if (p.prob) p.prob[row] = (float)((double)weight(bs_value(~(uint32_t)(key >> 32)), S.table) / (double)kept);
@@ -599,6 +685,13 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
                 const uint32_t mid = (lo + hi) >> 1;
                 if (bound < list_mass + S.run[mid]) hi = mid; else lo = mid + 1;
             }
+        if (question == 1) {
+            const unsigned long long off = slack();
+            if (off && scaled(top_p, kept + off) >= list_mass + S.run[lo]) {   // (with the most that the bound can be it is not this element)
+                question = 3;
+                return false;
+            }
+        }
         return answered(S.list[lo], list_mass + S.run[lo], list_cnt + lo + 1);
     };
     // Goes on until the cluster is needed; says what for.
@@ -634,12 +727,9 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
             answered(0ull, base + (th + 1) * w, n_base + th + 1);   // (which one it is does not matter to the sums)
         }
         while (!done) {
-            ask();
-            if (!filtered) {   // index order: the stretch of the crossing
-                unsigned long long ahead = 0ull;
-                uint32_t s = 0;
-                while (s + 1 < C * BS_WARPS && bound >= ahead + S.seg[s]) ahead += S.seg[s++];
-                say(BS_SEGMENT, s, 0, 0, bound - ahead);
+            if (question < 3) ask();
+            if (question == 3) {
+                say(BS_EXACT, 0, 0, 0, 0);
                 return;
             }
             const unsigned long long ahead = by_count() ? win_cnt : win_mass;
@@ -708,22 +798,25 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
     };
 
     // (Every part of this stands here once: code that runs once costs 12 clocks an instruction, and a row comes through here a few times only.)
-    bool merging = filtered;
+    bool merging = true;
 #pragma unroll 1
     for (bool first = true;; first = false) {
         if (merging) merge();
-        else if (first || last == BS_EXACT || last == BS_COUNT_TIES) barrier();   // the stretches' sums are there
+        else if (last == BS_EXACT || last == BS_COUNT_TIES) barrier();   // the stretches' sums are there
         if (rank == 0) {
             if (first || last == BS_EXACT) {
                 add_up();
                 exact = !first;
             }
-            if (first)
+            if (first) {
                 for (uint32_t r = 0; r < C; r++) {
                     n_min += S.part_min_cnt[r];
                     S_min += S.part_min[r];
                     there += S.part_cnt[r];
+                    loose += S.part_loose[r];
                 }
+                if (loose) loose = (unsigned long long)((double)loose * BS_LOOSE) + BS_LOOSE_EACH * p.n + C * BS_THREADS;   // (a thread makes a whole number of its sum)
+            }
             if (last == BS_LIST_BINS || last == BS_LIST_DIGITS) sorted();
             lead();
         }
@@ -749,11 +842,7 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
                 if (x > -INFINITY && (histogram ? bin < BS_BINS : a == 32 || order >> a == pre)) add(bin, weight(x, S.table));
             });
         } else if (step == BS_EXACT) {   // the stretches' sums from whole numbers; then all questions again
-            unsigned long long sum = 0ull;
-            sweep(w1 - w0, [&](uint32_t k) { return w0 + k; }, [&](uint32_t, float x) { sum += weight(x, S.table); });
-#pragma unroll
-            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (lane == 0) L.seg[rank * BS_WARPS + warp] = sum;
+            exact_sums();
         } else if (step == BS_LIST_BINS || step == BS_LIST_DIGITS) {
             // into this CTA's own list, a place for every warp's elements together; the first CTA fetches them from all
             if (tid == 0) S.listed = 0;
@@ -790,60 +879,6 @@ __global__ void __launch_bounds__(BS_THREADS, 2) batch_sample_kernel(const __gri
                 if (tid == 0) S.listed = min(all, BS_LIST);
                 __syncthreads();
             }
-        } else if (step == BS_SEGMENT) {   // index order: the element of warp a's stretch at which the running weight exceeds arg
-            // The CTA's warps share that stretch; the one whose part the crossing is in goes through it element by element.
-            if (rank == a / BS_WARPS) {
-                const uint32_t o = a % BS_WARPS, s0 = min(len, o * stretch), s1 = min(len, s0 + stretch), part = ((s1 - s0 + BS_WARPS - 1) / BS_WARPS + 31) & ~31u;
-                const uint32_t p0 = min(s1, s0 + warp * part), p1 = min(s1, p0 + part);
-                unsigned long long sum = 0ull;
-                sweep(p1 - p0, [&](uint32_t k) { return p0 + k; }, [&](uint32_t, float x) { sum += weight(x, S.table); });
-#pragma unroll
-                for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-                if (lane == 0) S.red[0][warp] = sum;
-                __syncthreads();
-                uint32_t mine = BS_WARPS;   // the part of the crossing; (rounding of the small weights: perhaps none, then the last with a weight)
-                unsigned long long left = arg, ahead = 0ull;
-                for (uint32_t k = 0; k < BS_WARPS; k++) {
-                    const unsigned long long m = S.red[0][k];
-                    if (m && (mine == BS_WARPS || arg >= ahead)) { mine = k; left = arg - ahead; }
-                    ahead += m;
-                }
-                if (warp == mine || (mine == BS_WARPS && warp == 0)) {
-                    uint32_t at = i0 + s0;
-                    unsigned long long at_w = 0ull;
-                    bool found = false;
-                    sweep(p1 - p0, [&](uint32_t k) { return p0 + k; }, [&](uint32_t i, float x) {
-                        if (found) return;
-                        const unsigned long long w = weight(x, S.table), all = bs_sum(w);
-                        found = left < all;
-                        const uint32_t some = __ballot_sync(0xffffffffu, w != 0ull);
-                        if (found || some) {
-                            int l = 31 - __clz(some);
-                            if (found) {
-                                unsigned long long run = w;
-#pragma unroll
-                                for (int d = 1; d < 32; d <<= 1) {
-                                    const unsigned long long t = __shfl_up_sync(0xffffffffu, run, d);
-                                    if ((int)lane >= d) run += t;
-                                }
-                                l = __ffs(__ballot_sync(0xffffffffu, left < run)) - 1;
-                            }
-                            at = i0 + __shfl_sync(0xffffffffu, i, l);
-                            at_w = __shfl_sync(0xffffffffu, w, l);
-                        }
-                        left -= all;
-                    });
-                    unsigned long long all = 0ull;
-                    for (uint32_t s = lane; s < C * BS_WARPS; s += 32) all += L.seg[s];
-#pragma unroll
-                    for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
-                    if (lane == 0) {
-                        p.token[row] = (int32_t)at;
-                        if (p.prob) p.prob[row] = (float)((double)at_w / (double)all);
-                    }
-                }
-            }
-            break;
         } else if (step == BS_COUNT_TIES) {   // more equal elements than the list holds: how many in every stretch
             uint32_t n = 0;
             for (uint32_t i = w0 + lane; i < w1; i += 32) n += ~bs_order(logit(i)) == pre;

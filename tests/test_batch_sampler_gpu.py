@@ -285,3 +285,94 @@ def test_odd_rows_among_many(backend, rows, vocab):
             want, p = choose(x[r], float(T[r]), top_k[r] if top_k else 0, top_p[r] if top_p else 1.0, min_p[r] if min_p else 0.0, coin[r])
             assert tokens[r] == want, (r, tokens[r], want)
             assert abs(probs[r] - p) <= p * (2**-24 + 2**-29) + vocab * 2**-44, (r, probs[r], p)
+
+
+def tails(vocab, rows, seed):
+    """Rows whose largest logits stand before a tail of equal values, or of few different ones, which has a part of the mass that is not small: what each of its weights is off by adds up."""
+    rng = np.random.default_rng(seed)
+    out = np.empty((rows, vocab), dtype=np.float32)
+    down = math.log(vocab)   # a tail that far down weighs as much as the largest
+    for r in range(rows):
+        kind, share = r % 5, rng.uniform(-2.5, 1.5)
+        if kind == 0:     # one value that takes rounding in every step
+            tail = np.full(vocab, -(down + share) * 1.0123456789)
+        elif kind == 1:   # few values
+            tail = -(down + share) + rng.integers(0, 5, vocab) * 0.30103
+        elif kind == 2:   # what a model in bf16 or f16 gives
+            tail = torch.from_numpy(-(down + share) + rng.standard_normal(vocab)).to((torch.bfloat16, torch.float16)[r // 5 % 2]).double().numpy()
+        elif kind == 3:   # all of it moved: the difference of two logits is rounded
+            tail = np.full(vocab, -(down + share))
+        else:
+            tail = np.where(rng.random(vocab) < 0.5, -(down + share), -(down + share) - 7.7)
+        x = tail.astype(np.float32)
+        x[rng.integers(0, vocab, 1 + r % 3)] = 0.0
+        out[r] = x + np.float32(20.3 if kind == 3 else 0.0)
+    out[0] = -13.65625
+    out[0, vocab // 7] = 0.0
+    return torch.from_numpy(out).cuda()
+
+
+def choices(x, T, k, top_p, min_p, coin, near):
+    """`choose`, and what else may come out where a bound is up to `near` of the sum off."""
+    x = x.astype(np.float64)
+    w = np.exp((x - x.max()) / float(np.float32(T)))
+    n = len(x)
+    by_k, by_p, by_min = 0 < k < n, 0 < top_p < 1, min_p > 0
+    order = np.lexsort((np.arange(n), -x)) if by_k or by_p or by_min else np.arange(n)
+    w = w[order]
+    least = max(1, int((w >= float(np.float32(min_p))).sum())) if by_min else n
+    top, sums, out = k if by_k else n, np.cumsum(w), []
+    for off in (-near, 0.0, near) if by_p else (0.0,):
+        m = min(top, least, int(np.searchsorted(sums[:top], (float(np.float32(top_p)) + off) * sums[top - 1], side="right")) + 1 if by_p else n)
+        for c in (-near, 0.0, near):
+            at = min(int(np.searchsorted(sums[:m], (float(np.float32(coin)) + c) * sums[m - 1], side="right")), m - 1)
+            out.append((int(order[at]), float(w[at] / sums[m - 1])))
+    return out
+
+
+def check_near(backend, logits, T, k, top_p, min_p, coin):
+    """`check`, but where a coin or a top_p is so near to a border that the units decide, the token on either side of it will do; returns how many rows were decided.  A sum is off by half a
+    unit and 2^-31 of itself per token, and so is the whole."""
+    tokens, probs = run(backend, logits, T, k, top_p, min_p, coin)
+    x, decided = logits.cpu().numpy(), 0
+    for r in range(len(tokens)):
+        may = choices(x[r], T[r], k[r] if k else 0, top_p[r] if top_p else 1.0, min_p[r] if min_p else 0.0, coin[r], logits.shape[1] * 2.0**-44 + 2.0**-30)
+        assert any(tokens[r] == t and abs(probs[r] - p) <= p * (2**-24 + 2**-29) + x.shape[1] * 2**-44 for t, p in may), (r, tokens[r], probs[r], may, T[r], k and k[r], top_p and top_p[r], coin[r])
+        decided += len({t for t, _ in may}) == 1
+    return decided
+
+
+@pytest.mark.parametrize("rows, vocab", [(3, 100000), (40, 100000), (24, 9000), (60, 32003), (300, 50000), (16, 524288)])
+def test_tails_of_equal_logits(backend, rows, vocab):
+    logits = tails(vocab, rows, vocab + rows)
+    rng = np.random.default_rng(rows)
+    coin = (1.0 - rng.random(rows) * 0.3).astype(np.float32).clip(max=1 - 2**-24).tolist()   # mostly in the tail, where the order is that of probabilities
+    T = [1.0] * rows
+    decided = []
+    for _ in range(3):
+        decided += [check_near(backend, logits, T, None, None, None, rng.random(rows).astype(np.float32).tolist())]
+    decided += [check_near(backend, logits, T, None, (0.5 + 0.499 * rng.random(rows)).tolist(), None, coin)]
+    decided += [check_near(backend, logits, T, [vocab - 1] * rows, (0.5 + 0.499 * rng.random(rows)).tolist(), None, coin)]
+    decided += [check_near(backend, logits, T, None, [0.97] * rows, [1e-9] * rows, coin)]
+    decided += [check_near(backend, logits, T, None, None, [1e-12] * rows, coin)]
+    decided += [check_near(backend, logits, (0.8 + 0.4 * rng.random(rows)).astype(np.float32).tolist(), [0, vocab // 2] * (rows // 2) + [0] * (rows % 2), (0.9 + 0.0999 * rng.random(rows)).tolist(), None, coin)]
+    assert sum(decided) >= 0.6 * rows * len(decided)   # (half a million tokens are some 3e-7 of the sum apart, at least, and the bounds 6e-8 wide)
+
+
+def test_a_top_p_next_to_a_border(backend):
+    """top_p and the coin so near to a border that the whole has to be known to a part in 10^8: on either side of it."""
+    vocab, rows = 40000, 32
+    logits = torch.randn(rows, vocab, generator=torch.Generator(device="cuda").manual_seed(11), device="cuda").mul_(2.0).bfloat16().float()
+    x = logits.cpu().numpy().astype(np.float64)
+    top_p, coin = [], []
+    for r in range(rows):
+        w = np.sort(np.exp(x[r] - x[r].max()))[::-1]
+        sums = np.cumsum(w)
+        at = 200 + 37 * r                                   # that many tokens are left, or one more
+        p = np.float32(sums[at - 1] / sums[-1])
+        while abs(float(p) - sums[at - 1] / sums[-1]) < 3e-9:   # (not on the border itself)
+            p = np.nextafter(p, np.float32(2))
+        top_p.append(float(p))
+        coin.append(1 - 2**-24)
+    check(backend, logits, [1.0] * rows, None, top_p, None, coin)
+    check(backend, logits, [1.0] * rows, None, [float(np.nextafter(np.float32(p), np.float32(0))) for p in top_p], None, coin)
