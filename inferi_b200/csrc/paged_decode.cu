@@ -325,14 +325,15 @@ __global__ void __launch_bounds__(PD_THREADS, PD_CTAS_PER_SM) paged_decode_kerne
             const bool store = rt < tokens && rg < heads;
             const uint64_t q_row = w.q.start + t0 + rt;
             float *out = a.out + q_row * a.out_stride + (uint64_t)(head0 + rg) * HS;
+            const bool sees = p_lo + (int32_t)rt >= 0;   // (a token ahead of the first position sees nothing: 0, whatever the tile's values are)
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             bool odd = false;
 #pragma unroll
             for (int i = 0; i < D; i++) {
-                y[i] *= inv;
+                y[i] = sees ? y[i] * inv : 0.f;
                 odd |= !isfinite(y[i]);
             }
-            odd = odd && isfinite(sum);
+            odd = odd && sees && isfinite(sum);
             if (store) {
                 if (a.vec)
 #pragma unroll

@@ -372,3 +372,18 @@ def test_a_wait_that_gave_up_leaves_no_arrivals_for_later_launches(hs):
     assert (want.double() - exact).abs().max() <= tol
     own.close()
     fresh.close()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("hs", [64, 128])
+@pytest.mark.parametrize("new,kv", [(3, 2), (6, 2), (40, 11), (300, 290), (300, 1)])
+def test_rows_that_see_nothing_beside_values_that_are_no_numbers(backend, hs, new, kv, dtype):
+    """Tokens ahead of position 0 get 0, also where rows of K and V that the tile's other tokens see hold anything."""
+    b = Batch([0], [new], 8, 4, hs, dtype=dtype, seed=new)
+    b.put(0, 0, 1, float("nan"))
+    b.put(0, kv - 1, 1, float("inf"))
+    b.put(0, kv - 1, 0, float("nan"))
+    b.kv_len = i32([kv])
+    b.out.fill_(5.0)
+    b.run(backend)
+    assert (b.out[: new - kv] == 0).all() and torch.isnan(b.out[new - kv:]).all()
