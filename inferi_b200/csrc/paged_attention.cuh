@@ -330,40 +330,74 @@ __device__ __forceinline__ int paged_exponent(float most) {
 
 // ---- rows that hold something that is not a finite number ----
 // A masked position's weight is 0, but 0 times an infinity or NaN in its row of V is not, and the tiles' products run over all of a tile's positions (those that no
-// row of the tile sees are zeroed on their way); a weight's remainder may be 0 or negative where the weight is not.  So a row with such a result is computed anew, position by position, with
-// the row's largest score (rounded up, in units of log2) known - unless its sum of weights is none either: then it sees a key, or is a query, that is none, and all of the row is rightly
-// so.  Called by a whole warp.
+// row of the tile sees are zeroed on their way); a weight's remainder may be 0 or negative where the weight is not.  And q's two operands times an infinity in K are infinities of either sign, whose sum is
+// NaN where the score is an infinity.  So a row that sees something and has such a result, or no sum of weights, is computed anew, position by position and in one product each: a score of -infinity weighs
+// nothing, one that is NaN or infinity makes all of the row NaN, and so do scores that are all -infinity.
+// most: the row's largest score (rounded up, in units of log2), -infinity where the sum of weights says that it is not known.  Called by a whole warp.
 template <typename T>
 static __device__ __noinline__ void paged_repair(const PagedAttn &a, uint32_t KT, uint32_t request, uint32_t kv_head, const KeySpan span, int32_t p, float most, const float *q, float *out, uint32_t hs) {
     const uint32_t lane = threadIdx.x & 31, E = hs / 32;
     const float scale = 1.4426950408889634f / sqrtf((float)hs);
-    float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t u = 0; u < span.units; u++)
-        for (uint32_t j0 = key_tile(span, u) * KT; j0 < min(key_tile(span, u) * KT + KT, span.end); j0 += 32) {
-            // a lane's position: its weight, then everybody's elements of all 32
-            const uint32_t j = j0 + lane;
-            uint64_t at = ~0ull;
-            float x = 0.f;
-            if (j < span.end && paged_sees(a, p, j)) {
-                const int32_t page = a.table[(size_t)request * a.max_pages + (j >> a.page_log2)];
-                if (page >= 0 && (uint32_t)page < a.n_pages) {
-                    at = (uint64_t)page * a.page_stride + (uint64_t)(j & ((1u << a.page_log2) - 1)) * a.kv_dim + kv_head * hs;
-                    const T *k = static_cast<const T *>(a.k) + at;
-                    float s = 0.f;
-#pragma unroll 8
-                    for (uint32_t e = 0; e < hs; e++) s += q[e] * (float)k[e];
-                    x = fmaxf(paged_ex2(s * scale - most), 1e-38f);   // (not nothing: an infinity that is seen counts, however small its weight)
-                }
-            }
-#pragma unroll 4
-            for (int i = 0; i < 32; i++) {
-                const uint64_t from = __shfl_sync(0xffffffffu, at, i);
-                const float y = __shfl_sync(0xffffffffu, x, i);
-                if (from == ~0ull) continue;
-                l += y;
-                for (uint32_t e = 0; e < E; e++) acc[e] += y * (float)static_cast<const T *>(a.v)[from + lane + 32 * e];
-            }
+    // a position's row of the cache, or ~0 where it is not seen; its score
+    auto place = [&](uint32_t j) {
+        if (j >= span.end || !paged_sees(a, p, j)) return ~0ull;
+        const int32_t page = a.table[(size_t)request * a.max_pages + (j >> a.page_log2)];
+        if (page < 0 || (uint32_t)page >= a.n_pages) return ~0ull;
+        return (unsigned long long)page * a.page_stride + (unsigned long long)(j & ((1u << a.page_log2) - 1)) * a.kv_dim + kv_head * hs;
+    };
+    auto score = [&](unsigned long long at) {
+        constexpr uint32_t N = 16 / sizeof(T);
+        float s = 0.f;
+#pragma unroll 2
+        for (uint32_t e = 0; e < hs; e += N) {
+            const uint4 piece = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.k) + at + e));
+            const T *k = reinterpret_cast<const T *>(&piece);
+#pragma unroll
+            for (uint32_t i = 0; i < N; i++) s += q[e + i] * (float)k[i];
         }
+        return s;
+    };
+    auto positions = [&](auto body) {   // a lane's in turn; false: enough
+        for (uint32_t u = 0; u < span.units; u++)
+            for (uint32_t j0 = key_tile(span, u) * KT; j0 < min(key_tile(span, u) * KT + KT, span.end); j0 += 32)
+                if (!body(place(j0 + lane))) return;
+    };
+    if (most == -INFINITY) {
+        float top = -INFINITY;
+        bool some = false, none = false;   // sees something; has a score that is none
+        positions([&](unsigned long long at) {
+            const float s = at != ~0ull ? score(at) : -INFINITY;
+            some = some || at != ~0ull;
+            none = __any_sync(0xffffffffu, !(s < INFINITY));
+            top = fmaxf(top, s);
+            return !none;
+        });
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        some = __any_sync(0xffffffffu, some);
+        if (none || top == -INFINITY) {
+            for (uint32_t e = 0; e < E; e++) out[lane + 32 * e] = some ? NAN : 0.f;   // (nothing: pages outside the cache)
+            return;
+        }
+        most = ceilf(top * scale);
+    }
+    float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    positions([&](unsigned long long at) {   // its weight, then everybody's elements of all 32
+        float x = 0.f;
+        if (at != ~0ull) {
+            const float s = score(at);
+            x = s == -INFINITY ? 0.f : fmaxf(paged_ex2(s * scale - most), 1e-38f);   // (not nothing: an infinity that is seen counts, however small its weight)
+        }
+#pragma unroll 4
+        for (int i = 0; i < 32; i++) {
+            const unsigned long long from = __shfl_sync(0xffffffffu, at, i);
+            const float y = __shfl_sync(0xffffffffu, x, i);
+            if (from == ~0ull) continue;
+            l += y;
+            for (uint32_t e = 0; e < E; e++) acc[e] += y * (float)static_cast<const T *>(a.v)[from + lane + 32 * e];
+        }
+        return true;
+    });
     for (uint32_t e = 0; e < E; e++) out[lane + 32 * e] = acc[e] / l;
 }
 

@@ -408,15 +408,16 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                 // through q's place in shared memory, from which warps store whole rows; column c of row r lies at c ^ (r % 32)
                 float *rows = reinterpret_cast<float *>(smem + half * 2 * HALF);
                 const bool sees = p >= 0;   // (a token ahead of the first position sees nothing: 0, whatever the tile's values are)
-                const float inv = l == 0.f ? 0.f : 1.f / l;
-                bool odd = false;
+                const float inv = 1.f / l;
+                bool odd = !(l > 0.f);
+                if (odd) m = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < (int)D; i++) {
                     const float y = sees ? acc[i] * inv : 0.f;
                     odd |= !isfinite(y);
                     rows[row * HS + ((D * side + i) ^ (row & 31))] = y;
                 }
-                const uint32_t mine = __ballot_sync(0xffffffffu, odd && sees && isfinite(l));
+                const uint32_t mine = __ballot_sync(0xffffffffu, odd && sees);
                 if (lane == 0) S.odd[half][side][warp & 3] = mine;
                 pc_sync_half(half);
 #pragma unroll 4

@@ -326,14 +326,15 @@ __global__ void __launch_bounds__(PD_THREADS, PD_CTAS_PER_SM) paged_decode_kerne
             const uint64_t q_row = w.q.start + t0 + rt;
             float *out = a.out + q_row * a.out_stride + (uint64_t)(head0 + rg) * HS;
             const bool sees = p_lo + (int32_t)rt >= 0;   // (a token ahead of the first position sees nothing: 0, whatever the tile's values are)
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            bool odd = false;
+            const float inv = 1.f / sum;
+            bool odd = !(sum > 0.f);
 #pragma unroll
             for (int i = 0; i < D; i++) {
                 y[i] = sees ? y[i] * inv : 0.f;
                 odd |= !isfinite(y[i]);
             }
-            odd = odd && sees && isfinite(sum);
+            odd = odd && sees;
+            const float most = sum > 0.f ? mx : -INFINITY;
             if (store) {
                 if (a.vec)
 #pragma unroll
@@ -349,7 +350,7 @@ __global__ void __launch_bounds__(PD_THREADS, PD_CTAS_PER_SM) paged_decode_kerne
                     const uint32_t r = 2 * warp + h, ft = r / shape.heads, fg = r % shape.heads;
                     const uint64_t fr = w.q.start + t0 + ft;
                     __syncwarp();
-                    paged_repair<T>(a, PD_KT, w.request, kv_head, w.span, p_lo + (int32_t)ft, __shfl_sync(0xffffffffu, mx, 16 * h), a.q + fr * a.q_stride + (uint64_t)(head0 + fg) * HS,
+                    paged_repair<T>(a, PD_KT, w.request, kv_head, w.span, p_lo + (int32_t)ft, __shfl_sync(0xffffffffu, most, 16 * h), a.q + fr * a.q_stride + (uint64_t)(head0 + fg) * HS,
                                     a.out + fr * a.out_stride + (uint64_t)(head0 + fg) * HS, HS);
                 }
         }

@@ -376,6 +376,44 @@ def test_a_wait_that_gave_up_leaves_no_arrivals_for_later_launches(hs):
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 @pytest.mark.parametrize("hs", [64, 128])
+@pytest.mark.parametrize("new", [1, 2, 3, 40, 300])
+def test_infinities_in_keys(backend, hs, new, dtype):
+    """A key with an infinite element gives a score of an infinity, by the sign of q's: weight 0 for rows where that is negative, no number for the others; for both signs in a key, none either.  The
+    elements of q are of any size, so that the remainders that the kernels split off have either sign, or are 0."""
+    inf = float("inf")
+
+    def key(b, r, j, *elements):
+        k = b.rows[r][0][j].clone()
+        for at, value in elements:
+            k[at] = value
+        b.put(r, j, 0, k)
+
+    for cached, window, sinks in ((50, 0, 0), (700, 0, 0), (700, 90, 3)):
+        b = Batch([cached, 20, 20], [new, 1, 2], 8, 4, hs, dtype=dtype, seed=new + cached)
+        b.q[:, ::3] = b.q[:, ::3].half().float()   # (no remainder)
+        b.q[:, 1::7] *= 1e-6
+        key(b, 0, cached - 3, (3, inf))                       # the first kv head's
+        key(b, 0, cached - 40, (hs + 5, -inf), (hs + 7, 2.0))   # the second one's
+        key(b, 0, 1, (0, -inf))
+        key(b, 1, 0, (hs - 1, inf))
+        key(b, 2, 7, (9, -inf), (hs + 30, inf))
+        if new > 1:
+            key(b, 0, cached + new // 2, (2 * hs - 1, inf))
+        b.check(backend, window, sinks)
+        assert torch.isfinite(b.out).any() and torch.isnan(b.out).any()
+        key(b, 0, cached - 3, (4, -inf))                      # both signs, mostly
+        b.put(0, cached - 5, 1, inf)                          # and an infinite value next to it
+        b.put(2, 7, 1, float("nan"))                          # at a weight of 0, or beside a score that is none: none
+        b.check(backend, window, sinks)
+    # no key but such: nothing to weigh
+    b = Batch([0], [new], 8, 4, hs, dtype=dtype, seed=new)
+    for j in range(new):
+        key(b, 0, j, (6, inf), (hs + 6, -inf))
+    b.check(backend)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("hs", [64, 128])
 @pytest.mark.parametrize("new,kv", [(3, 2), (6, 2), (40, 11), (300, 290), (300, 1)])
 def test_rows_that_see_nothing_beside_values_that_are_no_numbers(backend, hs, new, kv, dtype):
     """Tokens ahead of position 0 get 0, also where rows of K and V that the tile's other tokens see hold anything."""
