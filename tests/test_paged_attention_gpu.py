@@ -425,3 +425,23 @@ def test_rows_that_see_nothing_beside_values_that_are_no_numbers(backend, hs, ne
     b.out.fill_(5.0)
     b.run(backend)
     assert (b.out[: new - kv] == 0).all() and torch.isnan(b.out[new - kv:]).all()
+
+
+@pytest.mark.parametrize("hs", [64, 128])
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("bits", [0x7F800001, 0x7F801FFF, 0x7FC00000, 0x7FFFFFFF, -0x007FFFFF, -0x007FE001, -1])
+def test_nan_of_any_payload_in_a_32_bit_cache(backend, hs, which, bits):
+    """A NaN is one also where its payload is in the bits that tf32 does not hold: the rows that see it are NaN (of V: in its element), the others are as without it."""
+    for new in (1, 2, 40):
+        b = Batch([300], [new], 8, 4, hs, dtype=torch.float32, seed=new)
+        clean = b.run(backend).clone()
+        at = 300 + new // 2
+        (b.kc, b.vc)[which].view(torch.int32)[b.table[0, at // 16].item(), at % 16, hs + 9] = bits   # the second kv head's
+        got = b.run(backend).view(new, 8, hs)
+        nan = torch.zeros_like(got, dtype=torch.bool)
+        if which == 0:
+            nan[new // 2:, 4:] = True
+        else:
+            nan[new // 2:, 4:, 9] = True
+        assert torch.equal(torch.isnan(got), nan)
+        assert (got - clean.view(new, 8, hs))[~nan].abs().max() <= 1e-5   # (rows done again are in another order)
