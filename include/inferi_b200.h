@@ -200,7 +200,7 @@ typedef struct ib_paged_cache {
  * row of the table (INVALID; kv_len 0, and it returns no pages), a table row too short for the new tokens (TABLE_FULL), more tokens than max_tokens together with the requests before it
  * (NO_ROOM), more pages than are free together with those before it (NO_PAGES); once one does not fit, none behind it that needs the same does.  A page
  * belongs to one request.  A page number outside the cache is never followed: its slots are -1.
- * n_requests <= 8192. */
+ * n_requests <= 8192; of 0 requests there are no arrays of their own, and all rows are rows behind the last one. */
 enum { IB_PLAN_OK = 0, IB_PLAN_NO_PAGES = 1, IB_PLAN_TABLE_FULL = 2, IB_PLAN_NO_ROOM = 3, IB_PLAN_INVALID = 4 };
 typedef struct ib_page_plan_args {
     uint32_t n_requests, max_pages, max_tokens, n_pages, page_size;

@@ -152,8 +152,8 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(const ib_page_plan_a
         const uint32_t add = (uint32_t)R[i].tokens_end - tokens_before(i);
         p.kv_len[i] = R[i].cached + (int32_t)add;
         p.row_start[i + 1] = R[i].tokens_end;
-        if (i == 0) p.row_start[0] = 0;
     }
+    if (worker == 0) p.row_start[0] = 0;
     for (uint32_t g = worker; g < (uint32_t)takens; g += workers) {   // a thread per page: chunks of a prompt need many
         const uint32_t i = owner(&PlanRequest::need_before, g);
         p.block_table[(size_t)i * width + (uint32_t)pages_of(R[i].cached) + (g - R[i].need_before)] = stack((uint32_t)size - 1 - g);
@@ -347,9 +347,9 @@ int32_t ib_page_plan(ib_ctx *ctx, void *stream, const ib_page_plan_args *args) {
     IB_REQUIRE(a.page_size >= 16 && a.page_size <= 1024 && (a.page_size & (a.page_size - 1)) == 0, "ib_page_plan: page_size=%u must be a power of two from 16 to 1024", a.page_size);
     IB_REQUIRE(a.n_pages >= 1 && (uint64_t)a.n_pages * a.page_size < (1ull << 31), "ib_page_plan: %u pages of %u positions (1 to 2^31 - 1 slots)", a.n_pages, a.page_size);
     IB_REQUIRE(a.max_pages >= 1 && (uint64_t)a.max_pages * a.page_size < (1ull << 31), "ib_page_plan: rows of %u pages of %u positions (1 to 2^31 - 1 positions)", a.max_pages, a.page_size);
-    IB_REQUIRE(a.n_requests >= 1 && a.n_requests <= PLAN_MAX_REQUESTS, "ib_page_plan: %u requests (1 to %u)", a.n_requests, PLAN_MAX_REQUESTS);
+    IB_REQUIRE(a.n_requests <= PLAN_MAX_REQUESTS, "ib_page_plan: %u requests (up to %u)", a.n_requests, PLAN_MAX_REQUESTS);
     IB_REQUIRE(a.max_tokens >= 1 && a.max_tokens < (1u << 31), "ib_page_plan: room for %u tokens (1 to 2^31 - 1)", a.max_tokens);
-    IB_REQUIRE(a.cached_len && a.new_len && a.n_free && a.block_table && a.free_pages && a.kv_len && a.row_start && a.positions && a.slots && a.n_free_out && a.status,
+    IB_REQUIRE(a.n_free && a.free_pages && a.row_start && a.positions && a.slots && a.n_free_out && (a.n_requests == 0 || (a.cached_len && a.new_len && a.block_table && a.kv_len && a.status)),
                "ib_page_plan: null array");
     static bool attr_set[16] = {false};
     const bool beyond = ctx->device >= 16;

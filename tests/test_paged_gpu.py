@@ -335,3 +335,10 @@ def test_plan_writes_its_rows_and_no_others(backend, offset, room):
 @pytest.mark.parametrize("hs,heads,kv_heads,n", [(64, 4, 2, 1776), (64, 4, 2, 1777), (128, 3, 3, 2500), (8, 40, 2, 2000)])
 def test_append_of_more_rows_than_have_a_place_together(backend, variant, dtype, hs, heads, kv_heads, n):
     check_append(backend, variant, hs, heads, kv_heads, n, 32, dtype, 2000)
+
+
+def test_plan_of_no_requests(backend):
+    """A server's step without any: no tokens, and the stack as it was."""
+    for room, in_place in ((1, False), (9, True), (5000, False)):
+        got = run_plan(backend, 16, [], [], np.zeros((0, 3)), np.arange(7), 5, room, in_place)
+        assert list(got["starts"]) == [0] and (got["positions"] == 0).all() and (got["slots"] == -1).all() and got["n_free"] == 5 and list(got["free"]) == list(range(7))
