@@ -445,3 +445,52 @@ def test_nan_of_any_payload_in_a_32_bit_cache(backend, hs, which, bits):
             nan[new // 2:, 4:, 9] = True
         assert torch.equal(torch.isnan(got), nan)
         assert (got - clean.view(new, 8, hs))[~nan].abs().max() <= 1e-5   # (rows done again are in another order)
+
+
+LONG = [(5000, 1, 128), (12000, 1, 16), (17000, 9, 256), (3000, 300, 16), (6000, 40, 32)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("hs", [64, 128])
+@pytest.mark.parametrize("cached,new,P", LONG)
+def test_rows_of_long_requests_by_their_own_size(backend, cached, new, P, hs, dtype):
+    """Every row's error by its own norm.  A score is off by the 2^-22 of q's split and by hs / 8 truncations of two products, 2^-23 each, of partial sums that are of its own size (1 here, 4 at most):
+    2e-6 where all go one way; what all of a row's scores have in common cancels, and what they do not adds up as the row's own elements do.  Twice that for the sums.  (A product without its remainder is
+    off by 2^-12 of a score's terms.)"""
+    b = Batch([cached, 700], [new, 1], 8, 4, hs, P=P, dtype=dtype, seed=cached + new)
+    for window, sinks in ((0, 0), (2500, 130)):
+        b.run(backend, window, sinks)
+        want = b.exact(0, window, sinks)[0].view(new, 8, hs)
+        off = (b.out[:new].view(new, 8, hs).double() - want).norm(dim=-1) / want.norm(dim=-1)
+        assert off.max() <= 4e-6, f"off by {float(off.max()):.2e} of a row's norm"
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("hs", [64, 128])
+@pytest.mark.parametrize("cached,new,P,window,sinks", [c + (0, 0) for c in LONG] + [(0, 700, 64, 0, 0), (4000, 1, 64, 1100, 70), (3000, 260, 16, 900, 200)])
+def test_every_position_counts_once(backend, cached, new, P, window, sinks, hs, dtype):
+    """Values that are 1 in a column of their own for a position each, and 0 otherwise: the result is the weights, one by one, at every border of ranges, tiles and pages.  The bound is that of a weight in
+    `Batch.exact`, relative to itself, and half a step of the remainders of f16 (2^-24 of 2^14 times the largest weight)."""
+    b = Batch([cached, 70], [new, 1], 8, 4, hs, P=P, dtype=dtype, seed=cached + new + window)
+    kv = cached + new
+    k = b.rows[0][0].double().view(kv, 2, hs)
+    q = b.q[:new].double().view(new, 2, 4, hs)
+    s = torch.einsum("nhgd,khd->nhgk", q, k) / math.sqrt(hs)
+    p, j = torch.arange(cached, kv, device="cuda")[:, None, None, None], torch.arange(kv, device="cuda")
+    seen = (j <= p) & ((p - j < window) | (j < sinks)) if window else j <= p
+    w = torch.where(seen, s, -math.inf).softmax(-1)
+    A = float(torch.einsum("nhgd,khd->nhgk", q.abs(), k.abs()).max()) / math.sqrt(hs)
+    tol = 2 * A * (hs / 8 + 4) * 2**-23 + (8 + kv / 16) * 2**-23
+    pages = b.table[0, : -(-kv // P)].long()
+    for first in range(0, kv, 2 * hs):
+        values = torch.zeros(len(pages) * P, 2, hs, dtype=dtype, device="cuda")
+        at = torch.arange(2 * hs, device="cuda")
+        at = at[first + at < kv]
+        values[first + at, at // hs, at % hs] = 1.0
+        values[kv:] = float("nan")
+        b.vc[pages] = values.view(len(pages), P, 2 * hs)
+        b.run(backend, window, sinks)
+        got = b.out[:new].view(new, 2, 4, hs).double().permute(0, 2, 1, 3).reshape(new, 4, 2 * hs)[..., : len(at)]
+        want = torch.stack([w[:, h // hs, :, first + h] for h in range(len(at))], -1)
+        off = (got - want).abs() - tol * want - torch.where(want > 0, 2.0**-38, 0.0) * w.amax()
+        assert off.max() <= 0, f"position {first + int(off.amax((0, 1)).argmax())}"
