@@ -231,6 +231,8 @@ IB_API int32_t ib_paged_append(ib_ctx *ctx, void *stream, const ib_paged_append_
  * head h / kv_mul.  head_size 64 or 128; kv_mul up to 64; kv_dim of the cache = n_heads / kv_mul * head_size.  Rows of q and out are *_stride floats apart; rows
  * behind row_start[n_requests] are neither read nor written, and out does not overlap q (out = q is refused).  Masked positions and rows of pages behind kv_len may hold anything, infinities and NaN too.
  * A page number outside the cache is never followed; what the rows of that request get then is not specified.
+ * Rows that see something that is no finite number are done again position by position: where a whole chunk behind more than 400,000 positions does, that takes longer than the default limit
+ * of ib_ctx_set_wait_limit, and the launch gives up.
  * longest_new: the most new tokens that a request has, where the host knows it, else 0.  It chooses kernels, and any value gives right results. */
 typedef struct ib_paged_attn_args {
     const float *q_dev;

@@ -334,71 +334,123 @@ __device__ __forceinline__ int paged_exponent(float most) {
 // NaN where the score is an infinity.  So a row that sees something and has such a result, or no sum of weights, is computed anew, position by position and in one product each: a score of -infinity weighs
 // nothing, one that is NaN or infinity makes all of the row NaN, and so do scores that are all -infinity.
 // most: the row's largest score (rounded up, in units of log2), -infinity where the sum of weights says that it is not known.  Called by a whole warp.
-template <typename T>
-static __device__ __noinline__ void paged_repair(const PagedAttn &a, uint32_t KT, uint32_t request, uint32_t kv_head, const KeySpan span, int32_t p, float most, const float *q, float *out, uint32_t hs) {
-    const uint32_t lane = threadIdx.x & 31, E = hs / 32;
-    const float scale = 1.4426950408889634f / sqrtf((float)hs);
-    // a position's row of the cache, or ~0 where it is not seen; its score
-    auto place = [&](uint32_t j) {
-        if (j >= span.end || !paged_sees(a, p, j)) return ~0ull;
-        const int32_t page = a.table[(size_t)request * a.max_pages + (j >> a.page_log2)];
-        if (page < 0 || (uint32_t)page >= a.n_pages) return ~0ull;
-        return (unsigned long long)page * a.page_stride + (unsigned long long)(j & ((1u << a.page_log2) - 1)) * a.kv_dim + kv_head * hs;
-    };
-    auto score = [&](unsigned long long at) {
-        constexpr uint32_t N = 16 / sizeof(T);
-        float s = 0.f;
-#pragma unroll 2
-        for (uint32_t e = 0; e < hs; e += N) {
-            const uint4 piece = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.k) + at + e));
-            const T *k = reinterpret_cast<const T *>(&piece);
+// 8 positions at a time, of 32 which lie in two pages at most: a lane has HS / 32 columns of each row of K, the sums over the lanes are formed for all 8 together (9 exchanges), which leaves four lanes each
+// the score of a position; then the weights are handed round, and a lane adds up its columns of V.  (More at a time takes registers, which the callers' own loops pay for.)
+// L2's bandwidth bounds it where all rows of many tiles are done again: 2400 tokens after 40,000, 32 heads of 128: 410 ms, 0.2 s for a tile's 256 rows (a position per lane: 905); one token after 40,000: 14 ms.
+// Of more than 400,000 positions a chunk's tile takes longer than the 2 s that the warps of its CTA wait for it by default, and the launch gives up.
+template <uint32_t E>
+__device__ __forceinline__ void paged_elements(const __half *from, float (&x)[E]) {
+    uint32_t w[E / 2];
+    if constexpr (E == 4) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(from));
+        w[0] = v.x; w[1] = v.y;
+    } else w[0] = __ldg(reinterpret_cast<const uint32_t *>(from));
 #pragma unroll
-            for (uint32_t i = 0; i < N; i++) s += q[e + i] * (float)k[i];
+    for (uint32_t e = 0; e < E; e += 2) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[e / 2]));
+        x[e] = f.x; x[e + 1] = f.y;
+    }
+}
+template <uint32_t E>
+__device__ __forceinline__ void paged_elements(const float *from, float (&x)[E]) {
+#pragma unroll
+    for (uint32_t e = 0; e < E; e += 2) {
+        const float2 f = __ldg(reinterpret_cast<const float2 *>(from + e));
+        x[e] = f.x; x[e + 1] = f.y;
+    }
+}
+template <typename T, uint32_t HS>
+__device__ __forceinline__ void paged_repair(const PagedAttn &a, uint32_t KT, uint32_t request, uint32_t kv_head, const KeySpan span, int32_t p, float most, const float *q, float *out) {
+    constexpr uint32_t E = HS / 32;
+    const uint32_t lane = threadIdx.x & 31, column = lane * E, kv_dim = a.kv_dim;
+    const float scale = 1.4426950408889634f / sqrtf((float)HS);
+    const T *k = static_cast<const T *>(a.k) + kv_head * HS + column, *v = static_cast<const T *>(a.v) + kv_head * HS + column;
+    const int32_t *table = a.table + (size_t)request * a.max_pages;
+    float qr[E];
+#pragma unroll
+    for (uint32_t e = 0; e < E; e++) qr[e] = q[column + e];
+    unsigned long long row0 = 0, row1 = 0;   // of 32 positions: the first and the 17th one's (of pages that are none: the cache's first)
+    uint32_t mask = 0;                    // which of them are seen
+    auto score = [&](uint32_t g) {        // of position 8 g + lane / 4 of those
+        const T *from = k + (g < 2 ? row0 : row1) + (unsigned long long)(g % 2 * 8) * kv_dim;
+        float s[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            float x[E];
+            paged_elements(from + (unsigned long long)i * kv_dim, x);
+            s[i] = qr[0] * x[0];
+#pragma unroll
+            for (uint32_t e = 1; e < E; e++) s[i] += qr[e] * x[e];
         }
-        return s;
+#pragma unroll
+        for (uint32_t o = 4; o; o >>= 1)
+#pragma unroll
+            for (uint32_t i = 0; i < o; i++) {
+                const bool upper = lane & (4 * o);
+                const float send = upper ? s[i] : s[i + o], keep = upper ? s[i + o] : s[i];
+                s[i] = keep + __shfl_xor_sync(0xffffffffu, send, 4 * o);
+            }
+        s[0] += __shfl_xor_sync(0xffffffffu, s[0], 2);
+        s[0] += __shfl_xor_sync(0xffffffffu, s[0], 1);
+        return mask >> (8 * g + lane / 4) & 1 ? s[0] : -INFINITY;
     };
-    auto positions = [&](auto body) {   // a lane's in turn; false: enough
+    auto positions = [&](auto body) {   // 8 at a time; false: enough
         for (uint32_t u = 0; u < span.units; u++)
-            for (uint32_t j0 = key_tile(span, u) * KT; j0 < min(key_tile(span, u) * KT + KT, span.end); j0 += 32)
-                if (!body(place(j0 + lane))) return;
+            for (uint32_t j0 = key_tile(span, u) * KT; j0 < min(key_tile(span, u) * KT + KT, span.end); j0 += 32) {
+                const uint32_t j = j0 + lane;
+                const int32_t page = j < span.end ? table[j >> a.page_log2] : -1;
+                const bool there = page >= 0 && (uint32_t)page < a.n_pages;
+                const unsigned long long at = there ? (unsigned long long)page * a.page_stride + (unsigned long long)(j & ((1u << a.page_log2) - 1)) * kv_dim : 0ull;
+                row0 = __shfl_sync(0xffffffffu, at, 0);
+                row1 = __shfl_sync(0xffffffffu, at, 16);
+                mask = __ballot_sync(0xffffffffu, there && paged_sees(a, p, j));
+#pragma unroll 1
+                for (uint32_t g = 0; g < 4; g++)
+                    if ((mask >> 8 * g & 0xFFu) && !body(g)) return;
+            }
     };
     if (most == -INFINITY) {
         float top = -INFINITY;
         bool some = false, none = false;   // sees something; has a score that is none
-        positions([&](unsigned long long at) {
-            const float s = at != ~0ull ? score(at) : -INFINITY;
-            some = some || at != ~0ull;
+        positions([&](uint32_t g) {
+            const float s = score(g);
+            some = true;
             none = __any_sync(0xffffffffu, !(s < INFINITY));
             top = fmaxf(top, s);
             return !none;
         });
 #pragma unroll
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        some = __any_sync(0xffffffffu, some);
         if (none || top == -INFINITY) {
-            for (uint32_t e = 0; e < E; e++) out[lane + 32 * e] = some ? NAN : 0.f;   // (nothing: pages outside the cache)
+#pragma unroll
+            for (uint32_t e = 0; e < E; e++) out[column + e] = some ? NAN : 0.f;   // (nothing: pages outside the cache)
             return;
         }
         most = ceilf(top * scale);
     }
-    float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    positions([&](unsigned long long at) {   // its weight, then everybody's elements of all 32
-        float x = 0.f;
-        if (at != ~0ull) {
-            const float s = score(at);
-            x = s == -INFINITY ? 0.f : fmaxf(paged_ex2(s * scale - most), 1e-38f);   // (not nothing: an infinity that is seen counts, however small its weight)
-        }
-#pragma unroll 4
-        for (int i = 0; i < 32; i++) {
-            const unsigned long long from = __shfl_sync(0xffffffffu, at, i);
-            const float y = __shfl_sync(0xffffffffu, x, i);
-            if (from == ~0ull) continue;
-            l += y;
-            for (uint32_t e = 0; e < E; e++) acc[e] += y * (float)static_cast<const T *>(a.v)[from + lane + 32 * e];
+    float l = 0.f, acc[E];
+#pragma unroll
+    for (uint32_t e = 0; e < E; e++) acc[e] = 0.f;
+    positions([&](uint32_t g) {
+        const float s = score(g);
+        const uint32_t seen = mask >> 8 * g;
+        const float w = !(seen >> lane / 4 & 1) || s == -INFINITY ? 0.f : fmaxf(paged_ex2(s * scale - most), 1e-38f);   // (not nothing: an infinity that is seen counts, however small its weight)
+        const T *from = v + (g < 2 ? row0 : row1) + (unsigned long long)(g % 2 * 8) * kv_dim;
+        l += w;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            float x[E];
+            paged_elements(from + (unsigned long long)i * kv_dim, x);
+            const float wi = __shfl_sync(0xffffffffu, w, 4 * i);
+#pragma unroll
+            for (uint32_t e = 0; e < E; e++) acc[e] += seen >> i & 1 ? wi * x[e] : 0.f;
         }
         return true;
     });
-    for (uint32_t e = 0; e < E; e++) out[lane + 32 * e] = acc[e] / l;
+#pragma unroll
+    for (int o = 16; o > 2; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);   // (four lanes have the same)
+#pragma unroll
+    for (uint32_t e = 0; e < E; e++) out[column + e] = acc[e] / l;
 }
 
 // paged_decode.cu

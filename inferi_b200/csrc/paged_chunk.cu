@@ -127,12 +127,29 @@ __device__ __forceinline__ bool pc_wait(uint32_t bar, uint32_t parity, const Pag
 // moves every operand of every MMA over by itself (70 clocks an MMA instead of 20).
 __device__ __forceinline__ uint32_t pc_uniform(uint32_t x) { return __reduce_or_sync(0xffffffffu, x); }
 
-// A half that gave up arrives at the tiles that it would still have had a part of, from the one that it was at on (it gives up before it arrives there): the counters are zero again when the launch
-// ends, whoever gave up, and launches that follow, replayed ones too, find their last arrivals where they are.  Called by a warp.
-static __device__ __noinline__ void pc_arrive_at_rest(const PagedAttn &a, const TileShape &shape, const PcShared &S, uint32_t half) {
+// The CTA's range, as far as places and arrivals go, while registers have other things to hold
+__device__ __forceinline__ PagedRange pc_range(const PcShared &S) {
     PagedRange range = {};
     range.total = S.range.sum[0];
     range.length = S.range.sum[1];
+    return range;
+}
+// Rows `who` of a warp's 32 of the kept walk's tile, anew.  (A call that needs nothing of its caller's registers: the loops around it would pay for each.)
+template <int HS>
+static __device__ __noinline__ void pc_repair(const PagedAttn &a, const TileShape &shape, const PcShared &S, uint32_t half, uint32_t first, uint32_t who, int32_t p, float m) {
+    const PagedWalk<PC_KT> &w = S.walk[half];
+    for (; who; who &= who - 1) {
+        const int b = __ffs(who) - 1;
+        const uint32_t at = first + b, token = at / a.kv_mul;
+        if (token >= shape.tokens || w.tile * shape.tokens + token >= w.q.n) break;
+        const uint64_t q_row = w.q.start + w.tile * shape.tokens + token, from = (uint64_t)(w.group * a.kv_mul + at - token * a.kv_mul) * HS;
+        paged_repair<__half, HS>(a, PC_KT, w.request, w.group, w.span, __shfl_sync(0xffffffffu, p, b), __shfl_sync(0xffffffffu, m, b), a.q + q_row * a.q_stride + from, a.out + q_row * a.out_stride + from);
+    }
+}
+// A half that gave up arrives at the tiles that it would still have had a part of, from the one that it was at on (it gives up before it arrives there): the counters are zero again when the launch
+// ends, whoever gave up, and launches that follow, replayed ones too, find their last arrivals where they are.  Called by a warp.
+static __device__ __noinline__ void pc_arrive_at_rest(const PagedAttn &a, const TileShape &shape, const PcShared &S, uint32_t half) {
+    const PagedRange range = pc_range(S);
     PagedWalk<PC_KT> w = S.walk[half];
     do {
         if (w.whole() || (half == 1 && min(shape.tokens, w.q.n - w.tile * shape.tokens) * a.kv_mul <= 128)) continue;
@@ -156,7 +173,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
     const PagedRange range = paged_range<PC_KT, PC_THREADS, true>(a, shape, S.range);
     if (range.total == 0 || blockIdx.x >= range.ranges) return;
     if (warp == 0 && lane == 0) {
-        S.range.sum[0] = range.total;   // (nobody reads these any more, but who leaves early)
+        S.range.sum[0] = range.total;   // (free from here on: pc_range)
         S.range.sum[1] = range.length;
         for (uint32_t i = 0; i < SLOTS; i++) {
             pg_bar_init(b_full + 8 * i, 1);
@@ -373,6 +390,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
             // ---- the half's result, or its part of it ----
             bool finish = w.whole();
             if (!finish) {
+                const PagedRange range = pc_range(S);
                 const uint32_t c0 = range.range_of(w.tile_unit()), c1 = range.range_of(w.tile_unit() + w.span.units - 1);
                 float *part = a.scratch + ((size_t)paged_place(range, w.tile_unit(), blockIdx.x) * 2 + half) * pc_partial_floats(HS);
 #pragma unroll
@@ -432,14 +450,9 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_chunk_kernel(const __grid
                 for (uint32_t i = 0; i < 8; i++) any |= S.odd[half][i >> 2][i & 3];
                 if (any) {
                     pc_sync_half(half);   // (the rows are stored)
-                    for (uint32_t who = (mine | S.odd[half][side ^ 1][warp & 3]) & (side ? 0xFFFF0000u : 0xFFFFu); who; who &= who - 1) {   // (the two warps of the rows share them)
-                        const int b = __ffs(who) - 1;
-                        const uint32_t at = 128 * half + 32 * (warp & 3) + b, token = token_of(at);
-                        if (token >= shape.tokens || w.tile * shape.tokens + token >= w.q.n) break;
-                        const uint64_t q_row = w.q.start + w.tile * shape.tokens + token, from = (uint64_t)(w.group * a.kv_mul + at - token * a.kv_mul) * HS;
-                        paged_repair<__half>(a, PC_KT, w.request, w.group, w.span, __shfl_sync(0xffffffffu, p, b), __shfl_sync(0xffffffffu, m, b), a.q + q_row * a.q_stride + from,
-                                             a.out + q_row * a.out_stride + from, HS);
-                    }
+                    // (the two warps of the rows share them)
+                    pc_repair<HS>(a, shape, S, half, 128 * half + 32 * (warp & 3), (mine | S.odd[half][side ^ 1][warp & 3]) & (side ? 0xFFFF0000u : 0xFFFFu), p, m);
+                    unpark();
                 }
             }
             pc_sync_half(half);   // (what is shared may be written again)

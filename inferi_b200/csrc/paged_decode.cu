@@ -57,6 +57,13 @@ __device__ __forceinline__ void pd_cut_tf32(uint32_t x, uint32_t &hi, uint32_t &
 __device__ __forceinline__ uint4 pd_load(const void *p) { return __ldcg(reinterpret_cast<const uint4 *>(p)); }
 __device__ __forceinline__ uint32_t pd_word(const uint4 &v, int i) { return i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w)); }
 
+// A call, so that what it takes in registers is not the loop's
+template <typename T, uint32_t HS>
+static __device__ __noinline__ void pd_repair(const PagedAttn &a, uint32_t request, uint32_t kv_head, uint32_t sink_tiles, uint32_t first, uint32_t units, uint32_t end, int32_t p, float most, uint32_t row,
+                                              uint32_t head) {
+    paged_repair<T, HS>(a, PD_KT, request, kv_head, {sink_tiles, first, units, end}, p, most, a.q + row * a.q_stride + head * HS, a.out + row * a.out_stride + head * HS);
+}
+
 constexpr uint32_t pd_partial_floats(uint32_t hs) { return PD_ROWS * (hs + 2); }
 constexpr uint32_t PD_CTAS_PER_SM = 3;   // (32-bit, with two of 237 registers a thread: 140 us instead of 133, see above)
 
@@ -349,14 +356,13 @@ __global__ void __launch_bounds__(PD_THREADS, PD_CTAS_PER_SM) paged_decode_kerne
                     for (int i = 0; i < D; i++) out[d0 + i] = y[i];
             }
             const uint32_t rows = __ballot_sync(0xffffffffu, odd && store);   // of the warp's two
-#pragma unroll
+#pragma unroll 1
             for (uint32_t h = 0; h < 2; h++)
                 if (rows & (0xFFFFu << (16 * h))) {
                     const uint32_t r = 2 * warp + h, ft = r / shape.heads, fg = r % shape.heads;
-                    const uint64_t fr = w.q.start + t0 + ft;
                     __syncwarp();
-                    paged_repair<T>(a, PD_KT, w.request, kv_head, w.span, p_lo + (int32_t)ft, __shfl_sync(0xffffffffu, most, 16 * h), a.q + fr * a.q_stride + (uint64_t)(head0 + fg) * HS,
-                                    a.out + fr * a.out_stride + (uint64_t)(head0 + fg) * HS, HS);
+                    pd_repair<T, HS>(a, w.request, kv_head, w.span.sink_tiles, w.span.first, w.span.units, w.span.end, p_lo + (int32_t)ft, __shfl_sync(0xffffffffu, most, 16 * h),
+                                     w.q.start + t0 + ft, head0 + fg);
                 }
         }
         __syncthreads();   // shared memory is used again

@@ -494,3 +494,22 @@ def test_every_position_counts_once(backend, cached, new, P, window, sinks, hs, 
         want = torch.stack([w[:, h // hs, :, first + h] for h in range(len(at))], -1)
         off = (got - want).abs() - tol * want - torch.where(want > 0, 2.0**-38, 0.0) * w.amax()
         assert off.max() <= 0, f"position {first + int(off.amax((0, 1)).argmax())}"
+
+
+def test_infinities_in_a_long_prompt(backend):
+    """Every row of a chunk behind 260,000 positions sees an infinity, so each is done again: 256 of them, while other warps of the CTA wait for the next tile, take two thirds of the waits' limit."""
+    b = Batch([260000], [2400], 32, 4, 128, P=256)
+    clean = b.run(backend).clone()
+    k, v = (b.rows[0][which][at].clone() for which, at in ((0, 250000), (1, 5)))
+    b.put(0, 5, 1, float("inf"))
+    odd = k.clone()
+    odd[130] = -float("inf")   # a score of an infinity for the second kv head: weight 0, or no number
+    b.put(0, 250000, 0, odd)
+    b.run(backend)
+    assert backend.lib.ib_stream_sync(backend.handle, torch.cuda.current_stream().cuda_stream) == 0
+    out, lost = b.out.view(2400, 32, 128), b.q.view(2400, 32, 128)[:, 4:8, 2] < 0
+    assert torch.isposinf(out[:, :4]).all() and torch.isposinf(out[:, 8:]).all()
+    assert torch.isnan(out[:, 4:8][lost]).all() and torch.isposinf(out[:, 4:8][~lost]).all() and lost.any() and (~lost).any()
+    b.put(0, 5, 1, v)
+    b.put(0, 250000, 0, k)
+    assert torch.equal(b.run(backend), clean)
