@@ -88,6 +88,11 @@ class Backend:
         IB_ERR_TIMEOUT (default 2 s).  Applies to launches issued, and token graphs recorded, after the call."""
         check(self.lib.ib_ctx_set_wait_limit(self.handle, int(nanoseconds)))
 
+    def synchronize(self) -> None:
+        """Waits for the device's current stream, and says (IB_ERR_TIMEOUT) whether a kernel of this context gave up waiting since
+        the last time: torch's own synchronisation does not know."""
+        check(self.lib.ib_stream_sync(self.handle, _stream_of(self)))
+
     def close(self) -> None:
         if getattr(self, "handle", None):
             self.lib.ib_ctx_destroy(self.handle)

@@ -513,3 +513,23 @@ def test_infinities_in_a_long_prompt(backend):
     b.put(0, 5, 1, v)
     b.put(0, 250000, 0, k)
     assert torch.equal(b.run(backend), clean)
+
+
+def test_synchronize_says_that_a_launch_gave_up():
+    own = Backend(0)
+    own.synchronize()
+    b = Batch([3000], [4100], 16, 4, 64, P=64)
+    b.put(0, 5, 1, float("inf"))
+    own.set_wait_limit(300_000)
+    b.run(own)
+    with pytest.raises(InferiError) as e:
+        own.synchronize()
+    assert e.value.code == 5 and "gave up waiting" in e.value.message
+    own.synchronize()
+    own.set_wait_limit(2_000_000_000)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        b.run(own)
+        own.synchronize()
+        assert side.query()
+    own.close()
