@@ -255,7 +255,7 @@ IB_API int32_t ib_paged_attention(ib_ctx *ctx, void *stream, const ib_paged_attn
  *                 without a limit: the same in the order of indices.  (ib_sample's rules, where it offers the same.)
  *   prob          the token's share of what was left (1 for the arg-max).  May be NULL
  * Logits are not modified; NaN counts as -infinity, which is never drawn, and +infinity as the largest float; a row without a number gives token 0.  Sums are exact in units of 2^-44 of the
- * largest probability, and weights are good to 2^-31.  vocab up to 524288. */
+ * largest probability, and weights are whole units, one at least, good to 2^-31 and half a unit.  vocab up to 524288. */
 typedef struct ib_sample_batch_args {
     const float *logits_dev;
     uint64_t stride;

@@ -6,7 +6,7 @@ namespace ib {
 int32_t check_paged_cache(const char *who, const ib_paged_cache *c);   // paged.cu
 uint32_t log2_of(uint32_t power);
 
-// Rows (new tokens * kv_mul) up to which a request is the decode kernel's.  At 32 requests over 4000 positions the two take the same at 20 rows (head size 64: 125 us and 131, 128: 186 and 181);
+// Rows (new tokens * kv_mul) up to which a request is the decode kernel's.  At 32 requests over 4000 positions the two take the same at 20 rows (head size 64: 125 us and 131, 128: 187 and 181);
 // 16 rows 83 and 131, 117 and 181; 32 rows 155 and 132, 243 and 181.  One request alone is faster with the decode kernel (17 us and 28, 27 and 49 at 64 rows), until it is long: 249 us and 86 at 256 rows over 16,000 positions.
 constexpr uint32_t PAGED_FEW_ROWS = 24;
 

@@ -4,7 +4,8 @@
 // head g of token t.  A query tile is some tokens of a request with all heads of a group (TileShape); the positions it sees are cut into key tiles of KT.
 //
 // The units (request, head group, query tile, key tile), in that order, are cut into contiguous, equally long ranges, one per CTA of a grid that fills the GPU once, whatever
-// the requests' lengths: a batch of one long and many short requests needs no other treatment than one of equal ones.  A query tile whose key tiles fall to several CTAs gets a
+// the requests' lengths: the requests of a launch may be one long and many short ones, or equal ones.  (Requests with few new rows and those with many are two launches, one behind the other, each of which
+// walks over all of them: paged_attention.cu.)  A query tile whose key tiles fall to several CTAs gets a
 // partial (maximum, sum, accumulator) from each; a CTA has at most two such tiles, the one that its range begins in and the one that it ends in, so the scratch has
 // two places per CTA whatever the lengths.  The last CTA of a tile to arrive (an atomic counter; nobody waits) adds up the partials in the order of the CTAs: the result does not depend on who
 // was last.  Every CTA finds its range by itself from row_start and kv_len, by a sum over the requests: lengths never have to come to the host, and no launch ahead

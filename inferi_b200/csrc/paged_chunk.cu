@@ -8,7 +8,7 @@
 // q = hi + lo and P = hi + lo hold about 22 bits, K and V are exact, so the result is as good as 32-bit arithmetic makes it; each product is two MMAs.  The sums of a tile go from tensor
 // memory to registers before the next one's: the tensor core truncates, and a chain of its additions over a long context would shrink the result.  With whole numbers m rescaling is exact.
 //
-// What bounds it: the MMAs.  Twice 4 * 128 * 128 * HS operations per half and key tile are 2048 clocks (HS 128); the exponentials are 1024 of the SM's special function units, and the
+// What bounds it at head size 128: the MMAs, and what they wait for.  Twice 4 * 128 * 128 * HS operations per half and key tile are 2048 clocks (HS 128); the exponentials are 1024 of the SM's special function units, and the
 // remaining work of a thread's 128 scores about 1000.  The halves take turns: while one is in softmax, the tensor cores do the other's products.  Two halves share a key tile's 64 KB, 16
 // bytes a clock and SM; a tile of 128 rows would take twice as much from L2, which is all that L2 has.
 //
@@ -23,8 +23,9 @@
 // turns, and each waits for its operands while the other one's products run.  From a product with A in shared memory to one with A in tensor memory the tensor cores lose 215 clocks.
 // Tensor memory (512 columns): S0 / P0, S1 / P1, O0, O1 of 128 columns each.  P's operands are interleaved by 16 positions, hi then lo, so that a thread overwrites only scores that it has read.
 //
-// 1000 tokens after 15,000, 32 heads of 128, four to a kv head (254 GFLOP): 452 us, 0.56 PFLOP/s of results and 1.12 of products, two thirds of the measured 1.68; the SM clock is at 1.4 GHz then,
-// by the power limit.  7 chunks of 700 with a window of 1024 and 4 sinks, heads of 64: 130 us; there each CTA has a tile of 10 key tiles, and its start and end count.
+// 1000 tokens after 15,000, 32 heads of 128, four to a kv head (254 GFLOP): 451 us, 0.56 PFLOP/s of results and 1.12 of products, two thirds of the measured 1.68; the SM clock is at 1.4 GHz then,
+// by the power limit, and the tensor pipe busy for 56 % of the time.  7 chunks of up to 700 with a window of 1024 and 4 sinks, heads of 64: 132 us, 26 %; there the exponentials and the rest of softmax take as
+// long as the products, and each CTA has a tile of 10 key tiles, whose start and end count.
 //
 // Every wait for a copy or a product is bounded; a wait that gives up raises the context's error word, and the kernel returns after freeing its tensor memory.  Barriers are only waited at where all
 // who take part come: a half's warps leave as one, the remaining warps meet nobody until the end.

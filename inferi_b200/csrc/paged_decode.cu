@@ -14,8 +14,8 @@
 //   K   lane (n, c) = (lane / 4, lane % 4) has elements 32 i + 8 c .. + 7 of position n: of the i-th piece two MMAs' columns {2c, 2c+1, 2c+8, 2c+9}.  q's lanes hold the same elements.
 //   V   lane (n, c) has elements 64 i + 8 n .. + 7 of positions 2c, 2c + 1, 2c + 8, 2c + 9: MMA t of a piece makes the result's elements 64 i + 8 n + t, n = 0 .. 7,
 //       from pairs of positions that a byte permute puts together.  A lane's results are elements 64 i + 16 c .. + 15 of row n.
-// 64 requests over up to 8000 positions, 32 heads of 128, four to a kv head (1.57 GB): 248 us, 6.3 TB/s.  One over 500: 7.1 us, of which a launch is 2.5; the rest is the chain of lengths,
-// pages, K, softmax, V, arrival and merge.  24 requests with 5 tokens and 8 heads to a kv head over 3000 positions of a 32-bit cache (224 MB): 133 us: up to five
+// 64 requests over up to 8000 positions, 32 heads of 128, four to a kv head (1.57 GB): 250 us, 6.3 TB/s.  One over 500: 7.2 us, of which a launch is 2.5; the rest is the chain of lengths,
+// pages, K, softmax, V, arrival and merge.  24 requests with 5 tokens and 8 heads to a kv head over 3000 positions of a 32-bit cache (224 MB): 134 us: up to five
 // tiles of 8 rows read and cut every row again, and a warp's step is a chain (data, K's products, softmax, V's products) that 12 warps on an SM do not hide.
 // (32-bit: pieces of 4 elements, MMAs of 8 columns: K elements 16 i + 4 c .. + 3, V elements 32 i + 4 n .. + 3 of positions 2c, 2c + 1; results 32 i + 8 c .. + 7.)
 #include "paged_attention.cuh"
